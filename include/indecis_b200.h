@@ -321,6 +321,61 @@ IG_API int ig_attention(const float *qkv, int32_t hidden, int32_t heads, const i
 IG_API int ig_attention_noalloc(const float *qkv, int32_t hidden, int32_t heads, const int64_t *offs, int32_t nseq,
                                 int32_t window, int32_t simd_lanes, float *ctx, void *stream);
 
+/* ---- vocabulary operators (device pointers, enqueued on stream) ----
+ * Answers read as tokens of a vocabulary, and learning from a teacher that
+ * answers with one. The reference scores its own small heads only
+ * (heads.go:62-74) and distils pooled vectors (distill.go); these work on
+ * rows of logits over a whole vocabulary. Notation, for a row x of `vocab`
+ * logits: z = x / temperature, lse = log sum exp z, p = exp(z - lse).
+ * dtype is IG_DT_F32, IG_DT_BF16 or IG_DT_F16; sums and statistics are
+ * float32. Rows may start at any multiple of the element size (ld is in
+ * elements). At most IG_VOCAB_IDS_MAX ids per row and IG_VOCAB_TOP_MAX
+ * alternatives; rows <= 2^28, vocab <= 2^30. IG_ERR_BAD_ARG for null
+ * pointers, negative sizes, strides shorter than a row or a temperature that
+ * is not positive and finite, before any GPU work. */
+#define IG_VOCAB_IDS_MAX 256
+#define IG_VOCAB_TOP_MAX 32
+
+/* Log probabilities of given tokens, entropy and top alternatives:
+ * logprobs[r][t] = z[ids[r][t]] - lse, lse[r] and entropy[r] = -sum p log p
+ * (either may be NULL), top_ids/top_logprobs[r][top_k] the columns of the
+ * largest logits (ties: the lowest column first). A negative id is not given:
+ * 0. An id >= vocab gives NaN and device error 5. -inf masks a column. A row
+ * of -inf only: lse and logprobs -inf, entropy 0. Past the unmasked columns:
+ * alternative -1, -inf. A row with NaN or +inf: NaN (alternatives -1). */
+IG_API int ig_token_logprobs(const void *logits, int32_t dtype, int64_t ld, int64_t rows, int32_t vocab,
+                             double temperature, const int32_t *ids, int32_t nids, float *logprobs, float *lse,
+                             float *entropy, int32_t top_k, int32_t *top_ids, float *top_logprobs, void *stream);
+
+/* Gradient of the above from dlogprobs [rows][nids] and dentropy [rows]
+ * (NULL: none), with the forward's lse and entropy (entropy may be NULL
+ * without dentropy): dlogits[r][j] = (sum_t dlogprobs[t] (1[j = ids[t]] - p_j)
+ * - dentropy p_j (log p_j + entropy)) / temperature, rounded once to the
+ * logits' type. Repeated ids add up; ids outside the vocabulary give nothing.
+ * Zero for a row of -inf only. dlogits may be logits (with ldd = ld). */
+IG_API int ig_token_logprobs_backward(const void *logits, int32_t dtype, int64_t ld, int64_t rows, int32_t vocab,
+                                      double temperature, const int32_t *ids, int32_t nids, const float *lse,
+                                      const float *entropy, const float *dlogprobs, const float *dentropy,
+                                      void *dlogits, int64_t ldd, void *stream);
+
+/* Divergence of the rows from a teacher's top k entries, and its gradient in
+ * the same call. teacher_ids [rows][k], negative where a list is shorter.
+ * tail = 0: q = softmax(teacher_logits / temperature) over the list;
+ *   loss[r] = w sum q (log q - log p).
+ * tail != 0: teacher_logits are log probabilities, q = exp of them, and what
+ *   is left of 1 is one more outcome against the mass of p outside the list:
+ *   loss[r] = w (sum q (log q - log p) + q_rest (log q_rest - log p_rest))
+ *   (left out where the row has no unmasked column outside the list).
+ * w = weights[r] (NULL: 1), the row's share of the total: dlogits (NULL: loss
+ * only; may be logits, with ldd = ld) is the gradient of sum_r loss[r]. A row
+ * with weight 0 or without entries: loss 0 and gradient 0. A row of -inf
+ * only: loss +inf, gradient 0; one with NaN or +inf: NaN. vocab <= 2^20 with
+ * the tail (IG_ERR_UNSUPPORTED). Ids >= vocab count as missing and leave
+ * device error 5. */
+IG_API int ig_distill_topk(const void *logits, int32_t dtype, int64_t ld, int64_t rows, int32_t vocab,
+                           double temperature, const int32_t *teacher_ids, const float *teacher_logits, int32_t k,
+                           int32_t tail, const float *weights, float *loss, void *dlogits, int64_t ldd, void *stream);
+
 /* Per-layer intermediates of one ig_encode call, copied to host buffers for
  * parity checks (NULL fields are skipped). Layouts as the oracle's. */
 typedef struct ig_dump {

@@ -33,7 +33,8 @@ SYMBOLS = ["ig_model_create", "ig_model_destroy", "ig_model_set_heads", "ig_enco
            "ig_spans_tags_device", "ig_spans_tags", "ig_spans_from_tags", "ig_model_set_int8",
            "ig_check_gelu_division", "ig_model_create_multi", "ig_model_replica", "ig_model_device_count",
            "ig_model_create_stored", "ig_model_create_stored_multi", "ig_device_count", "ig_gemm_geglu_quant",
-           "ig_profile_only", "ig_check_wait_timeout"]
+           "ig_profile_only", "ig_check_wait_timeout", "ig_token_logprobs", "ig_token_logprobs_backward",
+           "ig_distill_topk"]
 
 IG_EMB_F32 = 0
 IG_EMB_BF16 = 1
@@ -194,6 +195,10 @@ def load() -> C.CDLL:
     L.ig_profile_only.argtypes = [C.c_char_p]
     L.ig_profile_report.argtypes = [C.c_char_p, C.c_size_t]
     L.ig_profile_report.restype = C.c_int64
+    i64 = C.c_int64
+    L.ig_token_logprobs.argtypes = [vp, i32, i64, i64, i32, f64, vp, i32, vp, vp, vp, i32, vp, vp, vp]
+    L.ig_token_logprobs_backward.argtypes = [vp, i32, i64, i64, i32, f64, vp, i32, vp, vp, vp, vp, vp, i64, vp]
+    L.ig_distill_topk.argtypes = [vp, i32, i64, i64, i32, f64, vp, vp, i32, i32, vp, vp, vp, i64, vp]
     _lib = L
     return L
 

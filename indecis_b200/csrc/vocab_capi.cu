@@ -1,0 +1,113 @@
+// C entry points of the vocabulary operators (vocab_rows.cu, vocab_gemm.cu).
+#include <cmath>
+#include <string>
+
+#include "common.cuh"
+#include "internal.h"
+
+namespace ig {
+
+static int vocab_elem_size(int dtype) {
+  return dtype == IG_DT_F32 ? 4 : dtype == IG_DT_BF16 || dtype == IG_DT_F16 ? 2 : 0;
+}
+
+// A matrix argument: rows x cols elements of es bytes, row stride ld.
+static const char *bad_matrix(const void *p, int64_t rows, int64_t cols, int64_t ld, int es) {
+  if (rows > 0 && !p) return "null argument";
+  if (ld < cols) return "row stride shorter than the row";
+  if (reinterpret_cast<uintptr_t>(p) % es) return "matrix not aligned to its element size";
+  return nullptr;
+}
+
+static const char *bad_row_args(int64_t rows, int64_t vocab, int32_t nids, const void *ids, const float *io, double t) {
+  if (rows < 0 || vocab < 1 || nids < 0) return "negative or empty size";
+  if (vocab > (1 << 30) || rows > (int64_t)INT32_MAX / 8) return "too many rows or columns";
+  if (nids > IG_VOCAB_IDS_MAX) return "too many given tokens per row";
+  if (rows > 0 && nids > 0 && (!ids || !io)) return "null argument";
+  if (!(t > 0.0) || !std::isfinite(t) || !std::isfinite((float)(1.0 / t)) || (float)(1.0 / t) <= 0.0f)
+    return "temperature must be positive and finite";
+  return nullptr;
+}
+
+}  // namespace ig
+
+using namespace ig;
+
+extern "C" {
+
+int ig_token_logprobs(const void *logits, int32_t dtype, int64_t ld, int64_t rows, int32_t vocab, double temperature,
+                      const int32_t *ids, int32_t nids, float *logprobs, float *lse, float *entropy, int32_t top_k,
+                      int32_t *top_ids, float *top_logprobs, void *stream) {
+  t_last_error.clear();
+  const int es = vocab_elem_size(dtype);
+  if (!es) return fail(IG_ERR_BAD_ARG, "ig_token_logprobs: dtype must be float32, bfloat16 or float16");
+  if (const char *m = bad_row_args(rows, vocab, nids, ids, logprobs, temperature))
+    return fail(IG_ERR_BAD_ARG, std::string("ig_token_logprobs: ") + m);
+  if (const char *m = bad_matrix(logits, rows, vocab, ld, es))
+    return fail(IG_ERR_BAD_ARG, std::string("ig_token_logprobs: ") + m);
+  if (top_k < 0 || top_k > IG_VOCAB_TOP_MAX)
+    return fail(IG_ERR_BAD_ARG, "ig_token_logprobs: top_k must be between 0 and 32");
+  if (rows > 0 && top_k > 0 && (!top_ids || !top_logprobs)) return fail(IG_ERR_BAD_ARG, "ig_token_logprobs: null argument");
+  if (rows == 0) return 0;
+  LogprobArgs a{logits, ld, rows, vocab, nids, top_k, (float)(1.0 / temperature), ids, logprobs, lse, entropy, top_ids,
+                top_logprobs};
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  ProfScope ps("token_logprobs", (double)rows * ((double)vocab * es + 8.0 * (nids + 1 + top_k)), 8.0 * rows * vocab, 1, st);
+  IG_CU(dtype == IG_DT_F32    ? run_token_logprobs<IG_DT_F32>(a, st)
+        : dtype == IG_DT_BF16 ? run_token_logprobs<IG_DT_BF16>(a, st)
+                              : run_token_logprobs<IG_DT_F16>(a, st));
+  return 0;
+}
+
+int ig_token_logprobs_backward(const void *logits, int32_t dtype, int64_t ld, int64_t rows, int32_t vocab,
+                               double temperature, const int32_t *ids, int32_t nids, const float *lse,
+                               const float *entropy, const float *dlogprobs, const float *dentropy, void *dlogits,
+                               int64_t ldd, void *stream) {
+  t_last_error.clear();
+  const int es = vocab_elem_size(dtype);
+  if (!es) return fail(IG_ERR_BAD_ARG, "ig_token_logprobs_backward: dtype must be float32, bfloat16 or float16");
+  if (const char *m = bad_row_args(rows, vocab, nids, ids, dlogprobs, temperature))
+    return fail(IG_ERR_BAD_ARG, std::string("ig_token_logprobs_backward: ") + m);
+  const char *m = bad_matrix(logits, rows, vocab, ld, es);
+  if (!m) m = bad_matrix(dlogits, rows, vocab, ldd, es);
+  if (!m && rows > 0 && (!lse || (dentropy && !entropy))) m = "null argument";
+  if (m) return fail(IG_ERR_BAD_ARG, std::string("ig_token_logprobs_backward: ") + m);
+  if (logits == dlogits && ld != ldd)
+    return fail(IG_ERR_BAD_ARG, "ig_token_logprobs_backward: in place, both row strides must be the same");
+  if (rows == 0) return 0;
+  LogprobGradArgs a{logits, ld, rows, vocab, nids, 1, (float)(1.0 / temperature), ids, lse, entropy,
+                    nids > 0 ? dlogprobs : nullptr, dentropy, dlogits, ldd};
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  ProfScope ps("token_logprobs_backward", 2.0 * rows * vocab * es, 8.0 * rows * vocab, 1, st);
+  IG_CU(dtype == IG_DT_F32    ? run_token_logprobs_grad<IG_DT_F32>(a, st)
+        : dtype == IG_DT_BF16 ? run_token_logprobs_grad<IG_DT_BF16>(a, st)
+                              : run_token_logprobs_grad<IG_DT_F16>(a, st));
+  return 0;
+}
+
+int ig_distill_topk(const void *logits, int32_t dtype, int64_t ld, int64_t rows, int32_t vocab, double temperature,
+                    const int32_t *teacher_ids, const float *teacher_logits, int32_t k, int32_t tail,
+                    const float *weights, float *loss, void *dlogits, int64_t ldd, void *stream) {
+  t_last_error.clear();
+  const int es = vocab_elem_size(dtype);
+  if (!es) return fail(IG_ERR_BAD_ARG, "ig_distill_topk: dtype must be float32, bfloat16 or float16");
+  const char *m = bad_row_args(rows, vocab, k, teacher_ids, teacher_logits, temperature);
+  if (!m) m = bad_matrix(logits, rows, vocab, ld, es);
+  if (!m && dlogits) m = bad_matrix(dlogits, rows, vocab, ldd, es);
+  if (!m && rows > 0 && !loss) m = "null argument";
+  if (!m && logits == dlogits && ld != ldd) m = "in place, both row strides must be the same";
+  if (m) return fail(IG_ERR_BAD_ARG, std::string("ig_distill_topk: ") + m);
+  if (tail && vocab > (1 << 20))
+    return fail(IG_ERR_UNSUPPORTED, "ig_distill_topk: with the tail, at most 1048576 columns");
+  if (rows == 0) return 0;
+  DistillArgs a{logits, ld, rows, vocab, k, (float)(1.0 / temperature), teacher_ids, teacher_logits, weights, loss,
+                dlogits, ldd};
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  ProfScope ps("distill_topk", (double)rows * ((dlogits ? 2.0 : 1.0) * vocab * es + 8.0 * k), 10.0 * rows * vocab, 1, st);
+  IG_CU(dtype == IG_DT_F32    ? run_distill<IG_DT_F32>(a, tail != 0, st)
+        : dtype == IG_DT_BF16 ? run_distill<IG_DT_BF16>(a, tail != 0, st)
+                              : run_distill<IG_DT_F16>(a, tail != 0, st));
+  return 0;
+}
+
+}  // extern "C"

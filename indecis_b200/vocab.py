@@ -1,0 +1,129 @@
+"""Vocabulary operators on torch CUDA tensors: log probabilities of tokens with
+entropy and top alternatives, distillation from a teacher's top logits.
+
+Thin wrappers over the C ABI: each checks shapes, types and strides, allocates
+the outputs, enqueues the kernels on the current stream of the inputs' device
+and raises on a non-zero status. Logits are [rows, vocab] float32, bfloat16 or
+float16 with a unit column stride and any row stride.
+"""
+from __future__ import annotations
+
+from typing import NamedTuple, Optional
+
+import torch
+
+from . import _capi
+
+IDS_MAX = 256  # given tokens, or teacher entries, per row
+TOP_MAX = 32   # alternatives per row
+
+_DT = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+
+
+class TokenLogProbs(NamedTuple):
+    logprobs: torch.Tensor                # float32 [rows, given]
+    lse: torch.Tensor                     # float32 [rows]
+    entropy: torch.Tensor                 # float32 [rows]
+    top_ids: Optional[torch.Tensor]       # int32 [rows, top_k]
+    top_logprobs: Optional[torch.Tensor]  # float32 [rows, top_k]
+
+
+def _matrix(t, name):
+    if t.dim() != 2 or t.dtype not in _DT or not t.is_cuda or (t.shape[1] > 1 and t.stride(1) != 1):
+        raise ValueError(f"{name}: expected a CUDA float32, bfloat16 or float16 matrix with a unit column stride")
+    ld = t.stride(0) if t.shape[0] > 1 else t.shape[1]
+    if ld < t.shape[1]:
+        raise ValueError(f"{name}: row stride shorter than the row")
+    return ld
+
+
+def _dense(t, dtype, shape, like, name):
+    if t is None:
+        return None
+    if t.dtype != dtype or t.shape != shape or t.device != like.device or not t.is_contiguous():
+        raise ValueError(f"{name}: expected a contiguous {dtype} tensor of shape {tuple(shape)} on {like.device}")
+    return t.data_ptr()
+
+
+def _call(like, fn, *args):
+    """fn on the current stream of like's device."""
+    if like.device.index == torch.cuda.current_device():
+        rc = fn(*args, torch.cuda.current_stream().cuda_stream)
+    else:
+        with torch.cuda.device(like.device):
+            rc = fn(*args, torch.cuda.current_stream().cuda_stream)
+    if rc:
+        _capi.check(rc)
+
+
+def token_logprobs(logits, ids, temperature=1.0, top_k=0) -> TokenLogProbs:
+    """log softmax(logits / temperature) at ids (int32 [rows, given], negative:
+    none, reported as 0), with each row's logsumexp, entropy and top_k largest
+    columns (ties: the lowest first)."""
+    ld = _matrix(logits, "logits")
+    N, V = logits.shape
+    if ids.dim() != 2:
+        raise ValueError("ids: expected a matrix")
+    T = ids.shape[1]
+    pid = _dense(ids, torch.int32, (N, T), logits, "ids")
+    dev = logits.device
+    lp = torch.empty((N, T), dtype=torch.float32, device=dev)
+    lse = torch.empty(N, dtype=torch.float32, device=dev)
+    ent = torch.empty(N, dtype=torch.float32, device=dev)
+    ti = torch.empty((N, top_k), dtype=torch.int32, device=dev) if top_k > 0 else None
+    tl = torch.empty((N, top_k), dtype=torch.float32, device=dev) if top_k > 0 else None
+    _call(logits, _capi.load().ig_token_logprobs, logits.data_ptr(), _DT[logits.dtype], ld, N, V, temperature, pid, T,
+          lp.data_ptr(), lse.data_ptr(), ent.data_ptr(), top_k, ti.data_ptr() if ti is not None else None,
+          tl.data_ptr() if tl is not None else None)
+    return TokenLogProbs(lp, lse, ent, ti, tl)
+
+
+def token_logprobs_backward(logits, ids, lse, entropy, dlogprobs, dentropy=None, temperature=1.0, out=None):
+    """Gradient with respect to the logits, in their type, from the gradients
+    of token_logprobs' logprobs and entropy. out: where to write it (may be
+    logits itself)."""
+    ld = _matrix(logits, "logits")
+    N, V = logits.shape
+    if ids.dim() != 2:
+        raise ValueError("ids: expected a matrix")
+    T = ids.shape[1]
+    out, ldd = _out_like(logits, out)
+    _call(logits, _capi.load().ig_token_logprobs_backward, logits.data_ptr(), _DT[logits.dtype], ld, N, V, temperature,
+          _dense(ids, torch.int32, (N, T), logits, "ids"), T, _dense(lse, torch.float32, (N,), logits, "lse"),
+          _dense(entropy, torch.float32, (N,), logits, "entropy"),
+          _dense(dlogprobs, torch.float32, (N, T), logits, "dlogprobs"),
+          _dense(dentropy, torch.float32, (N,), logits, "dentropy"), out.data_ptr(), ldd)
+    return out
+
+
+def _out_like(logits, out):
+    if out is None:
+        out = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+    ldd = _matrix(out, "out")
+    if out.shape != logits.shape or out.dtype != logits.dtype or out.device != logits.device:
+        raise ValueError("out: expected the logits' shape, type and device")
+    return out, ldd
+
+
+def distill_topk(logits, teacher_ids, teacher_logits, temperature=1.0, tail=False, weights=None, grad=True, out=None):
+    """Divergence of softmax(logits / temperature) from a teacher's top entries
+    (int32 ids [rows, k], negative where a list is shorter; float32 values).
+
+    tail=False: the teacher's softmax over its list. tail=True: the values are
+    log probabilities, and the mass they leave is one more outcome. Returns
+    (loss float32 [rows], already weighted by `weights`; the gradient of its
+    sum with respect to the logits, or None with grad=False). out: where to
+    write the gradient (may be logits itself)."""
+    ld = _matrix(logits, "logits")
+    N, V = logits.shape
+    if teacher_ids.dim() != 2:
+        raise ValueError("teacher_ids: expected a matrix")
+    K = teacher_ids.shape[1]
+    loss = torch.empty(N, dtype=torch.float32, device=logits.device)
+    d, ldd = _out_like(logits, out) if grad else (None, 0)
+    _call(logits, _capi.load().ig_distill_topk, logits.data_ptr(), _DT[logits.dtype], ld, N, V, temperature,
+          _dense(teacher_ids, torch.int32, (N, K), logits, "teacher_ids"),
+          _dense(teacher_logits, torch.float32, (N, K), logits, "teacher_logits"), K, 1 if tail else 0,
+          _dense(weights, torch.float32, (N,), logits, "weights"), loss.data_ptr(),
+          d.data_ptr() if d is not None else None, ldd)
+    return loss, d
