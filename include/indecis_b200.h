@@ -376,6 +376,38 @@ IG_API int ig_distill_topk(const void *logits, int32_t dtype, int64_t ld, int64_
                            double temperature, const int32_t *teacher_ids, const float *teacher_logits, int32_t k,
                            int32_t tail, const float *weights, float *loss, void *dlogits, int64_t ldd, void *stream);
 
+/* Workspace bytes of ig_vocab_logprobs (backward = 0) or
+ * ig_vocab_logprobs_backward (backward != 0; top_k unused) on the current
+ * device; 0 for sizes those refuse. The caller owns the workspace (256-byte
+ * aligned): calls that share one must not overlap on the GPU. */
+IG_API int64_t ig_vocab_workspace(int64_t rows, int32_t vocab, int32_t hidden_size, int32_t top_k, int32_t backward);
+
+/* ig_token_logprobs on the logits hidden . weight^T (hidden
+ * [rows][hidden_size], weight [vocab][hidden_size], both IG_DT_BF16 or both
+ * IG_DT_F16, float32 accumulation), which are never stored. Rows of both
+ * matrices start at multiples of 16 bytes (strides ldh, ldw in elements,
+ * multiples of 8); hidden_size is free. A bias per token is one more column:
+ * hidden extended by 1, weight by the bias. rows <= 2^24. */
+IG_API int ig_vocab_logprobs(const void *hidden, int64_t ldh, const void *weight, int64_t ldw, int32_t dtype,
+                             int64_t rows, int32_t vocab, int32_t hidden_size, double temperature, const int32_t *ids,
+                             int32_t nids, float *logprobs, float *lse, float *entropy, int32_t top_k,
+                             int32_t *top_ids, float *top_logprobs, void *workspace, int64_t workspace_bytes,
+                             void *stream);
+
+/* Its gradient with respect to hidden and weight (either may be NULL), from
+ * the forward's logprobs, lse and entropy: with G the gradient
+ * ig_token_logprobs_backward gives for the logits, dhidden = G . weight and
+ * dweight = G^T . hidden, in the operands' type, strides free. G is formed
+ * in the workspace in column chunks and rounded to the operands' type (for
+ * float16 scaled by a power of two, so that small probabilities keep their
+ * bits); the sums are float32 in a fixed order. */
+IG_API int ig_vocab_logprobs_backward(const void *hidden, int64_t ldh, const void *weight, int64_t ldw, int32_t dtype,
+                                      int64_t rows, int32_t vocab, int32_t hidden_size, double temperature,
+                                      const int32_t *ids, int32_t nids, const float *logprobs, const float *lse,
+                                      const float *entropy, const float *dlogprobs, const float *dentropy,
+                                      void *dhidden, int64_t lddh, void *dweight, int64_t lddw, void *workspace,
+                                      int64_t workspace_bytes, void *stream);
+
 /* Per-layer intermediates of one ig_encode call, copied to host buffers for
  * parity checks (NULL fields are skipped). Layouts as the oracle's. */
 typedef struct ig_dump {

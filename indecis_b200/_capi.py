@@ -34,7 +34,7 @@ SYMBOLS = ["ig_model_create", "ig_model_destroy", "ig_model_set_heads", "ig_enco
            "ig_check_gelu_division", "ig_model_create_multi", "ig_model_replica", "ig_model_device_count",
            "ig_model_create_stored", "ig_model_create_stored_multi", "ig_device_count", "ig_gemm_geglu_quant",
            "ig_profile_only", "ig_check_wait_timeout", "ig_token_logprobs", "ig_token_logprobs_backward",
-           "ig_distill_topk"]
+           "ig_distill_topk", "ig_vocab_workspace", "ig_vocab_logprobs", "ig_vocab_logprobs_backward"]
 
 IG_EMB_F32 = 0
 IG_EMB_BF16 = 1
@@ -199,6 +199,12 @@ def load() -> C.CDLL:
     L.ig_token_logprobs.argtypes = [vp, i32, i64, i64, i32, f64, vp, i32, vp, vp, vp, i32, vp, vp, vp]
     L.ig_token_logprobs_backward.argtypes = [vp, i32, i64, i64, i32, f64, vp, i32, vp, vp, vp, vp, vp, i64, vp]
     L.ig_distill_topk.argtypes = [vp, i32, i64, i64, i32, f64, vp, vp, i32, i32, vp, vp, vp, i64, vp]
+    L.ig_vocab_workspace.argtypes = [i64, i32, i32, i32, i32]
+    L.ig_vocab_workspace.restype = i64
+    L.ig_vocab_logprobs.argtypes = [vp, i64, vp, i64, i32, i64, i32, i32, f64, vp, i32, vp, vp, vp, i32, vp, vp, vp, i64,
+                                    vp]
+    L.ig_vocab_logprobs_backward.argtypes = [vp, i64, vp, i64, i32, i64, i32, i32, f64, vp, i32, vp, vp, vp, vp, vp, vp,
+                                             i64, vp, i64, vp, i64, vp]
     _lib = L
     return L
 

@@ -29,6 +29,19 @@ static const char *bad_row_args(int64_t rows, int64_t vocab, int32_t nids, const
   return nullptr;
 }
 
+static const char *bad_vocab_args(const void *h, int64_t ldh, const void *w, int64_t ldw, int32_t dtype, int64_t rows,
+                                  int32_t vocab, int32_t hidden) {
+  if (dtype != IG_DT_BF16 && dtype != IG_DT_F16) return "dtype must be bfloat16 or float16";
+  if (hidden < 1 || hidden > (1 << 20)) return "hidden size out of range";
+  if (rows > (1 << 24)) return "too many rows";
+  const char *m = bad_matrix(h, rows, hidden, ldh, 2);
+  if (!m) m = bad_matrix(w, vocab, hidden, ldw, 2);
+  if (m) return m;
+  if (ldh % 8 || ldw % 8 || ((reinterpret_cast<uintptr_t>(h) | reinterpret_cast<uintptr_t>(w)) & 15))
+    return "rows of hidden and weight must start at multiples of 16 bytes (strides multiples of 8)";
+  return nullptr;
+}
+
 }  // namespace ig
 
 using namespace ig;
@@ -108,6 +121,84 @@ int ig_distill_topk(const void *logits, int32_t dtype, int64_t ld, int64_t rows,
         : dtype == IG_DT_BF16 ? run_distill<IG_DT_BF16>(a, tail != 0, st)
                               : run_distill<IG_DT_F16>(a, tail != 0, st));
   return 0;
+}
+
+int64_t ig_vocab_workspace(int64_t rows, int32_t vocab, int32_t hidden, int32_t top_k, int32_t backward) {
+  if (rows <= 0 || rows > (1 << 24) || vocab < 1 || vocab > (1 << 30) || hidden < 1 || hidden > (1 << 20) || top_k < 0 ||
+      top_k > IG_VOCAB_TOP_MAX)
+    return 0;
+  const VPlan p = vocab_plan(rows, vocab, hidden, backward ? 0 : top_k);
+  return (int64_t)(backward ? p.bwd_bytes : p.fwd_bytes);
+}
+
+int ig_vocab_logprobs(const void *hidden, int64_t ldh, const void *weight, int64_t ldw, int32_t dtype, int64_t rows,
+                      int32_t vocab, int32_t hidden_size, double temperature, const int32_t *ids, int32_t nids,
+                      float *logprobs, float *lse, float *entropy, int32_t top_k, int32_t *top_ids, float *top_logprobs,
+                      void *workspace, int64_t workspace_bytes, void *stream) {
+  t_last_error.clear();
+  const char *m = bad_row_args(rows, vocab, nids, ids, logprobs, temperature);
+  if (!m) m = bad_vocab_args(hidden, ldh, weight, ldw, dtype, rows, vocab, hidden_size);
+  if (!m && (top_k < 0 || top_k > IG_VOCAB_TOP_MAX)) m = "top_k must be between 0 and 32";
+  if (!m && rows > 0 && top_k > 0 && (!top_ids || !top_logprobs)) m = "null argument";
+  if (m) return fail(IG_ERR_BAD_ARG, std::string("ig_vocab_logprobs: ") + m);
+  if (rows == 0) return 0;
+  const VPlan p = vocab_plan(rows, vocab, hidden_size, top_k);
+  if (!workspace || workspace_bytes < (int64_t)p.fwd_bytes || (reinterpret_cast<uintptr_t>(workspace) & 255))
+    return fail(IG_ERR_BAD_ARG, "ig_vocab_logprobs: workspace missing, too small or not aligned to 256 bytes");
+  LogprobArgs o{};
+  o.rows = rows;
+  o.V = vocab;
+  o.T = nids;
+  o.K = top_k;
+  o.c = (float)(1.0 / temperature);
+  o.ids = ids;
+  o.logprobs = logprobs;
+  o.lse = lse;
+  o.entropy = entropy;
+  o.top_ids = top_ids;
+  o.top_logprobs = top_logprobs;
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  ProfScope ps("vocab_logprobs", 2.0 * ((double)rows + vocab) * hidden_size, 2.0 * rows * vocab * hidden_size, 2, st);
+  return run_vocab_logprobs(VMatrices{hidden, weight, ldh, ldw, dtype}, p, o, static_cast<uint8_t *>(workspace), st);
+}
+
+int ig_vocab_logprobs_backward(const void *hidden, int64_t ldh, const void *weight, int64_t ldw, int32_t dtype,
+                               int64_t rows, int32_t vocab, int32_t hidden_size, double temperature, const int32_t *ids,
+                               int32_t nids, const float *logprobs, const float *lse, const float *entropy,
+                               const float *dlogprobs, const float *dentropy, void *dhidden, int64_t lddh, void *dweight,
+                               int64_t lddw, void *workspace, int64_t workspace_bytes, void *stream) {
+  t_last_error.clear();
+  const char *m = bad_row_args(rows, vocab, nids, ids, dlogprobs, temperature);
+  if (!m) m = bad_vocab_args(hidden, ldh, weight, ldw, dtype, rows, vocab, hidden_size);
+  if (!m && dhidden) m = bad_matrix(dhidden, rows, hidden_size, lddh, 2);
+  if (!m && dweight) m = bad_matrix(dweight, vocab, hidden_size, lddw, 2);
+  if (!m && rows > 0 && (!lse || (nids > 0 && !logprobs) || (dentropy && !entropy))) m = "null argument";
+  if (!m && ((dhidden && dhidden == hidden) || (dweight && dweight == weight))) m = "the gradients cannot replace the operands";
+  if (m) return fail(IG_ERR_BAD_ARG, std::string("ig_vocab_logprobs_backward: ") + m);
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  if (!dhidden && !dweight) return 0;
+  if (rows == 0) {
+    if (dweight) IG_CU(cudaMemset2DAsync(dweight, (size_t)lddw * 2, 0, (size_t)hidden_size * 2, vocab, st));
+    return 0;
+  }
+  const VPlan p = vocab_plan(rows, vocab, hidden_size, 0);
+  if (!workspace || workspace_bytes < (int64_t)p.bwd_bytes || (reinterpret_cast<uintptr_t>(workspace) & 255))
+    return fail(IG_ERR_BAD_ARG, "ig_vocab_logprobs_backward: workspace missing, too small or not aligned to 256 bytes");
+  LogprobGradArgs g{};
+  g.rows = rows;
+  g.V = vocab;
+  g.T = nids;
+  g.c = (float)(1.0 / temperature);
+  g.ids = ids;
+  g.lse = lse;
+  g.entropy = entropy;
+  g.dlogprobs = nids > 0 ? dlogprobs : nullptr;
+  g.dentropy = dentropy;
+  const int products = 1 + (dhidden != nullptr) + (dweight != nullptr);
+  ProfScope ps("vocab_logprobs_backward", 4.0 * ((double)rows + vocab) * hidden_size,
+               2.0 * products * rows * vocab * hidden_size, 4 + products, st);
+  return run_vocab_grad(VMatrices{hidden, weight, ldh, ldw, dtype}, p, g,
+                        VocabGradOut{logprobs, dhidden, dweight, lddh, lddw}, static_cast<uint8_t *>(workspace), st);
 }
 
 }  // extern "C"

@@ -1,5 +1,6 @@
 """Vocabulary operators on torch CUDA tensors: log probabilities of tokens with
-entropy and top alternatives, distillation from a teacher's top logits.
+entropy and top alternatives (from stored logits, or straight from hidden
+states and the vocabulary matrix), distillation from a teacher's top logits.
 
 Thin wrappers over the C ABI: each checks shapes, types and strides, allocates
 the outputs, enqueues the kernels on the current stream of the inputs' device
@@ -127,3 +128,84 @@ def distill_topk(logits, teacher_ids, teacher_logits, temperature=1.0, tail=Fals
           _dense(weights, torch.float32, (N,), logits, "weights"), loss.data_ptr(),
           d.data_ptr() if d is not None else None, ldd)
     return loss, d
+
+
+def aligned(t):
+    """t itself if its rows start at multiples of 16 bytes, else a copy that does. Lay a weight out once: the calls
+    below do it on every call for what is not."""
+    ld = _matrix(t, "matrix")
+    if t.data_ptr() % 16 == 0 and ld % 8 == 0:
+        return t
+    n, h = t.shape
+    buf = torch.empty((n, (h + 7) // 8 * 8), dtype=t.dtype, device=t.device)
+    return buf[:, :h].copy_(t)
+
+
+def _operands(hidden, weight):
+    for t, name in ((hidden, "hidden"), (weight, "weight")):
+        _matrix(t, name)
+        if t.dtype == torch.float32:
+            raise ValueError(f"{name}: expected bfloat16 or float16")
+    if hidden.dtype != weight.dtype or hidden.device != weight.device or hidden.shape[1] != weight.shape[1]:
+        raise ValueError("hidden and weight: expected one type, device and row length")
+    hidden, weight = aligned(hidden), aligned(weight)
+    h8 = (hidden.shape[1] + 7) // 8 * 8
+    return (hidden, hidden.stride(0) if hidden.shape[0] > 1 else h8, weight,
+            weight.stride(0) if weight.shape[0] > 1 else h8)
+
+
+def _workspace(like, *sizes):
+    L = _capi.load()
+    if like.device.index == torch.cuda.current_device():
+        n = L.ig_vocab_workspace(*sizes)
+    else:
+        with torch.cuda.device(like.device):
+            n = L.ig_vocab_workspace(*sizes)
+    return torch.empty(max(int(n), 1), dtype=torch.uint8, device=like.device)
+
+
+def vocab_logprobs(hidden, weight, ids, temperature=1.0, top_k=0) -> TokenLogProbs:
+    """token_logprobs of the logits hidden @ weight.T (hidden [rows, H], weight
+    [vocab, H], both bfloat16 or both float16), which are never stored."""
+    hidden, ldh, weight, ldw = _operands(hidden, weight)
+    N, H = hidden.shape
+    V = weight.shape[0]
+    if ids.dim() != 2:
+        raise ValueError("ids: expected a matrix")
+    T = ids.shape[1]
+    pid = _dense(ids, torch.int32, (N, T), hidden, "ids")
+    dev = hidden.device
+    lp = torch.empty((N, T), dtype=torch.float32, device=dev)
+    lse = torch.empty(N, dtype=torch.float32, device=dev)
+    ent = torch.empty(N, dtype=torch.float32, device=dev)
+    ti = torch.empty((N, top_k), dtype=torch.int32, device=dev) if top_k > 0 else None
+    tl = torch.empty((N, top_k), dtype=torch.float32, device=dev) if top_k > 0 else None
+    ws = _workspace(hidden, N, V, H, top_k, 0)
+    _call(hidden, _capi.load().ig_vocab_logprobs, hidden.data_ptr(), ldh, weight.data_ptr(), ldw, _DT[hidden.dtype], N, V,
+          H, temperature, pid, T, lp.data_ptr(), lse.data_ptr(), ent.data_ptr(), top_k,
+          ti.data_ptr() if ti is not None else None, tl.data_ptr() if tl is not None else None, ws.data_ptr(), ws.numel())
+    return TokenLogProbs(lp, lse, ent, ti, tl)
+
+
+def vocab_logprobs_backward(hidden, weight, ids, logprobs, lse, entropy, dlogprobs, dentropy=None, temperature=1.0,
+                            need_hidden=True, need_weight=True):
+    """Gradients with respect to hidden and weight, in their type (None where
+    not needed), from the gradients of vocab_logprobs' logprobs and entropy and
+    its results."""
+    hidden, ldh, weight, ldw = _operands(hidden, weight)
+    N, H = hidden.shape
+    V = weight.shape[0]
+    if ids.dim() != 2:
+        raise ValueError("ids: expected a matrix")
+    T = ids.shape[1]
+    dh = torch.empty((N, H), dtype=hidden.dtype, device=hidden.device) if need_hidden else None
+    dw = torch.empty((V, H), dtype=weight.dtype, device=hidden.device) if need_weight else None
+    ws = _workspace(hidden, N, V, H, 0, 1)
+    _call(hidden, _capi.load().ig_vocab_logprobs_backward, hidden.data_ptr(), ldh, weight.data_ptr(), ldw,
+          _DT[hidden.dtype], N, V, H, temperature, _dense(ids, torch.int32, (N, T), hidden, "ids"), T,
+          _dense(logprobs, torch.float32, (N, T), hidden, "logprobs"), _dense(lse, torch.float32, (N,), hidden, "lse"),
+          _dense(entropy, torch.float32, (N,), hidden, "entropy"),
+          _dense(dlogprobs, torch.float32, (N, T), hidden, "dlogprobs"),
+          _dense(dentropy, torch.float32, (N,), hidden, "dentropy"), dh.data_ptr() if dh is not None else None, H,
+          dw.data_ptr() if dw is not None else None, H, ws.data_ptr(), ws.numel())
+    return dh, dw
