@@ -63,7 +63,7 @@ int ig_token_logprobs(const void *logits, int32_t dtype, int64_t ld, int64_t row
   if (rows > 0 && top_k > 0 && (!top_ids || !top_logprobs)) return fail(IG_ERR_BAD_ARG, "ig_token_logprobs: null argument");
   if (rows == 0) return 0;
   LogprobArgs a{logits, ld, rows, vocab, nids, top_k, (float)(1.0 / temperature), ids, logprobs, lse, entropy, top_ids,
-                top_logprobs};
+                top_logprobs, 1};
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   ProfScope ps("token_logprobs", (double)rows * ((double)vocab * es + 8.0 * (nids + 1 + top_k)), 8.0 * rows * vocab, 1, st);
   IG_CU(dtype == IG_DT_F32    ? run_token_logprobs<IG_DT_F32>(a, st)
@@ -114,7 +114,7 @@ int ig_distill_topk(const void *logits, int32_t dtype, int64_t ld, int64_t rows,
     return fail(IG_ERR_UNSUPPORTED, "ig_distill_topk: with the tail, at most 1048576 columns");
   if (rows == 0) return 0;
   DistillArgs a{logits, ld, rows, vocab, k, (float)(1.0 / temperature), teacher_ids, teacher_logits, weights, loss,
-                dlogits, ldd};
+                dlogits, ldd, 1};
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   ProfScope ps("distill_topk", (double)rows * ((dlogits ? 2.0 : 1.0) * vocab * es + 8.0 * k), 10.0 * rows * vocab, 1, st);
   IG_CU(dtype == IG_DT_F32    ? run_distill<IG_DT_F32>(a, tail != 0, st)

@@ -9,7 +9,6 @@
 // scaling: x c would overflow for masks of the type's lowest value. y is
 // clamped at kYMin so that a masked element (-inf, or far below the maximum)
 // adds 0 to u instead of 0 * inf; the clamp and the sums keep NaN.
-#include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -20,13 +19,11 @@
 
 namespace ig {
 
-namespace cg = cooperative_groups;
-
 constexpr int kVocThreads = 256;
 constexpr int kVocWarps = kVocThreads / 32;
 constexpr int kVocUnroll = 4;     // 16-byte vectors in flight per thread
 constexpr int kTopMax = 32;       // alternatives per row
-constexpr int kTopCap = 128;      // a warp's candidate buffer
+constexpr int kTopCap = 512;      // candidates a CTA collects
 constexpr int kTeacherMax = kVocThreads;  // teacher entries per row: one thread each
 constexpr float kLog2e = 1.44269504088896340736f;
 constexpr float kLn2 = 0.69314718055994530942f;
@@ -47,6 +44,9 @@ __device__ __forceinline__ float max_nan(float a, float b) {
 
 // ---- element types --------------------------------------------------------------
 
+// unpack/pack: a 16-byte vector as floats; kNegInf: -inf in every element;
+// hmax: element-wise maximum (NaN ignored) of two words; top: the largest of a
+// word's elements as a float.
 template <int DT>
 struct VElem;
 template <>
@@ -62,6 +62,12 @@ struct VElem<IG_DT_F32> {
   __device__ __forceinline__ static uint4 pack(const float *x) {
     return make_uint4(__float_as_uint(x[0]), __float_as_uint(x[1]), __float_as_uint(x[2]), __float_as_uint(x[3]));
   }
+  static constexpr uint32_t kNegInf = 0xFF800000u;
+  __device__ __forceinline__ static uint32_t hmax(uint32_t a, uint32_t b) {
+    return __float_as_uint(fmaxf(__uint_as_float(a), __uint_as_float(b)));
+  }
+  __device__ __forceinline__ static float top(uint32_t a) { return fmaxf(__uint_as_float(a), -IG_INF); }
+  __device__ __forceinline__ static uint32_t bits(T v) { return __float_as_uint(v); }
   __device__ __forceinline__ static float get(T v) { return v; }
   __device__ __forceinline__ static T put(float v) { return v; }
 };
@@ -86,6 +92,15 @@ struct VElem<IG_DT_BF16> {
     }
     return make_uint4(w[0], w[1], w[2], w[3]);
   }
+  static constexpr uint32_t kNegInf = 0xFF80FF80u;
+  __device__ __forceinline__ static uint32_t hmax(uint32_t a, uint32_t b) {
+    const __nv_bfloat162 m = __hmax2(*reinterpret_cast<__nv_bfloat162 *>(&a), *reinterpret_cast<__nv_bfloat162 *>(&b));
+    return *reinterpret_cast<const uint32_t *>(&m);
+  }
+  __device__ __forceinline__ static float top(uint32_t a) {
+    return fmaxf(fmaxf(__uint_as_float(a << 16), __uint_as_float(a & 0xFFFF0000u)), -IG_INF);
+  }
+  __device__ __forceinline__ static uint32_t bits(T v) { return __bfloat16_as_ushort(v); }
   __device__ __forceinline__ static float get(T v) { return __bfloat162float(v); }
   __device__ __forceinline__ static T put(float v) { return __float2bfloat16_rn(v); }
 };
@@ -111,6 +126,16 @@ struct VElem<IG_DT_F16> {
     }
     return make_uint4(w[0], w[1], w[2], w[3]);
   }
+  static constexpr uint32_t kNegInf = 0xFC00FC00u;
+  __device__ __forceinline__ static uint32_t hmax(uint32_t a, uint32_t b) {
+    const __half2 m = __hmax2(*reinterpret_cast<__half2 *>(&a), *reinterpret_cast<__half2 *>(&b));
+    return *reinterpret_cast<const uint32_t *>(&m);
+  }
+  __device__ __forceinline__ static float top(uint32_t a) {
+    const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&a));
+    return fmaxf(fmaxf(f.x, f.y), -IG_INF);
+  }
+  __device__ __forceinline__ static uint32_t bits(T v) { return __half_as_ushort(v); }
   __device__ __forceinline__ static float get(T v) { return __half2float(v); }
   __device__ __forceinline__ static T put(float v) { return __float2half_rn(v); }
 };
@@ -131,14 +156,49 @@ struct RowVecs {
   }
   __device__ __forceinline__ int col(int v) const { return v * E::kN - mis; }
   __device__ __forceinline__ bool whole(int v) const { return col(v) >= 0 && col(v) + E::kN <= V; }
-  __device__ __forceinline__ void load_edge(int v, float *x) const {
+  // A partial vector, -inf outside the row.
+  __device__ __forceinline__ uint4 edge(int v) const {
+    constexpr int kPer = E::kN / 4;  // elements per word
+    uint32_t w[4];
 #pragma unroll
-    for (int i = 0; i < E::kN; i++) {
-      const int c = col(v) + i;
-      x[i] = c >= 0 && c < V ? E::get(row[c]) : -IG_INF;
+    for (int i = 0; i < 4; i++) {
+      w[i] = E::kNegInf;
+#pragma unroll
+      for (int j = 0; j < kPer; j++) {
+        const int c = col(v) + i * kPer + j;
+        if (c >= 0 && c < V) {
+          const uint32_t keep = kPer == 1 ? 0u : 0xFFFFu << (16 * (1 - j));
+          w[i] = (w[i] & keep) | (E::bits(row[c]) << (16 * j));
+        }
+      }
     }
+    return make_uint4(w[0], w[1], w[2], w[3]);
+  }
+  __device__ __forceinline__ uint4 load(int v) const {
+    return whole(v) ? *reinterpret_cast<const uint4 *>(row + col(v)) : edge(v);
   }
 };
+
+// A CTA's part of a row, vectors [v0, v1): the whole ones lie end to end from
+// `base` (n of them, the first is vector w0); the row's partial first and last
+// vector, if they fall into the part, are read on their own, so that the loops
+// over the whole ones test nothing but their end.
+template <int DT>
+struct RowPart {
+  const uint4 *base;
+  int v0, v1, w0, n;
+  bool first, last;
+  __device__ __forceinline__ RowPart(const RowVecs<DT> &rv, int part, int parts) {
+    v0 = (int)((int64_t)rv.nv * part / parts);
+    v1 = (int)((int64_t)rv.nv * (part + 1) / parts);
+    first = v0 < v1 && !rv.whole(v0);
+    last = v1 - v0 > (first ? 1 : 0) && !rv.whole(v1 - 1);
+    w0 = v0 + (first ? 1 : 0);
+    n = v1 - w0 - (last ? 1 : 0);
+    base = reinterpret_cast<const uint4 *>(rv.row + rv.col(w0));
+  }
+};
+constexpr int kFirstThread = 0, kLastThread = 32;  // the threads that take the partial vectors
 
 // ---- running statistics -----------------------------------------------------------
 
@@ -165,6 +225,19 @@ __device__ __forceinline__ void vstat_merge(VStat &a, VStat b, float c2) {
   if constexpr (U) a.u += b.u;
 }
 
+// One pair of values.
+template <bool U>
+__device__ __forceinline__ void vstat_pair(float2 x, float2 nm, float2 cc, float2 &s, float2 &u) {
+  float2 y = __fmul2_rn(__fadd2_rn(x, nm), cc);
+  if constexpr (U) {
+    y.x = max_nan(y.x, kYMin);
+    y.y = max_nan(y.y, kYMin);
+  }
+  const float2 e = make_float2(ex2(y.x), ex2(y.y));
+  s = __fadd2_rn(s, e);
+  if constexpr (U) u = __ffma2_rn(e, y, u);
+}
+
 // The N values x (N even) with maximum mx.
 template <bool U, int N>
 __device__ __forceinline__ void vstat_add(VStat &a, const float (&x)[N], float mx, float c2) {
@@ -174,38 +247,78 @@ __device__ __forceinline__ void vstat_add(VStat &a, const float (&x)[N], float m
   const float2 nm = make_float2(-mb, -mb), cc = make_float2(c2, c2);
   float2 s = make_float2(0.0f, 0.0f), u = s;
 #pragma unroll
-  for (int i = 0; i < N; i += 2) {
-    float2 y = __fmul2_rn(__fadd2_rn(make_float2(x[i], x[i + 1]), nm), cc);
-    if constexpr (U) {
-      y.x = max_nan(y.x, kYMin);
-      y.y = max_nan(y.y, kYMin);
-    }
-    const float2 e = make_float2(ex2(y.x), ex2(y.y));
-    s = __fadd2_rn(s, e);
-    if constexpr (U) u = __ffma2_rn(e, y, u);
+  for (int i = 0; i < N; i += 2) vstat_pair<U>(make_float2(x[i], x[i + 1]), nm, cc, s, u);
+  a.s += s.x + s.y;
+  if constexpr (U) a.u += u.x + u.y;
+}
+
+// R vectors: the maximum on the packed words, then vector by vector.
+template <int DT, bool U, int R>
+__device__ __forceinline__ void vstat_add_raw(VStat &a, const uint4 (&raw)[R], float c2) {
+  using E = VElem<DT>;
+  uint32_t w = E::hmax(E::hmax(raw[0].x, raw[0].y), E::hmax(raw[0].z, raw[0].w));
+#pragma unroll
+  for (int j = 1; j < R; j++)
+    w = E::hmax(w, E::hmax(E::hmax(raw[j].x, raw[j].y), E::hmax(raw[j].z, raw[j].w)));
+  const float m = fmaxf(a.m, E::top(w));
+  if (m > a.m) vstat_shift<U>(a, m, c2);
+  const float mb = m == -IG_INF ? 0.0f : m;
+  const float2 nm = make_float2(-mb, -mb), cc = make_float2(c2, c2);
+  float2 s = make_float2(0.0f, 0.0f), u = s;
+#pragma unroll
+  for (int j = 0; j < R; j++) {
+    float x[E::kN];
+    E::unpack(raw[j], x);
+#pragma unroll
+    for (int i = 0; i < E::kN; i += 2) vstat_pair<U>(make_float2(x[i], x[i + 1]), nm, cc, s, u);
   }
   a.s += s.x + s.y;
   if constexpr (U) a.u += u.x + u.y;
 }
 
+__device__ __forceinline__ float warp_max(float v) {
+  float r;
+  asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
+  return r;
+}
+__device__ __forceinline__ float warp_sum(float v) {
+#pragma unroll
+  for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(~0u, v, o);
+  return v;
+}
+
+// The warp's statistics, in all lanes.
 template <bool U>
 __device__ __forceinline__ VStat vstat_warp(VStat a, float c2) {
-#pragma unroll
-  for (int o = 16; o; o >>= 1) {
-    VStat b;
-    b.m = __shfl_xor_sync(~0u, a.m, o);
-    b.s = __shfl_xor_sync(~0u, a.s, o);
-    b.u = U ? __shfl_xor_sync(~0u, a.u, o) : 0.0f;
-    // Both lanes add in the same order (the lower lane's first), so all lanes hold the same bits.
-    if (threadIdx.x & o) {
-      const VStat t = a;
-      a = b;
-      b = t;
-    }
-    vstat_merge<U>(a, b, c2);
+  vstat_shift<U>(a, warp_max(a.m), c2);
+  a.s = warp_sum(a.s);
+  if constexpr (U) a.u = warp_sum(a.u);
+  return a;
+}
+
+// n statistics in shared memory, joined in order: one maximum, then
+// independent terms.
+template <bool U>
+__device__ __forceinline__ VStat vstat_join(const VStat *p, int n, float c2) {
+  VStat a{p[0].m, 0.0f, 0.0f};
+  for (int i = 1; i < n; i++) a.m = fmaxf(a.m, p[i].m);
+  for (int i = 0; i < n; i++) {
+    VStat b = p[i];
+    vstat_shift<U>(b, a.m, c2);
+    a.s += b.s;
+    if constexpr (U) a.u += b.u;
   }
   return a;
 }
+
+// Clusters: a CTA hands its statistics to others by asynchronous stores that
+// count on the receiver's barrier. The barriers are set up before the loops
+// over the row; cluster_ready() makes sure, before the first store to another
+// CTA, that it has started and set up its own.
+__device__ __forceinline__ void cluster_announce() {
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void cluster_ready() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 
 // ---- top alternatives ---------------------------------------------------------------
 
@@ -213,106 +326,152 @@ __device__ __forceinline__ VStat vstat_warp(VStat a, float c2) {
 __device__ __forceinline__ bool top_before(float va, int ca, float vb, int cb) {
   return va > vb || (va == vb && ca < cb);
 }
-__device__ __forceinline__ int ordered_bits(float v) {
-  const int b = __float_as_int(v);
-  return b >= 0 ? b : b ^ 0x7FFFFFFF;
-}
-__device__ __forceinline__ float from_ordered(int b) { return __int_as_float(b >= 0 ? b : b ^ 0x7FFFFFFF); }
-
-struct TopWarp {
-  float *val;  // [kTopCap] candidates of this warp (shared memory)
-  int *col;
-  int *cta_tau;  // ordered bits of the best K-th value any warp has (shared)
-  int n, K;      // n, tau, ctau: the same in all lanes
-  float tau;     // a candidate has to come before (tau, ctau)
-  int ctau;
-  bool started;
+// The K first (value, column) of a CTA's part of a row, after the statistics'
+// pass has left each thread its own maximum. 64 bins of four neighbouring
+// threads: the K-th largest of the bins' maxima is a lower bound of the K-th
+// largest value (K bins hold a value at least as large), and only bins that
+// reach it (K, or a few more with ties) are read again, from L2. What reaches
+// the bound is collected and ranked. With too many equal values for the
+// buffer (a row of few distinct values) the K are found one by one instead.
+constexpr int kTopBins = 64;
+struct TopShared {
+  float bin[kTopBins];
+  int kept[kTopBins];
+  float val[kTopCap];
+  int col[kTopCap];
+  float tau;
+  int nkept, n;
+  float wv[kVocWarps];
+  int wc[kVocWarps];
 };
 
-// Keeps the K first candidates, sorted: each entry's rank is the number of
-// entries before it (columns are distinct, so ranks are).
-__device__ __noinline__ void top_compact(TopWarp &t) {
-  const int lane = threadIdx.x & 31;
-  __syncwarp();
-  float v[kTopCap / 32];
-  int c[kTopCap / 32], r[kTopCap / 32];
+template <int DT>
+__device__ __noinline__ void top_one_by_one(const RowVecs<DT> rv, int v0, int v1, int K, TopShared &t, float *out_val,
+                                            int *out_col, int *out_n) {
+  using E = VElem<DT>;
+  float lv = IG_INF;
+  int lc = -1, n = 0;
+  for (; n < K; n++) {
+    float bv = -IG_INF;
+    int bc = 0x7FFFFFFF;
+    for (int v = v0 + (int)threadIdx.x; v < v1; v += kVocThreads) {
+      float x[E::kN];
+      E::unpack(rv.load(v), x);
 #pragma unroll
-  for (int k = 0; k < kTopCap / 32; k++) {
-    const int i = k * 32 + lane;
-    v[k] = i < t.n ? t.val[i] : -IG_INF;
-    c[k] = i < t.n ? t.col[i] : 0x7FFFFFFF;
-    r[k] = i < t.n ? 0 : kTopCap;
-  }
-  for (int j = 0; j < t.n; j++) {
-    const float vj = t.val[j];
-    const int cj = t.col[j];
-#pragma unroll
-    for (int k = 0; k < kTopCap / 32; k++) r[k] += top_before(vj, cj, v[k], c[k]);
-  }
-  __syncwarp();
-#pragma unroll
-  for (int k = 0; k < kTopCap / 32; k++)
-    if (r[k] < t.K) {
-      t.val[r[k]] = v[k];
-      t.col[r[k]] = c[k];
-    }
-  __syncwarp();
-  if (t.n >= t.K) {
-    t.n = t.K;
-    t.tau = t.val[t.K - 1];
-    t.ctau = t.col[t.K - 1];
-    if (lane == 0) atomicMax(t.cta_tau, ordered_bits(t.tau));
-  }
-}
-
-// The K-th largest of the lanes' maxima is at most the K-th largest value:
-// a first bound, so that the first values do not all become candidates.
-__device__ __noinline__ void top_start(TopWarp &t, float mx) {
-  const int lane = threadIdx.x & 31;
-  int r = 0;
-  for (int j = 0; j < 32; j++) {
-    const float o = __shfl_sync(~0u, mx, j);
-    r += top_before(o, j, mx, lane);
-  }
-  const float kth = __shfl_sync(~0u, mx, __ffs(__ballot_sync(~0u, r == t.K - 1)) - 1);
-  if (kth > t.tau) {
-    t.tau = kth;
-    t.ctau = 0x7FFFFFFF;
-  }
-  t.started = true;
-}
-
-// Offers N values; value i of a lane is column col(i). mx: their maximum.
-template <int N, typename ColFn>
-__device__ __forceinline__ void top_offer(TopWarp &t, const float (&x)[N], float mx, ColFn col) {
-  const float shared = from_ordered(*(volatile int *)t.cta_tau);
-  if (shared > t.tau) {
-    t.tau = shared;
-    t.ctau = 0x7FFFFFFF;
-  }
-  if (!__any_sync(~0u, mx >= t.tau && mx > -IG_INF)) return;
-  if (!t.started) {
-    // NaN maxima cannot arise (fmaxf), but a lane may hold -inf only.
-    top_start(t, mx);
-  }
-#pragma unroll
-  for (int i = 0; i < N; i++) {
-    bool p = x[i] > t.tau || (x[i] == t.tau && col(i) < t.ctau);
-    unsigned b = __ballot_sync(~0u, p);
-    if (b) {
-      if (t.n + __popc(b) > kTopCap) {
-        top_compact(t);
-        p = x[i] > t.tau || (x[i] == t.tau && col(i) < t.ctau);
-        b = __ballot_sync(~0u, p);
+      for (int i = 0; i < E::kN; i++) {
+        const int c = rv.col(v) + i;
+        if (x[i] > -IG_INF && top_before(lv, lc, x[i], c) && top_before(x[i], c, bv, bc)) {
+          bv = x[i];
+          bc = c;
+        }
       }
-      if (p) {
-        const int at = t.n + __popc(b & ((1u << (threadIdx.x & 31)) - 1));
+    }
+#pragma unroll
+    for (int o = 16; o; o >>= 1) {
+      const float ov = __shfl_xor_sync(~0u, bv, o);
+      const int oc = __shfl_xor_sync(~0u, bc, o);
+      if (top_before(ov, oc, bv, bc)) {
+        bv = ov;
+        bc = oc;
+      }
+    }
+    __syncthreads();
+    if ((threadIdx.x & 31) == 0) {
+      t.wv[threadIdx.x >> 5] = bv;
+      t.wc[threadIdx.x >> 5] = bc;
+    }
+    __syncthreads();
+    for (int w = 0; w < kVocWarps; w++)
+      if (top_before(t.wv[w], t.wc[w], bv, bc)) {
+        bv = t.wv[w];
+        bc = t.wc[w];
+      }
+    if (bc == 0x7FFFFFFF) break;
+    if (threadIdx.x == 0) {
+      out_val[n] = bv;
+      out_col[n] = bc;
+    }
+    lv = bv;
+    lc = bc;
+  }
+  if (threadIdx.x == 0) *out_n = n;
+}
+
+template <int DT>
+__device__ __forceinline__ void top_scan(const uint4 &raw, int col, float tau, TopShared &t) {
+  using E = VElem<DT>;
+  if (E::top(E::hmax(E::hmax(raw.x, raw.y), E::hmax(raw.z, raw.w))) < tau) return;
+  float x[E::kN];
+  E::unpack(raw, x);
+#pragma unroll
+  for (int i = 0; i < E::kN; i++)
+    if (x[i] >= tau && x[i] > -IG_INF) {
+      const int at = atomicAdd(&t.n, 1);
+      if (at < kTopCap) {
         t.val[at] = x[i];
-        t.col[at] = col(i);
+        t.col[at] = col + i;
       }
-      t.n += __popc(b);
+    }
+}
+
+// tmax: the thread's maximum over the part's whole vectors threadIdx.x + i
+// kVocThreads (and a partial one, which is read again in any case).
+template <int DT>
+__device__ __forceinline__ void top_select(const RowVecs<DT> &rv, const RowPart<DT> &rp, float tmax, int K, TopShared &t,
+                                           float *out_val, int *out_col, int *out_n) {
+  const int tid = (int)threadIdx.x;
+  float bm = fmaxf(tmax, __shfl_xor_sync(~0u, tmax, 1));
+  bm = fmaxf(bm, __shfl_xor_sync(~0u, bm, 2));
+  if ((tid & 3) == 0) t.bin[tid >> 2] = bm;
+  if (tid == 0) t.nkept = t.n = 0;
+  __syncthreads();
+  if (tid < kTopBins) {
+    const float b = t.bin[tid];
+    int r = 0;
+#pragma unroll 8
+    for (int j = 0; j < kTopBins; j++) r += top_before(t.bin[j], j, b, tid);
+    if (r == K - 1) t.tau = b;
+  }
+  __syncthreads();
+  const float tau = t.tau;
+  if (tid < kTopBins && t.bin[tid] >= tau && t.bin[tid] > -IG_INF) t.kept[atomicAdd(&t.nkept, 1)] = tid;
+  __syncthreads();
+  const int rounds = (rp.n + kVocThreads - 1) / kVocThreads;
+  const int items = t.nkept * rounds * 4;
+  constexpr int kAhead = 4;  // loads in flight per thread
+  for (int it = tid; it < items; it += kAhead * kVocThreads) {
+    uint4 raw[kAhead];
+    int at[kAhead];
+#pragma unroll
+    for (int j = 0; j < kAhead; j++) {
+      const int k = it + j * kVocThreads, r = k >> 2, b = r / rounds;
+      at[j] = k < items ? (r - b * rounds) * kVocThreads + t.kept[b] * 4 + (k & 3) : rp.n;
+      if (at[j] < rp.n) raw[j] = rp.base[at[j]];
+    }
+#pragma unroll
+    for (int j = 0; j < kAhead; j++)
+      if (at[j] < rp.n) top_scan<DT>(raw[j], rv.col(rp.w0 + at[j]), tau, t);
+  }
+  if (tid == kFirstThread && rp.first) top_scan<DT>(rv.edge(rp.v0), rv.col(rp.v0), tau, t);
+  if (tid == kLastThread && rp.last) top_scan<DT>(rv.edge(rp.v1 - 1), rv.col(rp.v1 - 1), tau, t);
+  __syncthreads();
+  const int n = t.n;
+  if (n > kTopCap) {
+    top_one_by_one<DT>(rv, rp.v0, rp.v1, K, t, out_val, out_col, out_n);
+    return;
+  }
+  // The order of arrival varies, the ranks do not.
+  for (int i = tid; i < n; i += kVocThreads) {
+    const float v = t.val[i];
+    const int c = t.col[i];
+    int r = 0;
+    for (int j = 0; j < n; j++) r += top_before(t.val[j], t.col[j], v, c);
+    if (r < K) {
+      out_val[r] = v;
+      out_col[r] = c;
     }
   }
+  if (tid == 0) *out_n = n < K ? n : K;
 }
 
 // ---- forward ------------------------------------------------------------------------
@@ -326,6 +485,7 @@ struct LogprobArgs {
   float *logprobs, *lse, *entropy;
   int32_t *top_ids;
   float *top_logprobs;
+  int parts;  // CTAs per row (a cluster)
 };
 
 // Row results from its statistics and, for top_k, its sorted candidates.
@@ -344,8 +504,7 @@ __device__ __forceinline__ float row_logprob(float x, const VStat &a, float c, f
 }
 
 // Merges `lists` sorted lists (list l: cnt[l] entries at val/col + l * stride)
-// of one CTA into the first K, written to out_val/out_col; returns through
-// *out_n. All threads call it; lists * K <= kVocThreads entries take part.
+// into the first K, written to out_val/out_col; their number to *out_n.
 __device__ __forceinline__ void top_merge(const float *val, const int *col, const int *cnt, int lists, int stride, int K,
                                           float *out_val, int *out_col, int *out_n) {
   int total = 0;
@@ -384,98 +543,93 @@ template <int DT, bool TOP>
 __global__ void __launch_bounds__(kVocThreads, 4) token_logprobs_kernel(const LogprobArgs a) {
   using E = VElem<DT>;
   using T = typename E::T;
-  constexpr int kN = E::kN, kX = kN * kVocUnroll;
   __shared__ VStat s_warp[kVocWarps];
-  __shared__ VStat s_cta;
-  __shared__ float s_val[TOP ? kVocWarps * kTopCap : 1];
-  __shared__ int s_col[TOP ? kVocWarps * kTopCap : 1];
+  __shared__ VStat s_part[8];  // on rank 0, the cluster's statistics
+  __shared__ TopShared s_top[1];
   __shared__ float s_oval[TOP ? 8 * kTopMax : 1];  // this CTA's list, and on rank 0 all the cluster's
   __shared__ int s_ocol[TOP ? 8 * kTopMax : 1];
-  __shared__ int s_cnt[8], s_on, s_tau;
+  __shared__ int s_cnt[8], s_on;
   __shared__ float s_fval[TOP ? kTopMax : 1];
   __shared__ int s_fcol[TOP ? kTopMax : 1];
+  __shared__ __align__(8) uint64_t s_bar;
 
-  cg::cluster_group cl = cg::this_cluster();
-  const int cs = (int)cl.num_blocks(), rank = (int)cl.block_rank();
+  const int cs = a.parts, rank = cs > 1 ? (int)cluster_ctarank() : 0;
   const int64_t row = blockIdx.x / cs;
   const RowVecs<DT> rv(static_cast<const T *>(a.x) + row * a.ld, a.V);
-  const int v0 = (int)((int64_t)rv.nv * rank / cs), v1 = (int)((int64_t)rv.nv * (rank + 1) / cs);
+  const RowPart<DT> rp(rv, rank, cs);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const float c2 = a.c * kLog2e;
+  if (cs > 1) {
+    if (threadIdx.x == 0) {
+      mbar_init(&s_bar, 1);
+      fence_barrier_init();
+      // Rank 0 waits for the others' statistics and lists.
+      if (rank == 0) mbar_arrive_expect_tx(&s_bar, (uint32_t)(cs - 1) * (12u + 8u * a.K + (TOP ? 4u : 0u)));
+    }
+    __syncwarp();
+    cluster_announce();
+  }
+  // The given tokens' logits, asked for early.
+  int id = -1;
+  float xt = 0.0f;
+  if (rank == 0 && (int)threadIdx.x < a.T) {
+    id = a.ids[row * a.T + threadIdx.x];
+    if (id >= 0 && id < a.V) xt = E::get(rv.row[id]);
+  }
 
   VStat st{-IG_INF, 0.0f, 0.0f};
-  TopWarp tw;
-  if constexpr (TOP) {
-    tw.val = s_val + warp * kTopCap;
-    tw.col = s_col + warp * kTopCap;
-    tw.cta_tau = &s_tau;
-    tw.n = 0;
-    tw.K = a.K;
-    tw.tau = -IG_INF;
-    tw.ctau = INT32_MIN;  // no -inf is a candidate
-    tw.started = false;
-    if (threadIdx.x == 0) s_tau = ordered_bits(-IG_INF);
-    __syncthreads();
-  }
-  for (int b = v0; b < v1; b += kVocUnroll * kVocThreads) {
-    float x[kX];
+  constexpr int kRound = kVocUnroll * kVocThreads;
+  const uint4 *p = rp.base + threadIdx.x;
+  int i = 0;
+  for (; i + kRound <= rp.n; i += kRound) {
     uint4 raw[kVocUnroll];
 #pragma unroll
-    for (int j = 0; j < kVocUnroll; j++) {
-      const int v = b + j * kVocThreads + (int)threadIdx.x;
-      if (v < v1 && rv.whole(v)) raw[j] = *reinterpret_cast<const uint4 *>(rv.row + rv.col(v));
-    }
-#pragma unroll
-    for (int j = 0; j < kVocUnroll; j++) {
-      const int v = b + j * kVocThreads + (int)threadIdx.x;
-      if (v < v1 && rv.whole(v)) {
-        E::unpack(raw[j], x + j * kN);
-      } else if (v < v1) {
-        rv.load_edge(v, x + j * kN);
-      } else {
-#pragma unroll
-        for (int i = 0; i < kN; i++) x[j * kN + i] = -IG_INF;
-      }
-    }
-    float mx = x[0];
-#pragma unroll
-    for (int i = 1; i < kX; i++) mx = fmaxf(mx, x[i]);
-    mx = fmaxf(mx, -IG_INF);  // a chunk of NaN only
-    vstat_add<true>(st, x, mx, c2);
-    if constexpr (TOP)
-      top_offer(tw, x, mx,
-                [&](int i) { return rv.col(b + (i / kN) * kVocThreads + (int)threadIdx.x) + i % kN; });
+    for (int j = 0; j < kVocUnroll; j++) raw[j] = p[i + j * kVocThreads];
+    vstat_add_raw<DT, true>(st, raw, c2);
   }
+  for (i += threadIdx.x; i < rp.n; i += kVocThreads) {
+    const uint4 raw[1] = {rp.base[i]};
+    vstat_add_raw<DT, true>(st, raw, c2);
+  }
+  if (threadIdx.x == kFirstThread && rp.first) {
+    const uint4 raw[1] = {rv.edge(rp.v0)};
+    vstat_add_raw<DT, true>(st, raw, c2);
+  }
+  if (threadIdx.x == kLastThread && rp.last) {
+    const uint4 raw[1] = {rv.edge(rp.v1 - 1)};
+    vstat_add_raw<DT, true>(st, raw, c2);
+  }
+  const float tmax = st.m;
   st = vstat_warp<true>(st, c2);
   if (lane == 0) s_warp[warp] = st;
-  if constexpr (TOP) {
-    top_compact(tw);
-    if (lane == 0) s_cnt[warp] = tw.n;
-  }
+  if constexpr (TOP) top_select<DT>(rv, rp, tmax, a.K, s_top[0], s_oval, s_ocol, &s_on);
   __syncthreads();
-  st = s_warp[0];
-  for (int w = 1; w < kVocWarps; w++) vstat_merge<true>(st, s_warp[w], c2);
-  if constexpr (TOP) top_merge(s_val, s_col, s_cnt, kVocWarps, kTopCap, a.K, s_oval, s_ocol, &s_on);
+  st = vstat_join<true>(s_warp, kVocWarps, c2);
   if (cs > 1) {
-    if (threadIdx.x == 0) s_cta = st;
-    cl.sync();
-    if (rank == 0) {
-      for (int r = 1; r < cs; r++) vstat_merge<true>(st, *cl.map_shared_rank(&s_cta, r), c2);
+    cluster_ready();
+    if (rank != 0) {
+      if (threadIdx.x == 0) {
+        st_async_f32(&s_part[rank].m, 0, st.m, &s_bar);
+        st_async_f32(&s_part[rank].s, 0, st.s, &s_bar);
+        st_async_f32(&s_part[rank].u, 0, st.u, &s_bar);
+        if constexpr (TOP) st_async_f32(reinterpret_cast<float *>(&s_cnt[rank]), 0, __int_as_float(s_on), &s_bar);
+      }
       if constexpr (TOP) {
-        if ((int)threadIdx.x < cs) s_cnt[threadIdx.x] = *cl.map_shared_rank(&s_on, threadIdx.x);
-        for (int i = threadIdx.x; i < (cs - 1) * a.K; i += kVocThreads) {
-          const int r = 1 + i / a.K, k = i % a.K;
-          s_oval[r * kTopMax + k] = cl.map_shared_rank(s_oval, r)[k];
-          s_ocol[r * kTopMax + k] = cl.map_shared_rank(s_ocol, r)[k];
+        if ((int)threadIdx.x < a.K) {  // past the list's end: not read
+          st_async_f32(&s_oval[rank * kTopMax + threadIdx.x], 0, s_oval[threadIdx.x], &s_bar);
+          st_async_f32(reinterpret_cast<float *>(&s_ocol[rank * kTopMax + threadIdx.x]), 0,
+                       __int_as_float(s_ocol[threadIdx.x]), &s_bar);
         }
       }
+      return;
     }
-    cl.sync();
-    if (rank != 0) return;
-  } else if constexpr (TOP) {
+    if (threadIdx.x == 0) {
+      s_part[0] = st;
+      s_cnt[0] = TOP ? s_on : 0;
+    }
+    mbar_wait_cluster(&s_bar, 0, kDevTimeoutFull);
     __syncthreads();
-    if (threadIdx.x == 0) s_cnt[0] = s_on;
-    __syncthreads();
+    st = vstat_join<true>(s_part, cs, c2);
   }
   float log_s, lse, entropy;
   row_lse(st, a.c, log_s, lse, entropy);
@@ -483,26 +637,31 @@ __global__ void __launch_bounds__(kVocThreads, 4) token_logprobs_kernel(const Lo
     if (a.lse) a.lse[row] = lse;
     if (a.entropy) a.entropy[row] = entropy;
   }
-  for (int t = threadIdx.x; t < a.T; t += kVocThreads) {
-    const int id = a.ids[row * a.T + t];
+  if ((int)threadIdx.x < a.T) {
     float v = 0.0f;
     if (id >= a.V) {
       v = __int_as_float(0x7FC00000);
       set_device_error(kDevBadId);
     } else if (id >= 0) {
-      v = row_logprob(E::get(rv.row[id]), st, a.c, log_s);
+      v = row_logprob(xt, st, a.c, log_s);
     }
-    a.logprobs[row * a.T + t] = v;
+    a.logprobs[row * a.T + threadIdx.x] = v;
   }
   if constexpr (TOP) {
-    top_merge(s_oval, s_ocol, s_cnt, cs, kTopMax, a.K, s_fval, s_fcol, &s_on);
-    __syncthreads();
+    const float *fval = s_oval;
+    const int *fcol = s_ocol;
+    if (cs > 1) {
+      top_merge(s_oval, s_ocol, s_cnt, cs, kTopMax, a.K, s_fval, s_fcol, &s_on);
+      __syncthreads();
+      fval = s_fval;
+      fcol = s_fcol;
+    }
     const bool nan = st.s != st.s;
     for (int k = threadIdx.x; k < a.K; k += kVocThreads) {
       const bool have = k < s_on && !nan;
-      a.top_ids[row * a.K + k] = have ? s_fcol[k] : -1;
+      a.top_ids[row * a.K + k] = have ? fcol[k] : -1;
       a.top_logprobs[row * a.K + k] =
-          have ? row_logprob(s_fval[k], st, a.c, log_s) : (nan ? __int_as_float(0x7FC00000) : -IG_INF);
+          have ? row_logprob(fval[k], st, a.c, log_s) : (nan ? __int_as_float(0x7FC00000) : -IG_INF);
     }
   }
 }
@@ -528,6 +687,13 @@ struct RowCoef {
 __device__ __forceinline__ float dense_grad(float x, float c, const RowCoef &k) {
   const float t = max_nan(fmaf(x, c, -k.lse), kYMin);
   return ex2(t * kLog2e) * fmaf(k.B, t, k.A);
+}
+__device__ __forceinline__ float2 dense_grad2(float2 x, float c, const RowCoef &k) {
+  float2 t = __ffma2_rn(x, make_float2(c, c), make_float2(-k.lse, -k.lse));
+  t.x = max_nan(t.x, kYMin);
+  t.y = max_nan(t.y, kYMin);
+  const float2 y = __fmul2_rn(t, make_float2(kLog2e, kLog2e));
+  return __fmul2_rn(make_float2(ex2(y.x), ex2(y.y)), __ffma2_rn(make_float2(k.B, k.B), t, make_float2(k.A, k.A)));
 }
 // The gradient a given token adds in its own column: c times the sum over the
 // row's entries with the same id, in order.
@@ -562,20 +728,25 @@ __device__ __forceinline__ RowCoef row_coef(float lse, float H, float G, float g
   return k;
 }
 
-// Writes the kN results of vector v of a row: as one 16-byte store where the
+// Writes the kN results of a whole vector: as one 16-byte store where the
 // output row has the input's alignment, else by element.
 template <int DT>
-__device__ __forceinline__ void store_vec(typename VElem<DT>::T *drow, const RowVecs<DT> &rv, int v, bool same,
-                                          const float *d) {
+__device__ __forceinline__ void store_whole(typename VElem<DT>::T *dst, bool same, const float *d) {
   using E = VElem<DT>;
-  if (same && rv.whole(v)) {
-    __stcs(reinterpret_cast<uint4 *>(drow + rv.col(v)), E::pack(d));
+  if (same) {
+    __stcs(reinterpret_cast<uint4 *>(dst), E::pack(d));
   } else {
 #pragma unroll
-    for (int i = 0; i < E::kN; i++) {
-      const int c = rv.col(v) + i;
-      if (c >= 0 && c < rv.V) drow[c] = E::put(d[i]);
-    }
+    for (int i = 0; i < E::kN; i++) dst[i] = E::put(d[i]);
+  }
+}
+template <int DT>
+__device__ __forceinline__ void store_edge(typename VElem<DT>::T *drow, const RowVecs<DT> &rv, int v, const float *d) {
+  using E = VElem<DT>;
+#pragma unroll
+  for (int i = 0; i < E::kN; i++) {
+    const int c = rv.col(v) + i;
+    if (c >= 0 && c < rv.V) drow[c] = E::put(d[i]);
   }
 }
 
@@ -590,53 +761,63 @@ __global__ void __launch_bounds__(kVocThreads, 4) token_logprobs_grad_kernel(con
   const RowVecs<DT> rv(static_cast<const T *>(a.x) + row * a.ld, a.V);
   T *drow = static_cast<T *>(a.dx) + row * a.ldd;
   const bool same = (reinterpret_cast<uintptr_t>(drow) & 15) == (reinterpret_cast<uintptr_t>(rv.row) & 15);
-  const int v0 = (int)((int64_t)rv.nv * seg / a.segs), v1 = (int)((int64_t)rv.nv * (seg + 1) / a.segs);
+  const RowPart<DT> rp(rv, seg, a.segs);
   const int32_t *ids = a.ids + row * a.T;
   const float *g = a.dlogprobs + row * a.T;
+  // One round of vectors per CTA, asked for before the row's scalars.
+  const uint4 *p = rp.base + threadIdx.x;
+  const int mine = rp.n - (int)threadIdx.x;  // vector j of the thread is there while j kVocThreads < mine
+  uint4 raw[kVocUnroll], edge;
+#pragma unroll
+  for (int j = 0; j < kVocUnroll; j++)
+    if (j * kVocThreads < mine) raw[j] = __ldcs(p + j * kVocThreads);
+  if (threadIdx.x == kFirstThread && rp.first) edge = rv.edge(rp.v0);
+  if (threadIdx.x == kLastThread && rp.last) edge = rv.edge(rp.v1 - 1);
+  const float lse = a.lse[row];
+  const float gh = a.dentropy ? a.dentropy[row] : 0.0f, H = a.dentropy ? a.entropy[row] : 0.0f;
   if (threadIdx.x < 32) {
     bool bad;
     const float s = a.dlogprobs ? given_grad_sum(ids, g, a.T, a.V, bad) : 0.0f;
     if (a.dlogprobs && bad) set_device_error(kDevBadId);
     if (threadIdx.x == 0) s_G = s;
   }
-  const float lse = a.lse[row];
-  const float gh = a.dentropy ? a.dentropy[row] : 0.0f, H = a.dentropy ? a.entropy[row] : 0.0f;
-  __syncthreads();
-  const RowCoef k = row_coef(lse, H, s_G, gh, a.c);
-  const int cfirst = max(rv.col(v0), 0), clast = min(rv.col(v1), a.V);
   // The given tokens' logits are read before any store: dx may be x.
+  const int cfirst = max(rv.col(rp.v0), 0), clast = min(rv.col(rp.v1), a.V);
   float xt = 0.0f;
-  int tid_id = -1;
+  int id = -1;
   if ((int)threadIdx.x < a.T && a.dlogprobs) {
-    tid_id = ids[threadIdx.x];
-    if (tid_id < cfirst || tid_id >= clast) tid_id = -1;
-    if (tid_id >= 0) xt = E::get(rv.row[tid_id]);
+    id = ids[threadIdx.x];
+    if (id < cfirst || id >= clast) id = -1;
+    if (id >= 0) xt = E::get(rv.row[id]);
   }
   __syncthreads();
-  for (int b = v0; b < v1; b += kVocUnroll * kVocThreads) {
-    uint4 raw[kVocUnroll];
+  const RowCoef k = row_coef(lse, H, s_G, gh, a.c);
+  auto grad = [&](const uint4 &v, float *d) {
+    float x[kN];
+    E::unpack(v, x);
 #pragma unroll
-    for (int j = 0; j < kVocUnroll; j++) {
-      const int v = b + j * kVocThreads + (int)threadIdx.x;
-      if (v < v1 && rv.whole(v)) raw[j] = __ldcs(reinterpret_cast<const uint4 *>(rv.row + rv.col(v)));
+    for (int i = 0; i < kN; i += 2) {
+      const float2 r = dense_grad2(make_float2(x[i], x[i + 1]), a.c, k);
+      d[i] = r.x;
+      d[i + 1] = r.y;
     }
+  };
+  T *dp = drow + rv.col(rp.w0) + (int64_t)threadIdx.x * kN;
 #pragma unroll
-    for (int j = 0; j < kVocUnroll; j++) {
-      const int v = b + j * kVocThreads + (int)threadIdx.x;
-      if (v >= v1) continue;
-      float x[kN], d[kN];
-      if (rv.whole(v))
-        E::unpack(raw[j], x);
-      else
-        rv.load_edge(v, x);
-#pragma unroll
-      for (int i = 0; i < kN; i++) d[i] = dense_grad(x[i], a.c, k);
-      store_vec<DT>(drow, rv, v, same, d);
-    }
+  for (int j = 0; j < kVocUnroll; j++) {
+    if (j * kVocThreads >= mine) break;
+    float d[kN];
+    grad(raw[j], d);
+    store_whole<DT>(dp + j * kVocThreads * kN, same, d);
+  }
+  if ((threadIdx.x == kFirstThread && rp.first) || (threadIdx.x == kLastThread && rp.last)) {
+    float d[kN];
+    grad(edge, d);
+    store_edge<DT>(drow, rv, threadIdx.x == kFirstThread ? rp.v0 : rp.v1 - 1, d);
   }
   if (a.T == 0 || !a.dlogprobs) return;
   __syncthreads();
-  if (tid_id >= 0 && lse != -IG_INF) drow[tid_id] = E::put(dense_grad(xt, a.c, k) + token_grad(ids, g, a.T, tid_id, a.c));
+  if (id >= 0 && lse != -IG_INF) drow[id] = E::put(dense_grad(xt, a.c, k) + token_grad(ids, g, a.T, id, a.c));
 }
 
 // ---- divergence from a teacher's top logits ----------------------------------------------
@@ -651,11 +832,11 @@ struct DistillArgs {
   float *loss;
   void *dx;
   int64_t ldd;
+  int parts;  // CTAs per row (a cluster)
 };
 
 __device__ __forceinline__ float block_sum(float v, float *s8) {
-#pragma unroll
-  for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(~0u, v, o);
+  v = warp_sum(v);
   __syncthreads();
   if ((threadIdx.x & 31) == 0) s8[threadIdx.x >> 5] = v;
   __syncthreads();
@@ -676,29 +857,70 @@ __device__ __forceinline__ float block_max(float v, float *s8) {
   return t;
 }
 
-// One cluster per row. With TAIL the mass outside the list is summed on its
-// own (1 - the list's mass would lose it to cancellation): a bit per vector
-// in shared memory says whether the vector holds listed columns, and those
-// vectors (at most K) compare their columns with the list. The second pass
-// writes the gradient while the row is still in L2.
-template <int DT, bool TAIL>
+// One cluster per row. The row's part is copied to shared memory in four bulk
+// copies (STAGED), so the statistics' pass starts on the first quarter and the
+// gradient's pass reads no global memory; rows too long for that (over 8 x
+// kStageMax bytes) are read twice, the second time from L2. With TAIL the mass
+// outside the list is summed on its own (1 - the list's mass would lose it to
+// cancellation): a bit per vector in shared memory says whether the vector
+// holds listed columns, and those vectors (at most K) compare their columns
+// with the list.
+constexpr int kStageParts = 4;
+constexpr int kStageMax = 160 * 1024;
+
+__device__ __forceinline__ void bulk_load(void *dst, const void *src, uint32_t bytes, uint64_t *bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+                   smem_u32(dst)),
+               "l"(src), "r"(bytes), "r"(smem_u32(bar))
+               : "memory");
+}
+
+template <int DT, bool TAIL, bool STAGED>
 __global__ void __launch_bounds__(kVocThreads, 4) distill_topk_kernel(const DistillArgs a) {
   using E = VElem<DT>;
   using T = typename E::T;
-  constexpr int kN = E::kN, kX = kN * kVocUnroll;
-  extern __shared__ uint32_t s_bits[];
+  constexpr int kN = E::kN;
+  constexpr int kR = 2;  // vectors per thread and step
+  extern __shared__ uint4 s_dyn[];
   __shared__ VStat s_warp[kVocWarps];
-  __shared__ VStat s_cta;
+  __shared__ VStat s_part[8];  // every CTA's statistics
   __shared__ float s8[kVocWarps];
   __shared__ int s_ids[kTeacherMax];
   __shared__ float s_q[kTeacherMax];
-  cg::cluster_group cl = cg::this_cluster();
-  const int cs = (int)cl.num_blocks(), rank = (int)cl.block_rank();
+  __shared__ float s_xk[kTeacherMax];
+  __shared__ __align__(8) uint64_t s_bar[kStageParts + 1];
+  const int cs = a.parts, rank = cs > 1 ? (int)cluster_ctarank() : 0;
   const int64_t row = blockIdx.x / cs;
   const RowVecs<DT> rv(static_cast<const T *>(a.x) + row * a.ld, a.V);
-  const int v0 = (int)((int64_t)rv.nv * rank / cs), v1 = (int)((int64_t)rv.nv * (rank + 1) / cs);
+  const RowPart<DT> rp(rv, rank, cs);
   const int tid = (int)threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const float c2 = a.c * kLog2e;
+  uint32_t *s_bits = reinterpret_cast<uint32_t *>(s_dyn + (STAGED ? rp.n : 0));  // one per vector v0 + i
+  // Quarters of whole steps.
+  constexpr int kStep = kR * kVocThreads;
+  const int quarter = ((rp.n + kStageParts - 1) / kStageParts + kStep - 1) / kStep * kStep;
+  if (tid == 0) {
+    for (int i = 0; i <= kStageParts; i++) mbar_init(&s_bar[i], 1);
+    fence_barrier_init();
+    mbar_arrive_expect_tx(&s_bar[kStageParts], (uint32_t)(cs - 1) * 8u);
+    if constexpr (STAGED) {
+      fence_proxy_async_smem();
+      for (int i = 0; i < kStageParts; i++) {
+        const int p0 = i * quarter, p1 = min(p0 + quarter, rp.n);
+        const uint32_t bytes = p1 > p0 ? (uint32_t)(p1 - p0) * 16u : 0u;
+        mbar_arrive_expect_tx(&s_bar[i], bytes);
+        if (bytes) bulk_load(s_dyn + p0, rp.base + p0, bytes, &s_bar[i]);
+      }
+    }
+  }
+  __syncwarp();
+  if (cs > 1) cluster_announce();
+  const uint4 *src = STAGED ? s_dyn : rp.base;
+  uint4 edge;
+  const bool has_edge = (tid == kFirstThread && rp.first) || (tid == kLastThread && rp.last);
+  const int edge_v = tid == kFirstThread ? rp.v0 : rp.v1 - 1;
+  if (has_edge) edge = rv.edge(edge_v);
+
   const float w = a.weights ? a.weights[row] : 1.0f;
   T *drow = a.dx ? static_cast<T *>(a.dx) + row * a.ldd : nullptr;
   const bool same = (reinterpret_cast<uintptr_t>(drow) & 15) == (reinterpret_cast<uintptr_t>(rv.row) & 15);
@@ -716,10 +938,11 @@ __global__ void __launch_bounds__(kVocThreads, 4) distill_topk_kernel(const Dist
     if (id < 0) id = -1;
     s_ids[tid] = id;
     if (id >= 0) xk = E::get(rv.row[id]);
+    s_xk[tid] = xk;
   }
   const int any = __syncthreads_or(id >= 0);
   const bool skip = !any || w == 0.0f;  // uniform over the cluster
-  const int cfirst = max(rv.col(v0), 0), clast = min(rv.col(v1), a.V);
+  const int cfirst = max(rv.col(rp.v0), 0), clast = min(rv.col(rp.v1), a.V);
   VStat st{-IG_INF, 0.0f, 0.0f};
   float q_rest = 0.0f;
   if (!skip) {
@@ -733,11 +956,11 @@ __global__ void __launch_bounds__(kVocThreads, 4) distill_topk_kernel(const Dist
       q = id >= 0 ? expf(t) : 0.0f;
       const float q_list = block_sum(q, s8);
       q_rest = q_list == q_list ? fmaxf(1.0f - q_list, 0.0f) : q_list;
-      const int nw = (v1 - v0 + 31) / 32;
+      const int nw = (rp.v1 - rp.v0 + 31) / 32;
       for (int i = tid; i < nw; i += kVocThreads) s_bits[i] = 0;
       __syncthreads();
       if (id >= cfirst && id < clast) {
-        const int v = (id + rv.mis) / kN - v0;
+        const int v = (id + rv.mis) / kN - rp.v0;
         atomicOr(&s_bits[v >> 5], 1u << (v & 31));
       }
       __syncthreads();
@@ -747,54 +970,66 @@ __global__ void __launch_bounds__(kVocThreads, 4) distill_topk_kernel(const Dist
       const float sum = block_sum(q, s8);
       if (sum > 0.0f || sum != sum) q /= sum;
     }
-    for (int b = v0; b < v1; b += kVocUnroll * kVocThreads) {
-      float x[kX];
-      uint4 raw[kVocUnroll];
+    // A vector as the statistics see it: the listed columns are left out of the tail's.
+    auto unlisted = [&](uint4 raw, int v) {
+      if constexpr (TAIL) {
+        const int i = v - rp.v0;
+        if (s_bits[i >> 5] >> (i & 31) & 1u) {
+          float x[kN];
+          E::unpack(raw, x);
+          for (int k = 0; k < a.K; k++) {
+            const int at = s_ids[k] - rv.col(v);
 #pragma unroll
-      for (int j = 0; j < kVocUnroll; j++) {
-        const int v = b + j * kVocThreads + tid;
-        if (v < v1 && rv.whole(v)) raw[j] = *reinterpret_cast<const uint4 *>(rv.row + rv.col(v));
-      }
-#pragma unroll
-      for (int j = 0; j < kVocUnroll; j++) {
-        const int v = b + j * kVocThreads + tid;
-        if (v < v1 && rv.whole(v)) {
-          E::unpack(raw[j], x + j * kN);
-        } else if (v < v1) {
-          rv.load_edge(v, x + j * kN);
-        } else {
-#pragma unroll
-          for (int i = 0; i < kN; i++) x[j * kN + i] = -IG_INF;
-        }
-        if constexpr (TAIL) {
-          if (v < v1 && (s_bits[(v - v0) >> 5] >> ((v - v0) & 31) & 1u)) {
-            for (int k = 0; k < a.K; k++) {
-              const int at = s_ids[k] - rv.col(v);
-#pragma unroll
-              for (int i = 0; i < kN; i++)
-                if (at == i) x[j * kN + i] = -IG_INF;
-            }
+            for (int e = 0; e < kN; e++)
+              if (at == e) x[e] = -IG_INF;
           }
+          raw = E::pack(x);
         }
       }
-      float mx = x[0];
+      return raw;
+    };
+    for (int b = 0; b < rp.n; b += quarter) {
+      if constexpr (STAGED) mbar_wait(&s_bar[b / quarter], 0, kDevTimeoutFull);
+      const int end = min(b + quarter, rp.n);
+      int i = b + tid;
+      for (; i + kStep - kVocThreads < end; i += kStep) {
+        uint4 raw[kR];
 #pragma unroll
-      for (int i = 1; i < kX; i++) mx = fmaxf(mx, x[i]);
-      mx = fmaxf(mx, -IG_INF);
-      vstat_add<false>(st, x, mx, c2);
+        for (int j = 0; j < kR; j++) raw[j] = unlisted(src[i + j * kVocThreads], rp.w0 + i + j * kVocThreads);
+        vstat_add_raw<DT, false>(st, raw, c2);
+      }
+      for (; i < end; i += kVocThreads) {
+        const uint4 raw[1] = {unlisted(src[i], rp.w0 + i)};
+        vstat_add_raw<DT, false>(st, raw, c2);
+      }
+    }
+    if (has_edge) {
+      const uint4 raw[1] = {unlisted(edge, edge_v)};
+      vstat_add_raw<DT, false>(st, raw, c2);
     }
     st = vstat_warp<false>(st, c2);
     if (lane == 0) s_warp[warp] = st;
     __syncthreads();
-    st = s_warp[0];
-    for (int i = 1; i < kVocWarps; i++) vstat_merge<false>(st, s_warp[i], c2);
+    st = vstat_join<false>(s_warp, kVocWarps, c2);
+  } else if constexpr (STAGED) {
+    // The copies end before this CTA does.
+    for (int i = 0; i < kStageParts; i++) mbar_wait(&s_bar[i], 0, kDevTimeoutFull);
   }
   if (cs > 1) {
-    if (tid == 0) s_cta = st;
-    cl.sync();
-    st = *cl.map_shared_rank(&s_cta, 0);
-    for (int r = 1; r < cs; r++) vstat_merge<false>(st, *cl.map_shared_rank(&s_cta, r), c2);
-    cl.sync();  // every CTA has read the others' statistics (and the list's logits) before any stores or exits
+    // Every CTA hands its statistics to every other one. (Each has its list's
+    // logits in s_xk by then, so the others may overwrite the row: dx may be x.)
+    cluster_ready();
+    if (tid < cs) {
+      if (tid == rank) {
+        s_part[rank] = st;
+      } else {
+        st_async_f32(&s_part[rank].m, tid, st.m, &s_bar[kStageParts]);
+        st_async_f32(&s_part[rank].s, tid, st.s, &s_bar[kStageParts]);
+      }
+    }
+    mbar_wait_cluster(&s_bar[kStageParts], 0, kDevTimeoutFull);
+    __syncthreads();
+    st = vstat_join<false>(s_part, cs, c2);
   }
   // Dense gradient: coef 2^((x - mb) c2 - l2); a listed column: listed p - w c q.
   float coef = 0.0f, listed = 0.0f, pk = 0.0f;
@@ -840,30 +1075,46 @@ __global__ void __launch_bounds__(kVocThreads, 4) distill_topk_kernel(const Dist
   }
   if (!drow) return;
   const bool zero = skip || st.s == 0.0f;
-  for (int b = v0; b < v1; b += kVocUnroll * kVocThreads) {
-    uint4 raw[kVocUnroll];
+  if (cs == 1) __syncthreads();  // the list's logits are read before any store: dx may be x
+  const float2 nm = make_float2(-mb, -mb), cc = make_float2(c2, c2), nl = make_float2(-l2, -l2);
+  auto grad = [&](const uint4 &v, float *d) {
+    float x[kN];
+    E::unpack(v, x);
 #pragma unroll
-    for (int j = 0; j < kVocUnroll; j++) {
-      const int v = b + j * kVocThreads + tid;
-      if (!zero && v < v1 && rv.whole(v)) raw[j] = __ldcs(reinterpret_cast<const uint4 *>(rv.row + rv.col(v)));
+    for (int e = 0; e < kN; e += 2) {
+      const float2 y = __ffma2_rn(__fadd2_rn(make_float2(x[e], x[e + 1]), nm), cc, nl);
+      const float2 r = __fmul2_rn(make_float2(ex2(y.x), ex2(y.y)), make_float2(coef, coef));
+      d[e] = r.x;
+      d[e + 1] = r.y;
     }
+  };
+  T *dp = drow + rv.col(rp.w0);
+  if (zero) {
+    float d[kN] = {};
+    for (int i = tid; i < rp.n; i += kVocThreads) store_whole<DT>(dp + (int64_t)i * kN, same, d);
+    if (has_edge) store_edge<DT>(drow, rv, edge_v, d);
+  } else {
+    int i = tid;
+    for (; i + kStep - kVocThreads < rp.n; i += kStep) {
+      uint4 raw[kR];
 #pragma unroll
-    for (int j = 0; j < kVocUnroll; j++) {
-      const int v = b + j * kVocThreads + tid;
-      if (v >= v1) continue;
-      float x[kN], d[kN];
-      if (zero) {
+      for (int j = 0; j < kR; j++) raw[j] = src[i + j * kVocThreads];
 #pragma unroll
-        for (int i = 0; i < kN; i++) d[i] = 0.0f;
-      } else {
-        if (rv.whole(v))
-          E::unpack(raw[j], x);
-        else
-          rv.load_edge(v, x);
-#pragma unroll
-        for (int i = 0; i < kN; i++) d[i] = coef * ex2(fmaf(x[i] - mb, c2, -l2));
+      for (int j = 0; j < kR; j++) {
+        float d[kN];
+        grad(raw[j], d);
+        store_whole<DT>(dp + (int64_t)(i + j * kVocThreads) * kN, same, d);
       }
-      store_vec<DT>(drow, rv, v, same, d);
+    }
+    for (; i < rp.n; i += kVocThreads) {
+      float d[kN];
+      grad(src[i], d);
+      store_whole<DT>(dp + (int64_t)i * kN, same, d);
+    }
+    if (has_edge) {
+      float d[kN];
+      grad(edge, d);
+      store_edge<DT>(drow, rv, edge_v, d);
     }
   }
   if (zero) return;
@@ -909,30 +1160,42 @@ static cudaError_t launch_rows(void (*kern)(Args), const Args &a, int64_t rows, 
 }
 
 template <int DT>
-static cudaError_t run_token_logprobs(const LogprobArgs &a, cudaStream_t st) {
-  const int cs = row_parts(a.rows, a.V, VElem<DT>::kN);
+static cudaError_t run_token_logprobs(LogprobArgs a, cudaStream_t st) {
+  const int cs = a.parts = row_parts(a.rows, a.V, VElem<DT>::kN);
   return a.K > 0 ? launch_rows(token_logprobs_kernel<DT, true>, a, a.rows, cs, 0, st)
                  : launch_rows(token_logprobs_kernel<DT, false>, a, a.rows, cs, 0, st);
 }
 
 template <int DT>
 static cudaError_t run_token_logprobs_grad(LogprobGradArgs a, cudaStream_t st) {
-  const int64_t nv = (a.V + VElem<DT>::kN - 1) / VElem<DT>::kN;
+  const int64_t nv = (a.V + VElem<DT>::kN - 1) / VElem<DT>::kN + 1;  // a row off the boundary spans one more
   const int64_t round = kVocUnroll * kVocThreads;
   a.segs = (int)((nv + round - 1) / round);
   return launch_rows(token_logprobs_grad_kernel<DT>, a, a.rows * a.segs, 1, 0, st);
 }
 
-template <int DT>
-static cudaError_t run_distill(const DistillArgs &a, bool tail, cudaStream_t st) {
-  const int cs = row_parts(a.rows, a.V, VElem<DT>::kN);
-  if (!tail) return launch_rows(distill_topk_kernel<DT, false>, a, a.rows, cs, 0, st);
-  const int64_t nv = a.V / VElem<DT>::kN + 2;
-  const size_t smem = ((nv / cs + 1 + 31) / 32 + 1) * 4;
+template <int DT, bool TAIL, bool STAGED>
+static cudaError_t launch_distill(const DistillArgs &a, int cs, size_t smem, cudaStream_t st) {
   static SmemOptIn attr;
-  const cudaError_t e = attr.ensure((const void *)distill_topk_kernel<DT, true>, (int)smem);
+  const cudaError_t e = attr.ensure((const void *)distill_topk_kernel<DT, TAIL, STAGED>, (int)smem);
   if (e != cudaSuccess) return e;
-  return launch_rows(distill_topk_kernel<DT, true>, a, a.rows, cs, smem, st);
+  return launch_rows(distill_topk_kernel<DT, TAIL, STAGED>, a, a.rows, cs, smem, st);
+}
+
+template <int DT>
+static cudaError_t run_distill(DistillArgs a, bool tail, cudaStream_t st) {
+  const int64_t nv = a.V / VElem<DT>::kN + 2;
+  int cs = row_parts(a.rows, a.V, VElem<DT>::kN);
+  // Parts of at most 52 KB where the cluster allows it: four CTAs per SM.
+  while (cs < 8 && nv * 16 / cs > 52 * 1024) cs *= 2;
+  a.parts = cs;
+  const int64_t part = nv / cs + 1;
+  const bool staged = part * 16 <= kStageMax;
+  const size_t bits = tail ? ((part + 31) / 32 + 1) * 4 : 0;
+  const size_t smem = bits + (staged ? part * 16 : 0);
+  if (staged)
+    return tail ? launch_distill<DT, true, true>(a, cs, smem, st) : launch_distill<DT, false, true>(a, cs, smem, st);
+  return tail ? launch_distill<DT, true, false>(a, cs, smem, st) : launch_distill<DT, false, false>(a, cs, smem, st);
 }
 
 }  // namespace ig

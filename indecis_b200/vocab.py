@@ -46,15 +46,39 @@ def _dense(t, dtype, shape, like, name):
     return t.data_ptr()
 
 
+# The current stream's handle. torch.cuda.current_stream builds a Stream object
+# on every call (3 us); torch's own generated code takes the raw handle.
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+    lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+
 def _call(like, fn, *args):
     """fn on the current stream of like's device."""
-    if like.device.index == torch.cuda.current_device():
-        rc = fn(*args, torch.cuda.current_stream().cuda_stream)
+    index = like.device.index
+    if index == torch.cuda.current_device():
+        rc = fn(*args, _raw_stream(index))
     else:
-        with torch.cuda.device(like.device):
-            rc = fn(*args, torch.cuda.current_stream().cuda_stream)
+        with torch.cuda.device(index):
+            rc = fn(*args, _raw_stream(index))
     if rc:
         _capi.check(rc)
+
+
+def _outputs(like, N, T, K):
+    """The forward's outputs as pieces of one float32 allocation (top_ids of its own), and the addresses of logprobs,
+    lse, entropy, top_ids and top_logprobs. (Taken from the allocation: the data_ptr of an empty piece is 0.)"""
+    K = max(K, 0)  # a negative top_k is refused by the call
+    buf = torch.empty(N * (T + 2 + K), dtype=torch.float32, device=like.device)
+    base, n = buf.data_ptr(), N * T
+    tl = ti = None
+    if K > 0:
+        tl = buf.as_strided((N, K), (K, 1), n + 2 * N)
+        ti = torch.empty((N, K), dtype=torch.int32, device=like.device)
+    r = TokenLogProbs(buf.as_strided((N, T), (T, 1)), buf.as_strided((N,), (1,), n), buf.as_strided((N,), (1,), n + N), ti,
+                      tl)
+    ptrs = (base, base + 4 * n, base + 4 * (n + N), ti.data_ptr() if K > 0 else None,
+            base + 4 * (n + 2 * N) if K > 0 else None)
+    return r, ptrs
 
 
 def token_logprobs(logits, ids, temperature=1.0, top_k=0) -> TokenLogProbs:
@@ -67,16 +91,10 @@ def token_logprobs(logits, ids, temperature=1.0, top_k=0) -> TokenLogProbs:
         raise ValueError("ids: expected a matrix")
     T = ids.shape[1]
     pid = _dense(ids, torch.int32, (N, T), logits, "ids")
-    dev = logits.device
-    lp = torch.empty((N, T), dtype=torch.float32, device=dev)
-    lse = torch.empty(N, dtype=torch.float32, device=dev)
-    ent = torch.empty(N, dtype=torch.float32, device=dev)
-    ti = torch.empty((N, top_k), dtype=torch.int32, device=dev) if top_k > 0 else None
-    tl = torch.empty((N, top_k), dtype=torch.float32, device=dev) if top_k > 0 else None
-    _call(logits, _capi.load().ig_token_logprobs, logits.data_ptr(), _DT[logits.dtype], ld, N, V, temperature, pid, T,
-          lp.data_ptr(), lse.data_ptr(), ent.data_ptr(), top_k, ti.data_ptr() if ti is not None else None,
-          tl.data_ptr() if tl is not None else None)
-    return TokenLogProbs(lp, lse, ent, ti, tl)
+    r, (lp, lse, ent, ti, tl) = _outputs(logits, N, T, top_k)
+    _call(logits, _capi.load().ig_token_logprobs, logits.data_ptr(), _DT[logits.dtype], ld, N, V, temperature, pid, T, lp,
+          lse, ent, top_k, ti, tl)
+    return r
 
 
 def token_logprobs_backward(logits, ids, lse, entropy, dlogprobs, dentropy=None, temperature=1.0, out=None):
@@ -174,17 +192,11 @@ def vocab_logprobs(hidden, weight, ids, temperature=1.0, top_k=0) -> TokenLogPro
         raise ValueError("ids: expected a matrix")
     T = ids.shape[1]
     pid = _dense(ids, torch.int32, (N, T), hidden, "ids")
-    dev = hidden.device
-    lp = torch.empty((N, T), dtype=torch.float32, device=dev)
-    lse = torch.empty(N, dtype=torch.float32, device=dev)
-    ent = torch.empty(N, dtype=torch.float32, device=dev)
-    ti = torch.empty((N, top_k), dtype=torch.int32, device=dev) if top_k > 0 else None
-    tl = torch.empty((N, top_k), dtype=torch.float32, device=dev) if top_k > 0 else None
-    ws = _workspace(hidden, N, V, H, top_k, 0)
+    r, (lp, lse, ent, ti, tl) = _outputs(hidden, N, T, top_k)
+    ws = _workspace(hidden, N, V, H, max(top_k, 0), 0)
     _call(hidden, _capi.load().ig_vocab_logprobs, hidden.data_ptr(), ldh, weight.data_ptr(), ldw, _DT[hidden.dtype], N, V,
-          H, temperature, pid, T, lp.data_ptr(), lse.data_ptr(), ent.data_ptr(), top_k,
-          ti.data_ptr() if ti is not None else None, tl.data_ptr() if tl is not None else None, ws.data_ptr(), ws.numel())
-    return TokenLogProbs(lp, lse, ent, ti, tl)
+          H, temperature, pid, T, lp, lse, ent, top_k, ti, tl, ws.data_ptr(), ws.numel())
+    return r
 
 
 def vocab_logprobs_backward(hidden, weight, ids, logprobs, lse, entropy, dlogprobs, dentropy=None, temperature=1.0,
