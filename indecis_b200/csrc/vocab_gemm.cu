@@ -5,7 +5,10 @@
 // One persistent kernel serves the four products:
 //   statistics  rows x vocab, K = hidden: the epilogue keeps each row's
 //               running (m, s, u) (vocab_rows.cu) in registers over the
-//               column tiles of its unit and writes one partial per unit;
+//               column tiles of its unit and writes one partial per unit, and
+//               for the alternatives the maximum of every 16 columns: the K
+//               best columns lie in the K best groups, whose logits the
+//               joining kernel computes again (16 K dot products a row);
 //   dZ          the same product again (a row's logits cost less to compute
 //               than to store and read back), turned into the gradient of the
 //               logits, rounded to the operands' type and stored;
@@ -31,7 +34,7 @@
 
 namespace ig {
 
-enum VEpi : int { kVStats = 0, kVStatsTop = 1, kVDz = 2, kVOut = 3 };
+enum VEpi : int { kVStats = 0, kVDz = 1, kVOut = 2 };
 
 constexpr int kVBN = 256;   // tile columns
 constexpr int kVBK = 64;    // 16-bit elements of K per stage (128 bytes)
@@ -43,36 +46,53 @@ struct VRowCoef {
   float A, B, lse, pad;
 };
 
+constexpr int kVGroup = 16;  // columns per stored maximum
+
 struct VGemmArgs {
-  int M, N, K;
+  int M, N;
+  int kblocks;  // blocks of kVBK of K
+  int kwrap;    // blocks from this one on read A's second part, `shift` elements further along its rows, and B from the start
+  int shift;
   uint32_t idesc;
   int units_m, units_n, units_s;  // units: M tiles x N parts x K parts
   int n_fastest;                  // unit order: N parts innermost, else M tiles
-  // kVStats, kVStatsTop: [units_n * 2][M] partials
+  // kVStats: [M][units_n * 2] partials; group maxima [M][ldmax] or NULL
   float c2;
   float4 *part;
-  int top_k;
-  float *top_val;
-  int32_t *top_col;  // [units_n * 2][M][top_k]
+  float *gmax;
+  int64_t ldmax;
   // kVDz
   float c;
   const VRowCoef *coef;
-  const float *scale;  // 2^k applied to dZ (power of two), removed from the outputs
-  // kVDz, kVOut: dtype of the 16-bit output
+  int split;  // dZ as two 16-bit parts, the second `shift` elements on
+  // kVDz, kVOut: dtype of the 16-bit output; bits of dZ's bound (vocab_scale), NULL: unscaled
   int dtype;
-  // kVOut: out16 (final) or part32 [units_s][M][N] (accumulate: added to what is there)
+  const int *bound;
+  // kVOut: out16 (final) or part32 [units_s][M][ldo] (accumulate: added to what is there)
   void *out16;
   int64_t ldo;
   float *part32;
   int accumulate;
 };
 
+// float16 has 5 exponent bits: dZ is scaled by a power of two that brings the
+// largest bound of the rows to 2^14..2^15, so that probabilities down to
+// 2^-28 of it keep all their bits; the products' float32 sums are scaled
+// back. bfloat16 has float32's range and needs none.
+__device__ __forceinline__ float vocab_scale(const int *bound) {
+  if (!bound) return 1.0f;
+  const int b = *bound;
+  if (b <= 0) return 1.0f;
+  const int e = min(max(14 - (((b >> 23) & 255) - 127), -100), 100);
+  return __int_as_float((e + 127) << 23);
+}
+
 template <int CG, int EPI>
 struct VSmem {
   static constexpr int kABytes = 128 * kVBK * 2;
   static constexpr int kBBytes = (kVBN / CG) * kVBK * 2;
   static constexpr int kStageBytes = kABytes + kBBytes;
-  static constexpr int kExtra = EPI == kVStatsTop ? 32 * kVEpiWarps * kTopMax * 8 : EPI == kVDz ? kVEpiWarps * 2 * 2048 : 0;
+  static constexpr int kExtra = EPI == kVDz ? kVEpiWarps * 2 * 2048 : 0;  // two staging buffers per warp
   static constexpr int kRaw = (224 * 1024 - kExtra) / kStageBytes;
   static constexpr int kStages = kRaw > 6 ? 6 : kRaw;
   static constexpr int kExtraOff = kStages * kStageBytes;
@@ -125,8 +145,7 @@ struct VUnit {
   int n0, n1;     // column tiles
   int k0, k1;     // K blocks
 };
-template <int EPI>
-__device__ __forceinline__ VUnit vunit(const VGemmArgs &a, int u, int ntiles, int kblocks) {
+__device__ __forceinline__ VUnit vunit(const VGemmArgs &a, int u, int ntiles) {
   VUnit r;
   if (a.n_fastest) {
     r.n = u % a.units_n;
@@ -141,23 +160,18 @@ __device__ __forceinline__ VUnit vunit(const VGemmArgs &a, int u, int ntiles, in
   }
   r.n0 = (int)((int64_t)ntiles * r.n / a.units_n);
   r.n1 = (int)((int64_t)ntiles * (r.n + 1) / a.units_n);
-  r.k0 = (int)((int64_t)kblocks * r.s / a.units_s);
-  r.k1 = (int)((int64_t)kblocks * (r.s + 1) / a.units_s);
+  r.k0 = (int)((int64_t)a.kblocks * r.s / a.units_s);
+  r.k1 = (int)((int64_t)a.kblocks * (r.s + 1) / a.units_s);
   return r;
 }
 
-// Inserts (v, col) into a thread's descending list of K (slot k at k *
-// stride); columns come in increasing order, so equal values stay behind.
-__device__ __noinline__ float list_insert(float *val, int *col, int stride, int K, float v, int c) {
-  int k = K - 1;
-  while (k > 0 && val[(k - 1) * stride] < v) {
-    val[k * stride] = val[(k - 1) * stride];
-    col[k * stride] = col[(k - 1) * stride];
-    k--;
-  }
-  val[k * stride] = v;
-  col[k * stride] = c;
-  return val[(K - 1) * stride];
+__device__ __forceinline__ float2 widen2(uint32_t v, int dtype) {
+  if (dtype == IG_DT_BF16) return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xFFFF0000u));
+  return __half22float2(*reinterpret_cast<const __half2 *>(&v));
+}
+__device__ __forceinline__ float widen1(uint16_t v, int dtype) {
+  if (dtype == IG_DT_BF16) return __uint_as_float((uint32_t)v << 16);
+  return __half2float(*reinterpret_cast<const __half *>(&v));
 }
 
 __device__ __forceinline__ uint32_t pack16(float a, float b, int dtype) {
@@ -193,7 +207,6 @@ __global__ void __launch_bounds__(kVGemmThreads, 1)
   const int rank = CG == 2 ? (int)cluster_ctarank() : 0;
   const int first = blockIdx.x / CG, step = gridDim.x / CG;
   const int ntiles = (a.N + kVBN - 1) / kVBN;
-  const int kblocks = (a.K + kVBK - 1) / kVBK;
   const int units = a.units_m * a.units_n * a.units_s;
 
   if (warp == 0 && lane == 0) {
@@ -229,7 +242,7 @@ __global__ void __launch_bounds__(kVGemmThreads, 1)
       int it = 0;
       bool ok = true;
       for (int u = first; u < units && ok; u += step) {
-        const VUnit q = vunit<EPI>(a, u, ntiles, kblocks);
+        const VUnit q = vunit(a, u, ntiles);
         const int m0 = q.m * (CG * 128) + rank * 128;
         for (int n = q.n0; n < q.n1 && ok; n++) {
           const int n0 = n * kVBN + rank * (kVBN / CG);
@@ -247,17 +260,19 @@ __global__ void __launch_bounds__(kVGemmThreads, 1)
               else
                 tma_load_2d(map, dst, &full[s], c0, c1);
             };
+            const bool second = kb >= a.kwrap;
+            const int kc = (second ? kb - a.kwrap : kb) * kVBK, as = second ? a.shift : 0;
             if constexpr (A_MN) {
 #pragma unroll
-              for (int i = 0; i < 2; i++) load(&mapA, sa + i * 8192, m0 + i * 64, kb * kVBK);
+              for (int i = 0; i < 2; i++) load(&mapA, sa + i * 8192, as + m0 + i * 64, kc);
             } else {
-              load(&mapA, sa, kb * kVBK, m0);
+              load(&mapA, sa, as + kc, m0);
             }
             if constexpr (B_MN) {
 #pragma unroll
-              for (int i = 0; i < kVBN / CG / 64; i++) load(&mapB, sb + i * 8192, n0 + i * 64, kb * kVBK);
+              for (int i = 0; i < kVBN / CG / 64; i++) load(&mapB, sb + i * 8192, n0 + i * 64, kc);
             } else {
-              load(&mapB, sb, kb * kVBK, n0);
+              load(&mapB, sb, kc, n0);
             }
           }
         }
@@ -273,7 +288,7 @@ __global__ void __launch_bounds__(kVGemmThreads, 1)
       int it = 0, tile = 0;
       bool ok = true;
       for (int u = first; u < units && ok; u += step) {
-        const VUnit q = vunit<EPI>(a, u, ntiles, kblocks);
+        const VUnit q = vunit(a, u, ntiles);
         for (int n = q.n0; n < q.n1 && ok; n++, tile++) {
           const int b = tile & 1;
           if (!mbar_wait(&acce[b], ((tile >> 1) & 1) ^ 1, kDevTimeoutEmpty)) {
@@ -314,38 +329,26 @@ __global__ void __launch_bounds__(kVGemmThreads, 1)
       }
     }
   } else {
-    const int q4 = warp & 3, e = warp - 2, g = e >> 2;  // TMEM lane quarter; column chunks g, g + 2, ...
+    const int q4 = warp & 3, e = warp - 2, g = e >> 2;  // TMEM lane quarter; columns [128 g, 128 g + 128)
     int tile = 0;
     bool ok = true;
     [[maybe_unused]] int stores = 0;
     for (int u = first; u < units && ok; u += step) {
-      const VUnit q = vunit<EPI>(a, u, ntiles, kblocks);
+      const VUnit q = vunit(a, u, ntiles);
       const int row0 = q.m * (CG * 128) + rank * 128 + q4 * 32, row = row0 + lane;
       const bool warp_live = row0 < a.M, live = row < a.M;
       [[maybe_unused]] VStat st{-IG_INF, 0.0f, 0.0f};
-      [[maybe_unused]] float thr = -IG_INF;
-      [[maybe_unused]] float *lval = nullptr;
-      [[maybe_unused]] int *lcol = nullptr;
-      constexpr int kLs = 32 * kVEpiWarps;  // list slot stride
-      if constexpr (EPI == kVStatsTop) {
-        lval = reinterpret_cast<float *>(smem + S::kExtraOff) + e * 32 + lane;
-        lcol = reinterpret_cast<int *>(lval) + kLs * kTopMax;
-        for (int k = 0; k < a.top_k; k++) {
-          lval[k * kLs] = -IG_INF;
-          lcol[k * kLs] = -1;
-        }
-      }
       [[maybe_unused]] RowCoef rc{0.0f, 0.0f, IG_INF};
       if constexpr (EPI == kVDz) {
         if (live) {
           const VRowCoef v = a.coef[row];
-          const float sc = __ldg(a.scale);
+          const float sc = vocab_scale(a.bound);
           rc = RowCoef{v.A * sc, v.B * sc, v.lse};
         }
       }
       [[maybe_unused]] float unscale = 1.0f;
       if constexpr (EPI == kVOut) {
-        if (a.out16 && a.scale) unscale = 1.0f / __ldg(a.scale);
+        if (a.out16) unscale = 1.0f / vocab_scale(a.bound);
       }
       for (int n = q.n0; n < q.n1; n++, tile++) {
         const int b = tile & 1;
@@ -371,57 +374,83 @@ __global__ void __launch_bounds__(kVGemmThreads, 1)
         const uint32_t tb = tmem + b * kVBN + ((uint32_t)(q4 * 32) << 16);
         constexpr int kChunks = kVBN / 64;
         uint32_t r[2][32];
-        tmem_ld_32x32b_x32(tb + g * 32, r[0]);
+        [[maybe_unused]] float gm[2 * kChunks];
+        tmem_ld_32x32b_x32(tb + g * 128, r[0]);
 #pragma unroll
         for (int i = 0; i < kChunks; i++) {
           __syncwarp();  // the branches below are per lane; the TMEM loads take the whole warp
           tmem_ld_wait();
           if (i + 1 < kChunks)
-            tmem_ld_32x32b_x32(tb + g * 32 + 64 * (i + 1), r[(i + 1) & 1]);
+            tmem_ld_32x32b_x32(tb + g * 128 + 32 * (i + 1), r[(i + 1) & 1]);
           else
             release();
-          const int col0 = n * kVBN + g * 32 + 64 * i;
-          if (col0 >= a.N) continue;
+          const int col0 = n * kVBN + g * 128 + 32 * i;
+          if constexpr (EPI != kVDz) {
+            if (col0 >= a.N) {
+              if constexpr (EPI == kVStats) gm[2 * i] = gm[2 * i + 1] = -IG_INF;
+              continue;
+            }
+          }
           float x[32];
 #pragma unroll
           for (int k = 0; k < 32; k++) x[k] = __uint_as_float(r[i & 1][k]);
-          if constexpr (EPI == kVStats || EPI == kVStatsTop) {
+          if constexpr (EPI == kVStats) {
             if (col0 + 32 > a.N) {
 #pragma unroll
               for (int k = 0; k < 32; k++)
                 if (col0 + k >= a.N) x[k] = -IG_INF;
             }
-            float m4[4] = {x[0], x[1], x[2], x[3]};
+            float m4[4] = {x[0], x[1], x[16], x[17]};
 #pragma unroll
-            for (int k = 4; k < 32; k++) m4[k & 3] = fmaxf(m4[k & 3], x[k]);
-            const float mx = fmaxf(fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])), -IG_INF);
-            vstat_add<true>(st, x, mx, a.c2);
-            if constexpr (EPI == kVStatsTop) {
-              if (live && mx > thr) {
-#pragma unroll
-                for (int k = 0; k < 32; k++)
-                  if (x[k] > thr) thr = list_insert(lval, lcol, kLs, a.top_k, x[k], col0 + k);
-              }
+            for (int k = 2; k < 16; k += 2) {
+              m4[0] = fmaxf(m4[0], x[k]);
+              m4[1] = fmaxf(m4[1], x[k + 1]);
+              m4[2] = fmaxf(m4[2], x[k + 16]);
+              m4[3] = fmaxf(m4[3], x[k + 17]);
             }
+            gm[2 * i] = fmaxf(fmaxf(m4[0], m4[1]), -IG_INF);
+            gm[2 * i + 1] = fmaxf(fmaxf(m4[2], m4[3]), -IG_INF);
+            vstat_add<true>(st, x, fmaxf(gm[2 * i], gm[2 * i + 1]), a.c2);
           } else if constexpr (EPI == kVDz) {
-            uint8_t *buf = smem + S::kExtraOff + (e * 2 + (stores & 1)) * 2048;
-            if (lane == 0) bulk_wait_read<1>();
-            __syncwarp();
-            uint32_t w[16];
+            float d[32];
 #pragma unroll
-            for (int k = 0; k < 16; k++)
-              w[k] = pack16(dense_grad(x[2 * k], a.c, rc), dense_grad(x[2 * k + 1], a.c, rc), a.dtype);
-#pragma unroll
-            for (int j = 0; j < 4; j++)
-              *reinterpret_cast<uint4 *>(buf + lane * 64 + ((j ^ ((lane >> 1) & 3)) << 4)) =
-                  make_uint4(w[4 * j], w[4 * j + 1], w[4 * j + 2], w[4 * j + 3]);
-            fence_proxy_async_smem();
-            __syncwarp();
-            if (lane == 0) {
-              tma_store_2d(&mapC, buf, col0, row0);
-              bulk_commit();
+            for (int k = 0; k < 32; k += 2) {
+              const float2 v = dense_grad2(make_float2(x[k], x[k + 1]), a.c, rc);
+              d[k] = v.x;
+              d[k + 1] = v.y;
             }
-            stores++;
+            if (col0 + 32 > a.N) {
+              // Zero up to the tile's end: dhidden's last block of K reads it.
+#pragma unroll
+              for (int k = 0; k < 32; k++)
+                if (col0 + k >= a.N) d[k] = 0.0f;
+            }
+            for (int part = 0; part <= a.split; part++) {
+              uint8_t *buf = smem + S::kExtraOff + (e * 2 + (stores & 1)) * 2048;
+              if (lane == 0) bulk_wait_read<1>();
+              __syncwarp();
+              uint32_t w[16];
+#pragma unroll
+              for (int k = 0; k < 16; k++) {
+                w[k] = pack16(d[2 * k], d[2 * k + 1], a.dtype);
+                if (a.split) {  // what this part leaves of d
+                  const float2 v = widen2(w[k], a.dtype);
+                  d[2 * k] -= v.x;
+                  d[2 * k + 1] -= v.y;
+                }
+              }
+#pragma unroll
+              for (int j = 0; j < 4; j++)
+                *reinterpret_cast<uint4 *>(buf + lane * 64 + ((j ^ ((lane >> 1) & 3)) << 4)) =
+                    make_uint4(w[4 * j], w[4 * j + 1], w[4 * j + 2], w[4 * j + 3]);
+              fence_proxy_async_smem();
+              __syncwarp();
+              if (lane == 0) {
+                tma_store_2d(&mapC, buf, part * a.shift + col0, row0);
+                bulk_commit();
+              }
+              stores++;
+            }
           } else {
             if (live && a.out16) {
 #pragma unroll
@@ -455,18 +484,16 @@ __global__ void __launch_bounds__(kVGemmThreads, 1)
             }
           }
         }
-      }
-      if constexpr (EPI == kVStats || EPI == kVStatsTop) {
-        if (ok && live) {
-          const int64_t at = (int64_t)(q.n * 2 + g) * a.M + row;
-          a.part[at] = make_float4(st.m, st.s, st.u, 0.0f);
-          if constexpr (EPI == kVStatsTop) {
-            for (int k = 0; k < a.top_k; k++) {
-              a.top_val[at * a.top_k + k] = lval[k * kLs];
-              a.top_col[at * a.top_k + k] = lcol[k * kLs];
-            }
+        if constexpr (EPI == kVStats) {
+          if (a.gmax && live) {
+            float4 *dst = reinterpret_cast<float4 *>(a.gmax + (int64_t)row * a.ldmax + n * (kVBN / kVGroup) + g * 8);
+            dst[0] = make_float4(gm[0], gm[1], gm[2], gm[3]);
+            dst[1] = make_float4(gm[4], gm[5], gm[6], gm[7]);
           }
         }
+      }
+      if constexpr (EPI == kVStats) {
+        if (ok && live) a.part[(int64_t)row * (2 * a.units_n) + q.n * 2 + g] = make_float4(st.m, st.s, st.u, 0.0f);
       }
     }
     if constexpr (EPI == kVDz) {
@@ -488,65 +515,84 @@ __global__ void __launch_bounds__(kVGemmThreads, 1)
   }
 }
 
-// ---- joining the partials, the given tokens' dot products ------------------------------
+// ---- joining the partials, the given tokens' and the alternatives' dot products ---------
 
 struct VJoinArgs {
   const uint16_t *h, *w;
   int64_t ldh, ldw;
-  int64_t rows;
   int V, H, T, K, parts, dtype;
   float c;
   const int32_t *ids;
   const float4 *part;
-  const float *top_val;
-  const int32_t *top_col;
+  const float *gmax;
+  int64_t ldmax;
+  int ngroups;
   float *logprobs, *lse, *entropy;
   int32_t *top_ids;
   float *top_logprobs;
 };
 
-constexpr int kJoinThreads = 128;
-
-__device__ __forceinline__ float2 widen2(uint32_t v, int dtype) {
-  if (dtype == IG_DT_BF16) return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xFFFF0000u));
-  return __half22float2(*reinterpret_cast<const __half2 *>(&v));
-}
-__device__ __forceinline__ float widen1(uint16_t v, int dtype) {
-  if (dtype == IG_DT_BF16) return __uint_as_float((uint32_t)v << 16);
-  return __half2float(*reinterpret_cast<const __half *>(&v));
-}
-
-// One CTA per row.
-__global__ void __launch_bounds__(kJoinThreads) vocab_join_kernel(const VJoinArgs a) {
-  __shared__ VStat s_warp[kJoinThreads / 32];
+// One CTA per row: the statistics of the row's parts, then the dot products of
+// the given tokens and of the best groups' columns, eight lanes each (128
+// bytes of either operand a step). A logit summed here is float32 in another
+// order than the tensor core's.
+template <bool TOP>
+__global__ void __launch_bounds__(kVocThreads) vocab_join_kernel(const VJoinArgs a) {
+  __shared__ VStat s_warp[kVocWarps];
+  __shared__ float s_dot[kTeacherMax];
+  __shared__ TopShared s_top[1];
+  __shared__ float s_oval[kTopMax];
+  __shared__ int s_ocol[kTopMax];
+  __shared__ int s_on;
   const int64_t row = blockIdx.x;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int tid = (int)threadIdx.x, warp = tid >> 5, lane = tid & 31, nthreads = (int)blockDim.x;
   const float c2 = a.c * kLog2e;
   dep_wait();
   VStat st{-IG_INF, 0.0f, 0.0f};
-  for (int p = threadIdx.x; p < a.parts; p += kJoinThreads) {
-    const float4 v = a.part[(int64_t)p * a.rows + row];
+  for (int p = tid; p < a.parts; p += nthreads) {
+    const float4 v = a.part[row * a.parts + p];
     vstat_merge<true>(st, VStat{v.x, v.y, v.z}, c2);
   }
   st = vstat_warp<true>(st, c2);
   if (lane == 0) s_warp[warp] = st;
+  if constexpr (TOP) {
+    // The best groups of columns.
+    const RowVecs<IG_DT_F32> rv(a.gmax + row * a.ldmax, a.ngroups);
+    const RowPart<IG_DT_F32> rp(rv, 0, 1);
+    uint32_t m = VElem<IG_DT_F32>::kNegInf;
+    for (int i = tid; i < rp.n; i += kVocThreads) {
+      const uint4 v = rp.base[i];
+      m = VElem<IG_DT_F32>::hmax(m, VElem<IG_DT_F32>::hmax(VElem<IG_DT_F32>::hmax(v.x, v.y), VElem<IG_DT_F32>::hmax(v.z, v.w)));
+    }
+    if (tid == kLastThread && rp.last)
+      for (int i = rv.col(rp.v1 - 1); i < a.ngroups; i++) m = VElem<IG_DT_F32>::hmax(m, __float_as_uint(rv.row[i]));
+    top_select<IG_DT_F32>(rv, rp, __uint_as_float(m), a.K, s_top[0], s_oval, s_ocol, &s_on);
+  } else {
+    if (tid == 0) s_on = 0;
+  }
   __syncthreads();
-  st = s_warp[0];
-  for (int w = 1; w < kJoinThreads / 32; w++) vstat_merge<true>(st, s_warp[w], c2);
+  st = vstat_join<true>(s_warp, nthreads / 32, c2);
   float log_s, lse, entropy;
   row_lse(st, a.c, log_s, lse, entropy);
-  if (threadIdx.x == 0) {
+  if (tid == 0) {
     if (a.lse) a.lse[row] = lse;
     if (a.entropy) a.entropy[row] = entropy;
   }
+  const int cand = s_on * kVGroup, total = a.T + cand;
   const uint16_t *h = a.h + row * a.ldh;
-  for (int t = warp; t < a.T; t += kJoinThreads / 32) {
-    const int id = a.ids[row * a.T + t];
-    float v = 0.0f;
+  const int sub = tid & 7;
+  for (int d0 = 0; d0 < total; d0 += nthreads / 8) {
+    const int d = d0 + (tid >> 3);
+    int id = -1;
+    if (d < a.T)
+      id = a.ids[row * a.T + d];
+    else if (d < total)
+      id = s_ocol[(d - a.T) / kVGroup] * kVGroup + (d - a.T) % kVGroup;
+    float s = 0.0f;
     if (id >= 0 && id < a.V) {
       const uint16_t *w = a.w + (int64_t)id * a.ldw;
-      float s = 0.0f;
-      for (int i = lane * 8; i + 8 <= a.H; i += 256) {
+#pragma unroll 4
+      for (int i = sub * 8; i + 8 <= a.H; i += 64) {
         const uint4 x = *reinterpret_cast<const uint4 *>(h + i), y = __ldg(reinterpret_cast<const uint4 *>(w + i));
         const uint32_t xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w};
 #pragma unroll
@@ -557,60 +603,49 @@ __global__ void __launch_bounds__(kJoinThreads) vocab_join_kernel(const VJoinArg
         }
       }
       const int tail = a.H & ~7;
-      if (tail + lane < a.H) s = fmaf(widen1(h[tail + lane], a.dtype), widen1(w[tail + lane], a.dtype), s);
-#pragma unroll
-      for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(~0u, s, o);
-      v = row_logprob(s, st, a.c, log_s);
-    } else if (id >= a.V) {
-      v = __int_as_float(0x7FC00000);
-      if (lane == 0) set_device_error(kDevBadId);
+      if (tail + sub < a.H) s = fmaf(widen1(h[tail + sub], a.dtype), widen1(w[tail + sub], a.dtype), s);
     }
-    if (lane == 0) a.logprobs[row * a.T + t] = v;
+    __syncwarp();
+#pragma unroll
+    for (int o = 4; o; o >>= 1) s += __shfl_xor_sync(~0u, s, o);
+    if (sub == 0) {
+      if (d < a.T) {
+        s_dot[d] = s;
+      } else if (TOP && d < total) {
+        s_top[0].val[d - a.T] = id < a.V ? s : -IG_INF;
+        s_top[0].col[d - a.T] = id < a.V ? id : 0x7FFFFFFF;
+      }
+    }
   }
-  if (a.K == 0 || warp != 0) return;
-  // The alternatives: every part's list is sorted; lane l walks the lists l,
-  // l + 32, ... (at most kHeads of them) and the best head wins.
-  constexpr int kHeads = 16;  // 2 * 256 parts
-  int head[kHeads];
-#pragma unroll
-  for (int i = 0; i < kHeads; i++) head[i] = 0;
-  const bool nan = st.s != st.s;
-  for (int k = 0; k < a.K; k++) {
-    float bv = -IG_INF;
-    int bc = 0x7FFFFFFF, bi = -1;
-#pragma unroll
-    for (int i = 0; i < kHeads; i++) {
-      const int p = lane + 32 * i;
-      if (p < a.parts && head[i] < a.K) {
-        const int64_t at = ((int64_t)p * a.rows + row) * a.K + head[i];
-        const float v = a.top_val[at];
-        const int c = a.top_col[at];
-        if (c >= 0 && top_before(v, c, bv, bc)) {
-          bv = v;
-          bc = c;
-          bi = i;
-        }
+  __syncthreads();
+  for (int t = tid; t < a.T; t += nthreads) {
+    const int id = a.ids[row * a.T + t];
+    float v = 0.0f;
+    if (id >= a.V) {
+      v = __int_as_float(0x7FC00000);
+      set_device_error(kDevBadId);
+    } else if (id >= 0) {
+      v = row_logprob(s_dot[t], st, a.c, log_s);
+    }
+    a.logprobs[row * a.T + t] = v;
+  }
+  if constexpr (TOP) {
+    const bool nan = st.s != st.s;
+    for (int i = tid; i < cand && !nan; i += nthreads) {
+      const float v = s_top[0].val[i];
+      const int c = s_top[0].col[i];
+      if (c == 0x7FFFFFFF) continue;
+      int r = 0;
+      for (int j = 0; j < cand; j++) r += top_before(s_top[0].val[j], s_top[0].col[j], v, c);
+      if (r < a.K) {
+        a.top_ids[row * a.K + r] = c;
+        a.top_logprobs[row * a.K + r] = row_logprob(v, st, a.c, log_s);
       }
     }
-    float wv = bv;
-    int wc = bc;
-#pragma unroll
-    for (int o = 16; o; o >>= 1) {
-      const float ov = __shfl_xor_sync(~0u, wv, o);
-      const int oc = __shfl_xor_sync(~0u, wc, o);
-      if (top_before(ov, oc, wv, wc)) {
-        wv = ov;
-        wc = oc;
-      }
-    }
-#pragma unroll
-    for (int i = 0; i < kHeads; i++)
-      if (bi == i && bc == wc && wc != 0x7FFFFFFF) head[i]++;
-    if (lane == 0) {
-      const bool have = wc != 0x7FFFFFFF && !nan;
-      a.top_ids[row * a.K + k] = have ? wc : -1;
-      a.top_logprobs[row * a.K + k] =
-          have ? row_logprob(wv, st, a.c, log_s) : (nan ? __int_as_float(0x7FC00000) : -IG_INF);
+    // Past the columns (all groups are in the list then), or in a row that is no distribution.
+    for (int k = (nan ? 0 : min(cand, a.V)) + tid; k < a.K; k += nthreads) {
+      a.top_ids[row * a.K + k] = -1;
+      a.top_logprobs[row * a.K + k] = nan ? __int_as_float(0x7FC00000) : -IG_INF;
     }
   }
 }
@@ -624,7 +659,7 @@ struct VCoefArgs {
   const int32_t *ids;
   const float *lse, *entropy, *dlogprobs, *dentropy;
   VRowCoef *coef;
-  int *bound;  // bits of the largest |dZ| bound of any row (float32 bits of a positive number order as integers)
+  int *bound;  // bits of the largest |dZ| bound of any row (positive floats order as their bits); NULL: not needed
 };
 
 // One warp per row.
@@ -648,22 +683,7 @@ __global__ void vocab_coef_kernel(const VCoefArgs a) {
   a.coef[row] = VRowCoef{k.A, k.B, k.lse, 0.0f};
   // |dZ| <= c (sum |g| (1 + p) + |gH| p (|log p| + H)) <= c (2 sum |g| + |gH| (1 + H))
   const float b = a.c * (2.0f * size + fabsf(gh) * (1.0f + H));
-  if (lse != -IG_INF && b > 0.0f && b < 3.0e38f) atomicMax(a.bound, __float_as_int(b));
-}
-
-// float16 has 5 exponent bits: dZ is scaled by a power of two that brings the
-// largest bound of the rows to 2^14..2^15, so that probabilities down to
-// 2^-28 of it keep all their bits; the products' float32 sums are scaled
-// back. bfloat16 has float32's range and needs none.
-__global__ void vocab_scale_kernel(const int *bound, float *scale, int dtype) {
-  float s = 1.0f;
-  const int b = *bound;
-  if (dtype == IG_DT_F16 && b > 0) {
-    int e = ((b >> 23) & 255) - 127;  // bound in [2^e, 2^(e+1))
-    e = min(max(14 - e, -100), 100);
-    s = __int_as_float((e + 127) << 23);
-  }
-  *scale = s;
+  if (a.bound && lse != -IG_INF && b > 0.0f && b < 3.0e38f) atomicMax(a.bound, __float_as_int(b));
 }
 
 struct VTokenArgs {
@@ -673,14 +693,16 @@ struct VTokenArgs {
   const int32_t *ids;
   const float *logprobs, *dlogprobs, *lse;
   const VRowCoef *coef;
-  const float *scale;
+  const int *bound;
   void *dz;
   int64_t ldz;
+  int shift;  // of dZ's second part (0: none)
 };
 
 // dZ at the given tokens of columns [v0, v1): the dense part from the saved
 // log probability plus the tokens' own gradients, rounded once.
 __global__ void vocab_token_kernel(const VTokenArgs a) {
+  dep_wait();
   const int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
   if (i >= a.n) return;
   const int64_t row = i / a.T;
@@ -688,20 +710,36 @@ __global__ void vocab_token_kernel(const VTokenArgs a) {
   if (id < a.v0 || id >= a.v1 || a.lse[row] == -IG_INF) return;
   const VRowCoef k = a.coef[row];
   const float t = max_nan(a.logprobs[i], kYMin);
-  const float d = ex2(t * kLog2e) * fmaf(k.B, t, k.A) + token_grad(a.ids + row * a.T, a.dlogprobs + row * a.T, a.T, id, a.c);
-  store16(a.dz, row * a.ldz + id - a.v0, d * __ldg(a.scale), a.dtype);
+  float d = ex2(t * kLog2e) * fmaf(k.B, t, k.A) + token_grad(a.ids + row * a.T, a.dlogprobs + row * a.T, a.T, id, a.c);
+  d *= vocab_scale(a.bound);
+  const int64_t at = row * a.ldz + id - a.v0;
+  const uint32_t w = pack16(d, 0.0f, a.dtype);
+  static_cast<uint16_t *>(a.dz)[at] = (uint16_t)w;
+  if (a.shift) store16(a.dz, at + a.shift, d - widen1((uint16_t)w, a.dtype), a.dtype);
 }
 
-// dhidden = sum over the K parts, in order, scaled back and rounded.
-__global__ void vocab_sum_kernel(const float *part, int parts, int64_t rows, int H, int64_t ldp, const float *scale,
-                                 void *out, int64_t ldo, int dtype) {
-  const int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
-  const int64_t row = i / H;
-  if (row >= rows) return;
-  const int col = (int)(i - row * H);
-  float s = 0.0f;
-  for (int p = 0; p < parts; p++) s += part[((int64_t)p * rows + row) * ldp + col];
-  store16(out, row * ldo + col, s * (1.0f / __ldg(scale)), dtype);
+// dhidden = sum over the K parts, in order, scaled back and rounded. One CTA
+// per row, four columns per thread.
+__global__ void __launch_bounds__(256) vocab_sum_kernel(const float *part, int parts, int64_t rows, int H, int64_t ldp,
+                                                        const int *bound, void *out, int64_t ldo, int dtype) {
+  dep_wait();
+  const int64_t row = blockIdx.x;
+  const float unscale = 1.0f / vocab_scale(bound);
+  for (int col = 4 * threadIdx.x; col < H; col += 4 * blockDim.x) {
+    float4 s = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 8
+    for (int p = 0; p < parts; p++) {
+      const float4 v = *reinterpret_cast<const float4 *>(part + ((int64_t)p * rows + row) * ldp + col);
+      s = make_float4(s.x + v.x, s.y + v.y, s.z + v.z, s.w + v.w);
+    }
+    const float v[4] = {s.x * unscale, s.y * unscale, s.z * unscale, s.w * unscale};
+    uint16_t *dst = static_cast<uint16_t *>(out) + row * ldo + col;
+    if (col + 4 <= H && (reinterpret_cast<uintptr_t>(dst) & 7) == 0) {
+      *reinterpret_cast<uint2 *>(dst) = make_uint2(pack16(v[0], v[1], dtype), pack16(v[2], v[3], dtype));
+    } else {
+      for (int k = 0; k < 4 && col + k < H; k++) store16(dst, k, v[k], dtype);
+    }
+  }
 }
 
 // ---- plans and launches ------------------------------------------------------------------
@@ -758,7 +796,7 @@ static cudaError_t launch_vgemm(const CUtensorMap &ma, const CUtensorMap &mb, co
   if (slots <= 0) return cudaErrorInvalidConfiguration;
   const int64_t units = (int64_t)a.units_m * a.units_n * a.units_s;
   cudaLaunchConfig_t cfg = {};
-  cudaLaunchAttribute at[1];
+  cudaLaunchAttribute at[2];
   cfg.gridDim = dim3((unsigned)(CG * (units < slots ? units : slots)));
   cfg.blockDim = dim3(kVGemmThreads);
   cfg.dynamicSmemBytes = VSmem<CG, EPI>::kTotal;
@@ -768,9 +806,10 @@ static cudaError_t launch_vgemm(const CUtensorMap &ma, const CUtensorMap &mb, co
     at[0].val.clusterDim.x = CG;
     at[0].val.clusterDim.y = 1;
     at[0].val.clusterDim.z = 1;
-    cfg.attrs = at;
     cfg.numAttrs = 1;
   }
+  cfg.attrs = at;
+  add_dep_attr(at, cfg.numAttrs);
   return cudaLaunchKernelEx(&cfg, vocab_gemm_kernel<CG, A_MN, B_MN, EPI>, ma, mb, mc, a);
 }
 
@@ -801,11 +840,13 @@ struct VPlan {
   int V, H;
   int cg;
   int units_m, units_n;  // statistics
-  size_t part_bytes, top_bytes, fwd_bytes;
+  int64_t ldmax;
+  size_t part_bytes, fwd_bytes;
   // backward
+  bool split;
   int64_t chunk, ldz, ldp;
   int ks;
-  size_t coef_bytes, dz_bytes, p32_bytes, bwd_bytes;
+  size_t coef_bytes, dz_bytes, bwd_bytes;
 };
 
 static VPlan vocab_plan(int64_t rows, int V, int H, int top_k) {
@@ -819,24 +860,24 @@ static VPlan vocab_plan(int64_t rows, int V, int H, int top_k) {
   const int64_t tiles = ((int64_t)V + kVBN - 1) / kVBN;
   p.units_n = best_parts(p.units_m, tiles, slots, kVMaxParts, 0.25);
   p.part_bytes = align_up((size_t)p.units_n * 2 * rows * sizeof(float4), 256);
-  p.top_bytes = align_up((size_t)p.units_n * 2 * rows * top_k * 4, 256);
-  p.fwd_bytes = p.part_bytes + 2 * p.top_bytes;
-  int64_t chunk = kVDzBytes / 2 / (rows > 0 ? rows : 1) / kVBN * kVBN;
+  p.ldmax = tiles * (kVBN / kVGroup);
+  p.fwd_bytes = p.part_bytes + (top_k > 0 ? (size_t)rows * p.ldmax * 4 : 0);
+  // With few rows, a given token's column or two carry most of the gradients,
+  // and nothing averages the rounding of dZ: it is kept in two 16-bit parts
+  // (16 or more bits), which doubles K where the weights' traffic bounds.
+  p.split = p.cg == 1;
+  int64_t chunk = kVDzBytes / (p.split ? 4 : 2) / (rows > 0 ? rows : 1) / kVBN * kVBN;
   if (chunk < kVBN) chunk = kVBN;
-  const int64_t vpad = tiles * kVBN;
-  if (chunk > vpad) chunk = vpad;
-  // Chunks of equal size.
-  const int64_t nch = (vpad + chunk - 1) / chunk;
-  chunk = ((tiles + nch - 1) / nch) * kVBN;
-  p.chunk = chunk;
-  p.ldz = chunk;
+  if (chunk > tiles * kVBN) chunk = tiles * kVBN;
+  const int64_t nch = (tiles * kVBN + chunk - 1) / chunk;  // chunks of about equal size
+  p.chunk = (tiles + nch - 1) / nch * kVBN;
+  p.ldz = p.chunk * (p.split ? 2 : 1);
   p.ldp = (H + 3) / 4 * 4;
   const int64_t out_tiles = p.units_m * (((int64_t)H + kVBN - 1) / kVBN);
-  p.ks = best_parts(out_tiles, chunk / kVBK, slots, 64, 8.0);
+  p.ks = best_parts(out_tiles, p.ldz / kVBK, slots, 64, 8.0);
   p.coef_bytes = align_up((size_t)rows * sizeof(VRowCoef), 256) + 256;
   p.dz_bytes = align_up((size_t)rows * p.ldz * 2, 256);
-  p.p32_bytes = align_up((size_t)p.ks * rows * p.ldp * 4, 256);
-  p.bwd_bytes = p.coef_bytes + p.dz_bytes + p.p32_bytes;
+  p.bwd_bytes = p.coef_bytes + p.dz_bytes + align_up((size_t)p.ks * rows * p.ldp * 4, 256);
   return p;
 }
 
@@ -858,29 +899,22 @@ static int run_vocab_logprobs(const VMatrices &x, const VPlan &p, const LogprobA
   VGemmArgs a{};
   a.M = (int)p.rows;
   a.N = p.V;
-  a.K = p.H;
+  a.kblocks = a.kwrap = (p.H + kVBK - 1) / kVBK;
   a.idesc = idesc_f16(128 * p.cg, kVBN, x.dtype, false, false);
   a.units_m = p.units_m;
   a.units_n = p.units_n;
   a.units_s = 1;
   a.c2 = o.c * kLog2e;
   a.part = reinterpret_cast<float4 *>(ws);
-  a.top_k = o.K;
-  a.top_val = reinterpret_cast<float *>(ws + p.part_bytes);
-  a.top_col = reinterpret_cast<int32_t *>(ws + p.part_bytes + p.top_bytes);
-  if (p.cg == 1) {
-    IG_CU(o.K > 0 ? (launch_vgemm<1, false, false, kVStatsTop>(ma, mb, mb, a, st))
-                  : (launch_vgemm<1, false, false, kVStats>(ma, mb, mb, a, st)));
-  } else {
-    IG_CU(o.K > 0 ? (launch_vgemm<2, false, false, kVStatsTop>(ma, mb, mb, a, st))
+  a.gmax = o.K > 0 ? reinterpret_cast<float *>(ws + p.part_bytes) : nullptr;
+  a.ldmax = p.ldmax;
+  IG_CU(p.cg == 1 ? (launch_vgemm<1, false, false, kVStats>(ma, mb, mb, a, st))
                   : (launch_vgemm<2, false, false, kVStats>(ma, mb, mb, a, st)));
-  }
   VJoinArgs j{};
   j.h = static_cast<const uint16_t *>(x.h);
   j.w = static_cast<const uint16_t *>(x.w);
   j.ldh = x.ldh;
   j.ldw = x.ldw;
-  j.rows = p.rows;
   j.V = p.V;
   j.H = p.H;
   j.T = o.T;
@@ -890,14 +924,16 @@ static int run_vocab_logprobs(const VMatrices &x, const VPlan &p, const LogprobA
   j.c = o.c;
   j.ids = o.ids;
   j.part = a.part;
-  j.top_val = a.top_val;
-  j.top_col = a.top_col;
+  j.gmax = a.gmax;
+  j.ldmax = p.ldmax;
+  j.ngroups = (p.V + kVGroup - 1) / kVGroup;
   j.logprobs = o.logprobs;
   j.lse = o.lse;
   j.entropy = o.entropy;
   j.top_ids = o.top_ids;
   j.top_logprobs = o.top_logprobs;
-  IG_CU(launch_dep(vocab_join_kernel, dim3((unsigned)p.rows), dim3(kJoinThreads), 0, st, j));
+  IG_CU(o.K > 0 ? launch_dep(vocab_join_kernel<true>, dim3((unsigned)p.rows), dim3(kVocThreads), 0, st, j)
+                : launch_dep(vocab_join_kernel<false>, dim3((unsigned)p.rows), dim3(64), 0, st, j));
   return 0;
 }
 
@@ -910,93 +946,93 @@ struct VocabGradOut {
 static int run_vocab_grad(const VMatrices &x, const VPlan &p, const LogprobGradArgs &g, const VocabGradOut &o, uint8_t *ws,
                           cudaStream_t st) {
   VRowCoef *coef = reinterpret_cast<VRowCoef *>(ws);
-  int *bound = reinterpret_cast<int *>(ws + p.coef_bytes - 256);
-  float *scale = reinterpret_cast<float *>(bound + 1);
+  int *bound = x.dtype == IG_DT_F16 ? reinterpret_cast<int *>(ws + p.coef_bytes - 256) : nullptr;
   uint8_t *dz = ws + p.coef_bytes;
   float *p32 = reinterpret_cast<float *>(dz + p.dz_bytes);
-  IG_CU(cudaMemsetAsync(bound, 0, 4, st));
-  VCoefArgs ca{p.rows, p.V, g.T, x.dtype, g.c, g.ids, g.lse, g.entropy, g.dlogprobs, g.dentropy, coef, bound};
+  if (bound) IG_CU(cudaMemsetAsync(bound, 0, 4, st));
+  const VCoefArgs ca{p.rows, p.V, g.T, x.dtype, g.c, g.ids, g.lse, g.entropy, g.dlogprobs, g.dentropy, coef, bound};
   vocab_coef_kernel<<<(unsigned)((p.rows + 7) / 8), 256, 0, st>>>(ca);
-  vocab_scale_kernel<<<1, 1, 0, st>>>(bound, scale, x.dtype);
   IG_CU(cudaGetLastError());
-  const int tm = 128 * p.cg;
+  const int tm = 128 * p.cg, shift = p.split ? (int)p.chunk : 0;
   CUtensorMap mh, mw, mz, mzs;
-  int chunks = 0;
-  for (int64_t v0 = 0; v0 < p.V; v0 += p.chunk) chunks++;
   int done = 0, parts = 1;
   for (int64_t v0 = 0; v0 < p.V; v0 += p.chunk, done++) {
     const int64_t vc = p.V - v0 < p.chunk ? p.V - v0 : p.chunk;
+    const bool last = v0 + vc == p.V;
     const uint8_t *wc = static_cast<const uint8_t *>(x.w) + v0 * x.ldw * 2;
     // dZ of the chunk.
     IG_VMAP(&mh, x.h, p.H, p.rows, x.ldh, kVBK, 128, x.dtype, false);
     IG_VMAP(&mw, wc, p.H, vc, x.ldw, kVBK, kVBN / p.cg, x.dtype, false);
-    IG_VMAP(&mzs, dz, vc, p.rows, p.ldz, 32, 32, x.dtype, true);
+    IG_VMAP(&mzs, dz, p.ldz, p.rows, p.ldz, 32, 32, x.dtype, true);
     VGemmArgs a{};
     a.M = (int)p.rows;
     a.N = (int)vc;
-    a.K = p.H;
+    a.kblocks = a.kwrap = (p.H + kVBK - 1) / kVBK;
     a.idesc = idesc_f16(tm, kVBN, x.dtype, false, false);
     a.units_m = p.units_m;
     a.units_n = (int)((vc + kVBN - 1) / kVBN);
     a.units_s = 1;
     a.c = g.c;
     a.coef = coef;
-    a.scale = scale;
+    a.split = p.split;
+    a.shift = shift;
+    a.bound = bound;
     a.dtype = x.dtype;
     IG_CU(p.cg == 1 ? (launch_vgemm<1, false, false, kVDz>(mh, mw, mzs, a, st))
                     : (launch_vgemm<2, false, false, kVDz>(mh, mw, mzs, a, st)));
     if (g.dlogprobs && g.T > 0) {
       VTokenArgs t{p.rows, p.rows * g.T, g.T, p.V, (int)v0, (int)(v0 + vc), x.dtype, g.c, g.ids, o.logprobs, g.dlogprobs,
-                   g.lse, coef, scale, dz, p.ldz};
-      vocab_token_kernel<<<(unsigned)((t.n + 255) / 256), 256, 0, st>>>(t);
-      IG_CU(cudaGetLastError());
+                   g.lse, coef, bound, dz, p.ldz, shift};
+      IG_CU(launch_dep(vocab_token_kernel, dim3((unsigned)((t.n + 255) / 256)), dim3(256), 0, st, t));
     }
+    IG_VMAP(&mz, dz, p.ldz, p.rows, p.ldz, kVBK, 128, x.dtype, false);
     if (o.dh) {
-      IG_VMAP(&mz, dz, vc, p.rows, p.ldz, kVBK, 128, x.dtype, false);
       IG_VMAP(&mw, wc, p.H, vc, x.ldw, 64, kVBK, x.dtype, false);
       VGemmArgs b{};
       b.M = (int)p.rows;
       b.N = p.H;
-      b.K = (int)vc;
+      b.kwrap = (int)((vc + kVBK - 1) / kVBK);
+      b.kblocks = b.kwrap * (p.split ? 2 : 1);
+      b.shift = shift;
       b.idesc = idesc_f16(tm, kVBN, x.dtype, false, true);
       b.units_m = p.units_m;
       b.units_n = (p.H + kVBN - 1) / kVBN;
-      const int64_t kb = (vc + kVBK - 1) / kVBK;
-      b.units_s = (int)(kb < p.ks ? kb : p.ks);
+      b.units_s = b.kblocks < p.ks ? b.kblocks : p.ks;
       b.n_fastest = 1;
       b.dtype = x.dtype;
-      b.scale = scale;
+      b.bound = bound;
       b.part32 = p32;
       b.ldo = p.ldp;
       b.accumulate = done > 0;
-      if (chunks == 1 && b.units_s == 1) {
+      if (done == 0) parts = b.units_s;  // a later, smaller chunk adds into the first of them
+      if (done == 0 && last && parts == 1) {
         b.out16 = o.dh;
         b.ldo = o.lddh;
       }
       IG_CU(p.cg == 1 ? (launch_vgemm<1, false, true, kVOut>(mz, mw, mw, b, st))
                       : (launch_vgemm<2, false, true, kVOut>(mz, mw, mw, b, st)));
-      if (done == 0) parts = b.units_s;  // a later, smaller chunk adds into the first of them
-      if (!b.out16 && done == chunks - 1) {
-        const int64_t n = p.rows * p.H;
-        vocab_sum_kernel<<<(unsigned)((n + 255) / 256), 256, 0, st>>>(p32, parts, p.rows, p.H, p.ldp, scale, o.dh, o.lddh,
-                                                                    x.dtype);
-        IG_CU(cudaGetLastError());
+      if (!b.out16 && last) {
+        const int threads = p.H >= 1024 ? 256 : (p.H + 127) / 128 * 32;
+        IG_CU(launch_dep(vocab_sum_kernel, dim3((unsigned)p.rows), dim3(threads), 0, st, (const float *)p32, parts, p.rows,
+                         p.H, p.ldp, (const int *)bound, o.dh, o.lddh, x.dtype));
       }
     }
     if (o.dw) {
-      IG_VMAP(&mz, dz, vc, p.rows, p.ldz, 64, kVBK, x.dtype, false);
+      IG_VMAP(&mz, dz, p.ldz, p.rows, p.ldz, 64, kVBK, x.dtype, false);
       IG_VMAP(&mh, x.h, p.H, p.rows, x.ldh, 64, kVBK, x.dtype, false);
       VGemmArgs b{};
       b.M = (int)vc;
       b.N = p.H;
-      b.K = (int)p.rows;
+      b.kwrap = (int)((p.rows + kVBK - 1) / kVBK);
+      b.kblocks = b.kwrap * (p.split ? 2 : 1);
+      b.shift = shift;
       b.idesc = idesc_f16(256, kVBN, x.dtype, true, true);
       b.units_m = (int)((vc + 255) / 256);
       b.units_n = (p.H + kVBN - 1) / kVBN;
       b.units_s = 1;
       b.n_fastest = 1;
       b.dtype = x.dtype;
-      b.scale = scale;
+      b.bound = bound;
       b.out16 = static_cast<uint8_t *>(o.dw) + v0 * o.lddw * 2;
       b.ldo = o.lddw;
       IG_CU((launch_vgemm<2, true, true, kVOut>(mz, mh, mh, b, st)));

@@ -164,6 +164,25 @@ def test_backward(voc, dtype, rows, V, H):
     assert ops.device_error() == 0
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,V,H", [(1, 5000, 256), (7, 33001, 72), (128, 1000, 136)])
+def test_few_rows_keep_more_bits(voc, dtype, rows, V, H):
+    """At most 128 rows: dZ in two 16-bit parts, so the gradients are off by their own rounding and little else (the
+    second part's rounding is 2^-8 of the first's: u (1 + 2^-6) bounds both, in the norm over a gradient)."""
+    h, w = make(rows, V, H, dtype, 19)
+    gen = torch.Generator(device="cuda").manual_seed(8)
+    ids = torch.randint(0, V, (rows, 1), generator=gen, device="cuda", dtype=torch.int32)
+    g = torch.rand((rows, 1), generator=gen, device="cuda") + 0.5
+    r = voc.vocab_logprobs(h, w, ids)
+    dh, dw = voc.vocab_logprobs_backward(h, w, ids, r.logprobs, r.lse, r.entropy, g)
+    G = -g.double() * torch.softmax(h.double() @ w.double().T, 1)
+    G.scatter_add_(1, ids.long(), g.double())
+    u = torch.finfo(dtype).eps / 2
+    for got, want in ((dh, G @ w.double()), (dw, G.T @ h.double())):
+        rounded = (want.to(dtype).double() - want).norm()
+        assert (got.double() - want).norm() <= 1.1 * rounded + u * 2**-6 * want.norm()
+
+
 def test_backward_column_chunks(voc):
     """A logits' gradient of more than its workspace's chunk: two chunks of columns."""
     rows, V, H = 8192, 70001, 64
