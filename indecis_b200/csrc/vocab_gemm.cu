@@ -55,6 +55,7 @@ struct VGemmArgs {
   int shift;
   uint32_t idesc;
   int units_m, units_n, units_s;  // units: M tiles x N parts x K parts
+  int a_rows;  // rows of A's box (one CTA per tile: the rows there are, rounded up to 8; else 128)
   int n_fastest;                  // unit order: N parts innermost, else M tiles
   // kVStats: [M][units_n * 2] partials; group maxima [M][ldmax] or NULL
   float c2;
@@ -253,7 +254,7 @@ __global__ void __launch_bounds__(kVGemmThreads, 1)
               break;
             }
             uint8_t *sa = smem + s * S::kStageBytes, *sb = sa + S::kABytes;
-            if (rank == 0) mbar_arrive_expect_tx(&full[s], CG * S::kStageBytes);
+            if (rank == 0) mbar_arrive_expect_tx(&full[s], CG * (S::kBBytes + a.a_rows * kVBK * 2));
             auto load = [&](const CUtensorMap *map, uint8_t *dst, int c0, int c1) {
               if constexpr (CG == 2)
                 tma_load_2d_pair(map, dst, cluster_addr(&full[s], 0), c0, c1);
@@ -560,9 +561,16 @@ __global__ void __launch_bounds__(kVocThreads) vocab_join_kernel(const VJoinArgs
     const RowVecs<IG_DT_F32> rv(a.gmax + row * a.ldmax, a.ngroups);
     const RowPart<IG_DT_F32> rp(rv, 0, 1);
     uint32_t m = VElem<IG_DT_F32>::kNegInf;
-    for (int i = tid; i < rp.n; i += kVocThreads) {
-      const uint4 v = rp.base[i];
-      m = VElem<IG_DT_F32>::hmax(m, VElem<IG_DT_F32>::hmax(VElem<IG_DT_F32>::hmax(v.x, v.y), VElem<IG_DT_F32>::hmax(v.z, v.w)));
+    constexpr int kAhead = 8;
+    for (int i = tid; i < rp.n; i += kAhead * kVocThreads) {
+      uint4 v[kAhead];
+#pragma unroll
+      for (int j = 0; j < kAhead; j++)
+        v[j] = rp.base[min(i + j * kVocThreads, i + (rp.n - 1 - i) / kVocThreads * kVocThreads)];  // the last again past the end
+#pragma unroll
+      for (int j = 0; j < kAhead; j++)
+        m = VElem<IG_DT_F32>::hmax(m, VElem<IG_DT_F32>::hmax(VElem<IG_DT_F32>::hmax(v[j].x, v[j].y),
+                                                             VElem<IG_DT_F32>::hmax(v[j].z, v[j].w)));
     }
     if (tid == kLastThread && rp.last)
       for (int i = rv.col(rp.v1 - 1); i < a.ngroups; i++) m = VElem<IG_DT_F32>::hmax(m, __float_as_uint(rv.row[i]));
@@ -591,15 +599,28 @@ __global__ void __launch_bounds__(kVocThreads) vocab_join_kernel(const VJoinArgs
     float s = 0.0f;
     if (id >= 0 && id < a.V) {
       const uint16_t *w = a.w + (int64_t)id * a.ldw;
-#pragma unroll 4
-      for (int i = sub * 8; i + 8 <= a.H; i += 64) {
-        const uint4 x = *reinterpret_cast<const uint4 *>(h + i), y = __ldg(reinterpret_cast<const uint4 *>(w + i));
-        const uint32_t xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w};
+      constexpr int kAhead = 6;  // loads in flight of either operand
+      const int h8 = a.H & ~7;
+      for (int i0 = sub * 8; i0 < h8; i0 += 64 * kAhead) {
+        uint4 x[kAhead], y[kAhead];
 #pragma unroll
-        for (int k = 0; k < 4; k++) {
-          const float2 p = widen2(xs[k], a.dtype), q = widen2(ys[k], a.dtype);
-          s = fmaf(p.x, q.x, s);
-          s = fmaf(p.y, q.y, s);
+        for (int j = 0; j < kAhead; j++) {
+          const int i = i0 + 64 * j;
+          x[j] = y[j] = make_uint4(0, 0, 0, 0);
+          if (i < h8) {
+            x[j] = *reinterpret_cast<const uint4 *>(h + i);
+            y[j] = __ldg(reinterpret_cast<const uint4 *>(w + i));
+          }
+        }
+#pragma unroll
+        for (int j = 0; j < kAhead; j++) {
+          const uint32_t xs[4] = {x[j].x, x[j].y, x[j].z, x[j].w}, ys[4] = {y[j].x, y[j].y, y[j].z, y[j].w};
+#pragma unroll
+          for (int k = 0; k < 4; k++) {
+            const float2 p = widen2(xs[k], a.dtype), q = widen2(ys[k], a.dtype);
+            s = fmaf(p.x, q.x, s);
+            s = fmaf(p.y, q.y, s);
+          }
         }
       }
       const int tail = a.H & ~7;
@@ -813,22 +834,26 @@ static cudaError_t launch_vgemm(const CUtensorMap &ma, const CUtensorMap &mb, co
   return cudaLaunchKernelEx(&cfg, vocab_gemm_kernel<CG, A_MN, B_MN, EPI>, ma, mb, mc, a);
 }
 
-// Parts (of column tiles, or of K blocks) per M tile: the fewest that keep the
-// rounds of units close to the work's share per slot. With `tiles` pieces to
+// Parts (of column tiles, or of K blocks) per M tile. With `tiles` pieces to
 // cut and `outer` M tiles, a cut in p parts runs ceil(outer p / slots) rounds
-// of ceil(tiles / p) pieces.
-static int best_parts(int64_t outer, int64_t tiles, int64_t slots, int most, double overhead) {
-  int best = 1;
-  double cost = 1e300;
-  for (int p = 1; p <= most && p <= tiles; p++) {
-    const double rounds = (double)((outer * p + slots - 1) / slots);
-    const double c = rounds * ((double)((tiles + p - 1) / p) + overhead);
+// of ceil(tiles / p) pieces plus a fixed overhead (in pieces); the best cuts
+// fill whole rounds, so only those are tried.
+static int best_parts(int64_t outer, int64_t tiles, int64_t slots, int64_t most, double overhead) {
+  if (most > tiles) most = tiles;
+  int64_t best = 1;
+  double cost = (double)((outer + slots - 1) / slots) * ((double)tiles + overhead);
+  for (int64_t rounds = (outer + slots - 1) / slots; rounds <= 64; rounds++) {
+    int64_t p = rounds * slots / outer;
+    if (p > most) p = most;
+    if (p < 1) continue;
+    const double c = (double)((outer * p + slots - 1) / slots) * ((double)((tiles + p - 1) / p) + overhead);
     if (c < cost * 0.995) {
       cost = c;
       best = p;
     }
+    if (p == most) break;
   }
-  return best;
+  return (int)best;
 }
 
 constexpr int kVMaxParts = 256;        // column parts per M tile (two partials each)
@@ -838,7 +863,7 @@ constexpr int64_t kVDzBytes = 1ll << 30;  // dZ is formed in column chunks of at
 struct VPlan {
   int64_t rows;
   int V, H;
-  int cg;
+  int cg, a_rows;
   int units_m, units_n;  // statistics
   int64_t ldmax;
   size_t part_bytes, fwd_bytes;
@@ -855,6 +880,7 @@ static VPlan vocab_plan(int64_t rows, int V, int H, int top_k) {
   p.V = V;
   p.H = H;
   p.cg = rows <= kVOneCtaRows ? 1 : 2;
+  p.a_rows = p.cg == 1 ? (int)((rows + 7) / 8 * 8) : 128;
   const int64_t tm = 128 * p.cg, slots = num_sms() / p.cg;
   p.units_m = (int)((rows + tm - 1) / tm);
   const int64_t tiles = ((int64_t)V + kVBN - 1) / kVBN;
@@ -894,11 +920,12 @@ struct VMatrices {
 
 static int run_vocab_logprobs(const VMatrices &x, const VPlan &p, const LogprobArgs &o, uint8_t *ws, cudaStream_t st) {
   CUtensorMap ma, mb;
-  IG_VMAP(&ma, x.h, p.H, p.rows, x.ldh, kVBK, 128, x.dtype, false);
+  IG_VMAP(&ma, x.h, p.H, p.rows, x.ldh, kVBK, p.a_rows, x.dtype, false);
   IG_VMAP(&mb, x.w, p.H, p.V, x.ldw, kVBK, kVBN / p.cg, x.dtype, false);
   VGemmArgs a{};
   a.M = (int)p.rows;
   a.N = p.V;
+  a.a_rows = p.a_rows;
   a.kblocks = a.kwrap = (p.H + kVBK - 1) / kVBK;
   a.idesc = idesc_f16(128 * p.cg, kVBN, x.dtype, false, false);
   a.units_m = p.units_m;
@@ -961,12 +988,13 @@ static int run_vocab_grad(const VMatrices &x, const VPlan &p, const LogprobGradA
     const bool last = v0 + vc == p.V;
     const uint8_t *wc = static_cast<const uint8_t *>(x.w) + v0 * x.ldw * 2;
     // dZ of the chunk.
-    IG_VMAP(&mh, x.h, p.H, p.rows, x.ldh, kVBK, 128, x.dtype, false);
+    IG_VMAP(&mh, x.h, p.H, p.rows, x.ldh, kVBK, p.a_rows, x.dtype, false);
     IG_VMAP(&mw, wc, p.H, vc, x.ldw, kVBK, kVBN / p.cg, x.dtype, false);
     IG_VMAP(&mzs, dz, p.ldz, p.rows, p.ldz, 32, 32, x.dtype, true);
     VGemmArgs a{};
     a.M = (int)p.rows;
     a.N = (int)vc;
+    a.a_rows = p.a_rows;
     a.kblocks = a.kwrap = (p.H + kVBK - 1) / kVBK;
     a.idesc = idesc_f16(tm, kVBN, x.dtype, false, false);
     a.units_m = p.units_m;
@@ -985,12 +1013,13 @@ static int run_vocab_grad(const VMatrices &x, const VPlan &p, const LogprobGradA
                    g.lse, coef, bound, dz, p.ldz, shift};
       IG_CU(launch_dep(vocab_token_kernel, dim3((unsigned)((t.n + 255) / 256)), dim3(256), 0, st, t));
     }
-    IG_VMAP(&mz, dz, p.ldz, p.rows, p.ldz, kVBK, 128, x.dtype, false);
+    IG_VMAP(&mz, dz, p.ldz, p.rows, p.ldz, kVBK, p.a_rows, x.dtype, false);
     if (o.dh) {
       IG_VMAP(&mw, wc, p.H, vc, x.ldw, 64, kVBK, x.dtype, false);
       VGemmArgs b{};
       b.M = (int)p.rows;
       b.N = p.H;
+      b.a_rows = p.a_rows;
       b.kwrap = (int)((vc + kVBK - 1) / kVBK);
       b.kblocks = b.kwrap * (p.split ? 2 : 1);
       b.shift = shift;
@@ -1023,6 +1052,7 @@ static int run_vocab_grad(const VMatrices &x, const VPlan &p, const LogprobGradA
       VGemmArgs b{};
       b.M = (int)vc;
       b.N = p.H;
+      b.a_rows = 128;  // of M: two boxes of 64
       b.kwrap = (int)((p.rows + kVBK - 1) / kVBK);
       b.kblocks = b.kwrap * (p.split ? 2 : 1);
       b.shift = shift;
