@@ -188,9 +188,10 @@ struct RowPart {
   const uint4 *base;
   int v0, v1, w0, n;
   bool first, last;
-  __device__ __forceinline__ RowPart(const RowVecs<DT> &rv, int part, int parts) {
-    v0 = (int)((int64_t)rv.nv * part / parts);
-    v1 = (int)((int64_t)rv.nv * (part + 1) / parts);
+  __device__ __forceinline__ RowPart(const RowVecs<DT> &rv, uint32_t part, uint32_t parts) {
+    const uint32_t per = ((uint32_t)rv.nv + parts - 1) / parts;
+    v0 = min(part * per, (uint32_t)rv.nv);
+    v1 = min(v0 + per, (uint32_t)rv.nv);
     first = v0 < v1 && !rv.whole(v0);
     last = v1 - v0 > (first ? 1 : 0) && !rv.whole(v1 - 1);
     w0 = v0 + (first ? 1 : 0);
@@ -835,36 +836,14 @@ struct DistillArgs {
   int parts;  // CTAs per row (a cluster)
 };
 
-__device__ __forceinline__ float block_sum(float v, float *s8) {
-  v = warp_sum(v);
-  __syncthreads();
-  if ((threadIdx.x & 31) == 0) s8[threadIdx.x >> 5] = v;
-  __syncthreads();
-  float t = 0.0f;
-#pragma unroll
-  for (int w = 0; w < kVocWarps; w++) t += s8[w];
-  return t;
-}
-__device__ __forceinline__ float block_max(float v, float *s8) {
-#pragma unroll
-  for (int o = 16; o; o >>= 1) v = max_nan(v, __shfl_xor_sync(~0u, v, o));
-  __syncthreads();
-  if ((threadIdx.x & 31) == 0) s8[threadIdx.x >> 5] = v;
-  __syncthreads();
-  float t = s8[0];
-#pragma unroll
-  for (int w = 1; w < kVocWarps; w++) t = max_nan(t, s8[w]);
-  return t;
-}
-
 // One cluster per row. The row's part is copied to shared memory in four bulk
 // copies (STAGED), so the statistics' pass starts on the first quarter and the
 // gradient's pass reads no global memory; rows too long for that (over 8 x
-// kStageMax bytes) are read twice, the second time from L2. With TAIL the mass
-// outside the list is summed on its own (1 - the list's mass would lose it to
-// cancellation): a bit per vector in shared memory says whether the vector
-// holds listed columns, and those vectors (at most K) compare their columns
-// with the list.
+// kStageMax bytes) are read twice, the second time from L2. The teacher's list
+// is worked on by one warp while the others start on the row. With TAIL the
+// mass outside the list is summed on its own (1 - the list's mass would lose
+// it to cancellation): a byte per vector in shared memory marks its listed
+// columns.
 constexpr int kStageParts = 4;
 constexpr int kStageMax = 160 * 1024;
 
@@ -880,14 +859,14 @@ __global__ void __launch_bounds__(kVocThreads, 4) distill_topk_kernel(const Dist
   using E = VElem<DT>;
   using T = typename E::T;
   constexpr int kN = E::kN;
-  constexpr int kR = 2;  // vectors per thread and step
+  constexpr int kR = 4;  // vectors per thread and step
   extern __shared__ uint4 s_dyn[];
   __shared__ VStat s_warp[kVocWarps];
   __shared__ VStat s_part[8];  // every CTA's statistics
-  __shared__ float s8[kVocWarps];
-  __shared__ int s_ids[kTeacherMax];
-  __shared__ float s_q[kTeacherMax];
-  __shared__ float s_xk[kTeacherMax];
+  __shared__ VStat s_list;     // with TAIL: the listed columns'
+  __shared__ float s_mass[2];  // the sum of q, what is left of 1
+  __shared__ int s_ids[kTeacherMax], s_once[kTeacherMax];
+  __shared__ float s_q[kTeacherMax], s_xk[kTeacherMax];
   __shared__ __align__(8) uint64_t s_bar[kStageParts + 1];
   const int cs = a.parts, rank = cs > 1 ? (int)cluster_ctarank() : 0;
   const int64_t row = blockIdx.x / cs;
@@ -895,7 +874,7 @@ __global__ void __launch_bounds__(kVocThreads, 4) distill_topk_kernel(const Dist
   const RowPart<DT> rp(rv, rank, cs);
   const int tid = (int)threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const float c2 = a.c * kLog2e;
-  uint32_t *s_bits = reinterpret_cast<uint32_t *>(s_dyn + (STAGED ? rp.n : 0));  // one per vector v0 + i
+  uint8_t *s_mask = reinterpret_cast<uint8_t *>(s_dyn + (STAGED ? rp.n : 0));  // of vector v0 + i
   // Quarters of whole steps.
   constexpr int kStep = kR * kVocThreads;
   const int quarter = ((rp.n + kStageParts - 1) / kStageParts + kStep - 1) / kStep * kStep;
@@ -925,10 +904,8 @@ __global__ void __launch_bounds__(kVocThreads, 4) distill_topk_kernel(const Dist
   T *drow = a.dx ? static_cast<T *>(a.dx) + row * a.ldd : nullptr;
   const bool same = (reinterpret_cast<uintptr_t>(drow) & 15) == (reinterpret_cast<uintptr_t>(rv.row) & 15);
 
-  // The teacher's list: thread k holds entry k.
+  // The teacher's list: thread k brings entry k.
   int id = -1;
-  float q = 0.0f, xk = -IG_INF;
-  bool once = false;  // the first entry with its id
   if (tid < a.K) {
     id = a.tids[row * a.K + tid];
     if (id >= a.V) {
@@ -937,52 +914,79 @@ __global__ void __launch_bounds__(kVocThreads, 4) distill_topk_kernel(const Dist
     }
     if (id < 0) id = -1;
     s_ids[tid] = id;
-    if (id >= 0) xk = E::get(rv.row[id]);
-    s_xk[tid] = xk;
+    s_q[tid] = id >= 0 ? a.tlogits[row * a.K + tid] : -IG_INF;
+    s_xk[tid] = id >= 0 ? E::get(rv.row[id]) : -IG_INF;
+  }
+  if constexpr (TAIL) {
+    const int nw = (rp.v1 - rp.v0 + 3) / 4;
+    for (int i = tid; i < nw; i += kVocThreads) reinterpret_cast<uint32_t *>(s_mask)[i] = 0;
   }
   const int any = __syncthreads_or(id >= 0);
   const bool skip = !any || w == 0.0f;  // uniform over the cluster
   const int cfirst = max(rv.col(rp.v0), 0), clast = min(rv.col(rp.v1), a.V);
   VStat st{-IG_INF, 0.0f, 0.0f};
-  float q_rest = 0.0f;
   if (!skip) {
-    if (id >= 0) {
-      once = true;
-      for (int k = 0; k < tid; k++)
-        if (s_ids[k] == id) once = false;
-    }
-    const float t = id >= 0 ? a.tlogits[row * a.K + tid] : -IG_INF;
     if constexpr (TAIL) {
-      q = id >= 0 ? expf(t) : 0.0f;
-      const float q_list = block_sum(q, s8);
-      q_rest = q_list == q_list ? fmaxf(1.0f - q_list, 0.0f) : q_list;
-      const int nw = (rp.v1 - rp.v0 + 31) / 32;
-      for (int i = tid; i < nw; i += kVocThreads) s_bits[i] = 0;
-      __syncthreads();
-      if (id >= cfirst && id < clast) {
-        const int v = (id + rv.mis) / kN - rp.v0;
-        atomicOr(&s_bits[v >> 5], 1u << (v & 31));
+      if (tid < a.K) {
+        int once = id >= 0;  // the first entry with its id
+        for (int k = 0; k < tid; k++)
+          if (s_ids[k] == id) once = 0;
+        s_once[tid] = once;
+        if (id >= cfirst && id < clast) {
+          const int at = id + rv.mis - rp.v0 * kN, i = at / kN;
+          atomicOr(reinterpret_cast<uint32_t *>(s_mask) + (i >> 2), 1u << ((i & 3) * 8 + at % kN));
+        }
       }
       __syncthreads();
-    } else {
-      const float top = block_max(t, s8);
-      q = id >= 0 && top != -IG_INF ? expf((t - top) * a.c) : 0.0f;
-      const float sum = block_sum(q, s8);
-      if (sum > 0.0f || sum != sum) q /= sum;
+    }
+    if (warp == 0) {
+      // q over the list, in place of the teacher's values.
+      float q_sum = 0.0f, q_rest = 0.0f;
+      if constexpr (TAIL) {
+        VStat l{-IG_INF, 0.0f, 0.0f};
+        for (int k = lane; k < a.K; k += 32) {
+          const float q = expf(s_q[k]);  // 0 for a missing entry
+          s_q[k] = q;
+          q_sum += q;
+          const float x = s_xk[k];
+          // A listed +inf or NaN: no distribution, s is NaN from here on.
+          const float one = x == -IG_INF ? 0.0f : (x < IG_INF ? 1.0f : __int_as_float(0x7FC00000));
+          if (s_once[k]) vstat_merge<false>(l, VStat{fmaxf(x, -IG_INF), one, 0.0f}, c2);
+        }
+        q_sum = warp_sum(q_sum);
+        q_rest = q_sum == q_sum ? fmaxf(1.0f - q_sum, 0.0f) : q_sum;
+        l = vstat_warp<false>(l, c2);
+        if (lane == 0) s_list = l;
+      } else {
+        float top = -IG_INF;
+        for (int k = lane; k < a.K; k += 32) top = max_nan(top, s_q[k]);
+        float nan = top != top ? top : 0.0f;
+        top = warp_max(top);
+        for (int k = lane; k < a.K; k += 32) {
+          const float e = top == -IG_INF ? 0.0f : expf((s_q[k] - top) * a.c);
+          s_q[k] = e;
+          q_sum += e;
+        }
+        q_sum = warp_sum(q_sum + nan);
+        const float inv = q_sum > 0.0f || q_sum != q_sum ? 1.0f / q_sum : 0.0f;
+        for (int k = lane; k < a.K; k += 32) s_q[k] *= inv;
+        q_sum = q_sum > 0.0f ? 1.0f : q_sum;
+      }
+      if (lane == 0) {
+        s_mass[0] = q_sum;
+        s_mass[1] = q_rest;
+      }
     }
     // A vector as the statistics see it: the listed columns are left out of the tail's.
     auto unlisted = [&](uint4 raw, int v) {
       if constexpr (TAIL) {
-        const int i = v - rp.v0;
-        if (s_bits[i >> 5] >> (i & 31) & 1u) {
+        const uint32_t m = s_mask[v - rp.v0];
+        if (m) {
           float x[kN];
           E::unpack(raw, x);
-          for (int k = 0; k < a.K; k++) {
-            const int at = s_ids[k] - rv.col(v);
 #pragma unroll
-            for (int e = 0; e < kN; e++)
-              if (at == e) x[e] = -IG_INF;
-          }
+          for (int e = 0; e < kN; e++)
+            if (m >> e & 1u) x[e] = -IG_INF;
           raw = E::pack(x);
         }
       }
@@ -1032,29 +1036,24 @@ __global__ void __launch_bounds__(kVocThreads, 4) distill_topk_kernel(const Dist
     st = vstat_join<false>(s_part, cs, c2);
   }
   // Dense gradient: coef 2^((x - mb) c2 - l2); a listed column: listed p - w c q.
-  float coef = 0.0f, listed = 0.0f, pk = 0.0f;
+  float coef = 0.0f, listed = 0.0f;
   float mb = 0.0f, l2 = 0.0f;
+  float row_m = 0.0f, row_l2 = 0.0f;  // p = 2^((x - row_m) c2 - row_l2)
+  bool zero = true;
   if (!skip) {
     VStat all = st;
-    if constexpr (TAIL) {
-      const float mk = block_max(once ? fmaxf(xk, -IG_INF) : -IG_INF, s8);
-      const float mb = mk == -IG_INF ? 0.0f : mk;
-      const float sk = block_sum(once ? ex2((xk - mb) * c2) : 0.0f, s8);
-      vstat_merge<false>(all, VStat{mk, sk, 0.0f}, c2);
-    }
+    const float q_sum = s_mass[0], q_rest = s_mass[1];
+    if constexpr (TAIL) vstat_merge<false>(all, s_list, c2);
     const float log_s = logf(all.s);
-    const float logp = all.s == 0.0f ? -IG_INF : (xk - all.m) * a.c - log_s;
-    const float q_list = block_sum(q, s8);
-    float loss = block_sum(q > 0.0f || q != q ? q * (logf(q) - logp) : 0.0f, s8);
-    float mass = q_list + q_rest, rest = 0.0f;
+    float mass = q_sum + q_rest, rest = 0.0f, tail_loss = 0.0f;
     bool far = false;
     if constexpr (TAIL) {
       if (st.s == 0.0f) {
         // Nothing outside the list: what is left of 1 is rounding.
-        mass = q_list;
+        mass = q_sum;
       } else if (q_rest > 0.0f || q_rest != q_rest) {
         const float logr = (st.m - all.m) * a.c + logf(st.s) - log_s;
-        loss += q_rest * (logf(q_rest) - logr);
+        tail_loss = q_rest * (logf(q_rest) - logr);
         // A tail of less than e^-60: p and q_rest / p_rest would leave the
         // float range. Its columns then take q_rest times their share of the
         // tail alone (p itself adds less than e^-60 / q_rest of that).
@@ -1062,19 +1061,27 @@ __global__ void __launch_bounds__(kVocThreads, 4) distill_topk_kernel(const Dist
         rest = q_rest * ex2(-logr * kLog2e);
       }
     }
-    if (all.s != all.s) loss = all.s;
-    if (rank == 0 && tid == 0) a.loss[row] = loss * w;
+    if (rank == 0 && warp == 0) {
+      float loss = 0.0f;
+      for (int k = lane; k < a.K; k += 32) {
+        const float q = s_q[k];
+        if (q > 0.0f || q != q) loss += q * (logf(q) - (all.s == 0.0f ? -IG_INF : (s_xk[k] - all.m) * a.c - log_s));
+      }
+      loss = warp_sum(loss) + tail_loss;
+      if (all.s != all.s) loss = all.s;
+      if (lane == 0) a.loss[row] = loss * w;
+    }
+    zero = all.s == 0.0f;
     listed = w * a.c * mass;
-    pk = ex2((xk - (all.s == 0.0f ? 0.0f : all.m)) * c2 - log_s * kLog2e);
+    row_m = zero ? 0.0f : all.m;
+    row_l2 = log_s * kLog2e;
     coef = far ? -w * a.c * q_rest : w * a.c * (mass - rest);
     mb = far ? st.m : all.m;
-    l2 = (far ? logf(st.s) : log_s) * kLog2e;
-    st = all;
+    l2 = far ? logf(st.s) * kLog2e : row_l2;
   } else if (rank == 0 && tid == 0) {
     a.loss[row] = 0.0f;
   }
   if (!drow) return;
-  const bool zero = skip || st.s == 0.0f;
   if (cs == 1) __syncthreads();  // the list's logits are read before any store: dx may be x
   const float2 nm = make_float2(-mb, -mb), cc = make_float2(c2, c2), nl = make_float2(-l2, -l2);
   auto grad = [&](const uint4 &v, float *d) {
@@ -1118,14 +1125,14 @@ __global__ void __launch_bounds__(kVocThreads, 4) distill_topk_kernel(const Dist
     }
   }
   if (zero) return;
-  if (tid < a.K) s_q[tid] = q;
   __syncthreads();
-  // The listed columns of this CTA's part; q of equal ids adds up.
-  if (once && id >= cfirst && id < clast) {
-    float sq = 0.0f;
-    for (int k = tid; k < a.K; k++)
-      if (s_ids[k] == id) sq += s_q[k];
-    drow[id] = E::put(listed * pk - w * a.c * sq);
+  // The listed columns of this CTA's part; q of equal ids adds up (each of
+  // their threads stores the same value).
+  if (id >= cfirst && id < clast) {
+    float q = 0.0f;
+    for (int k = 0; k < a.K; k++)
+      if (s_ids[k] == id) q += s_q[k];
+    drow[id] = E::put(listed * ex2((s_xk[tid] - row_m) * c2 - row_l2) - w * a.c * q);
   }
 }
 
@@ -1191,7 +1198,7 @@ static cudaError_t run_distill(DistillArgs a, bool tail, cudaStream_t st) {
   a.parts = cs;
   const int64_t part = nv / cs + 1;
   const bool staged = part * 16 <= kStageMax;
-  const size_t bits = tail ? ((part + 31) / 32 + 1) * 4 : 0;
+  const size_t bits = tail ? (part / 4 + 1) * 4 : 0;
   const size_t smem = bits + (staged ? part * 16 : 0);
   if (staged)
     return tail ? launch_distill<DT, true, true>(a, cs, smem, st) : launch_distill<DT, false, true>(a, cs, smem, st);

@@ -30,18 +30,23 @@ class TokenLogProbs(NamedTuple):
 
 
 def _matrix(t, name):
-    if t.dim() != 2 or t.dtype not in _DT or not t.is_cuda or (t.shape[1] > 1 and t.stride(1) != 1):
-        raise ValueError(f"{name}: expected a CUDA float32, bfloat16 or float16 matrix with a unit column stride")
-    ld = t.stride(0) if t.shape[0] > 1 else t.shape[1]
-    if ld < t.shape[1]:
-        raise ValueError(f"{name}: row stride shorter than the row")
-    return ld
+    """Row stride of a CUDA matrix with a unit column stride."""
+    shape = t.shape
+    if len(shape) == 2 and t.is_cuda and t.dtype in _DT:
+        ld, unit = t.stride()
+        n = shape[1]
+        if shape[0] <= 1:
+            ld = n
+        if (unit == 1 or n <= 1) and ld >= n:
+            return ld
+    raise ValueError(f"{name}: expected a CUDA float32, bfloat16 or float16 matrix with a unit column stride, rows apart "
+                     "by at least their length")
 
 
 def _dense(t, dtype, shape, like, name):
     if t is None:
         return None
-    if t.dtype != dtype or t.shape != shape or t.device != like.device or not t.is_contiguous():
+    if t.dtype is not dtype or t.shape != shape or t.device != like.device or not t.is_contiguous():
         raise ValueError(f"{name}: expected a contiguous {dtype} tensor of shape {tuple(shape)} on {like.device}")
     return t.data_ptr()
 
@@ -65,18 +70,18 @@ def _call(like, fn, *args):
 
 
 def _outputs(like, N, T, K):
-    """The forward's outputs as pieces of one float32 allocation (top_ids of its own), and the addresses of logprobs,
+    """The forward's outputs as pieces of one allocation of 32-bit words, and the addresses of logprobs,
     lse, entropy, top_ids and top_logprobs. (Taken from the allocation: the data_ptr of an empty piece is 0.)"""
     K = max(K, 0)  # a negative top_k is refused by the call
-    buf = torch.empty(N * (T + 2 + K), dtype=torch.float32, device=like.device)
+    buf = torch.empty(N * (T + 2 + 2 * K), dtype=torch.float32, device=like.device)
     base, n = buf.data_ptr(), N * T
     tl = ti = None
     if K > 0:
         tl = buf.as_strided((N, K), (K, 1), n + 2 * N)
-        ti = torch.empty((N, K), dtype=torch.int32, device=like.device)
+        ti = buf.view(torch.int32).as_strided((N, K), (K, 1), n + 2 * N + N * K)
     r = TokenLogProbs(buf.as_strided((N, T), (T, 1)), buf.as_strided((N,), (1,), n), buf.as_strided((N,), (1,), n + N), ti,
                       tl)
-    ptrs = (base, base + 4 * n, base + 4 * (n + N), ti.data_ptr() if K > 0 else None,
+    ptrs = (base, base + 4 * n, base + 4 * (n + N), base + 4 * (n + 2 * N + N * K) if K > 0 else None,
             base + 4 * (n + 2 * N) if K > 0 else None)
     return r, ptrs
 
@@ -160,16 +165,18 @@ def aligned(t):
 
 
 def _operands(hidden, weight):
-    for t, name in ((hidden, "hidden"), (weight, "weight")):
-        _matrix(t, name)
-        if t.dtype == torch.float32:
-            raise ValueError(f"{name}: expected bfloat16 or float16")
-    if hidden.dtype != weight.dtype or hidden.device != weight.device or hidden.shape[1] != weight.shape[1]:
-        raise ValueError("hidden and weight: expected one type, device and row length")
-    hidden, weight = aligned(hidden), aligned(weight)
-    h8 = (hidden.shape[1] + 7) // 8 * 8
-    return (hidden, hidden.stride(0) if hidden.shape[0] > 1 else h8, weight,
-            weight.stride(0) if weight.shape[0] > 1 else h8)
+    ldh, ldw = _matrix(hidden, "hidden"), _matrix(weight, "weight")
+    dtype = hidden.dtype
+    if dtype is torch.float32 or weight.dtype is not dtype:
+        raise ValueError("hidden and weight: expected both bfloat16 or both float16")
+    H = hidden.shape[1]
+    if weight.shape[1] != H or hidden.device != weight.device:
+        raise ValueError("hidden and weight: expected one device and row length")
+    if ldh % 8 or hidden.data_ptr() % 16:
+        hidden, ldh = aligned(hidden), (H + 7) // 8 * 8
+    if ldw % 8 or weight.data_ptr() % 16:
+        weight, ldw = aligned(weight), (H + 7) // 8 * 8
+    return hidden, ldh, weight, ldw
 
 
 def _workspace(like, *sizes):

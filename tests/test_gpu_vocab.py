@@ -321,6 +321,52 @@ def test_distill_edges(voc, dtype, tail):
     assert loss[7] == 0 and (d[7] == 0).all()
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("tail", [False, True])
+@pytest.mark.parametrize("V", [50, 20000])
+def test_distill_special(voc, dtype, tail, V):
+    """NaN and +inf, in a listed column and outside; a teacher of -inf only; entries at and past the row's ends."""
+    x = make(7, V, dtype, 63)
+    ids = torch.tensor([[0, 3, V - 1, V - 2]] * 7, dtype=torch.int32, device="cuda")
+    t = torch.tensor([[-1.0, -2.0, -3.0, -4.0]] * 7, device="cuda")
+    x[1, 3] = INF
+    x[2, 7] = INF
+    x[3, 0] = float("nan")
+    t[4] = -INF
+    t[5, 2] = -INF
+    ids[6] = -1
+    loss, d = voc.distill_topk(x, ids, t, tail=tail)
+    for n in (1, 2, 3):
+        assert loss[n].isnan() and d[n].isnan().all()
+    ok = torch.tensor([0, 5, 6], device="cuda")
+    wl, wd, p, q = ref_distill(x[ok], ids[ok], t[ok], 1.0, tail, None)
+    close(loss[ok], wl, 4 * STAT_TOL)
+    tol = 4 * P_TOL * (wd.abs() + p) + EPS[dtype] / 2 * wd.abs() * 1.01 + TINY[dtype]
+    assert ((d[ok].double() - wd).abs() <= tol).all()
+    # No mass in the list: nothing without the tail, all of it outside with it.
+    p4 = torch.softmax(x[4].double(), 0)
+    inside = torch.zeros(V, dtype=torch.bool, device="cuda")
+    inside[ids[4].long()] = True
+    if tail:
+        out = p4[~inside].sum()
+        close(loss[4], -out.log(), 4 * STAT_TOL)
+        want = p4 - torch.where(inside, torch.zeros_like(p4), p4 / out)
+        assert ((d[4].double() - want).abs() <= 1e-4 * p4 + EPS[dtype] * want.abs() + TINY[dtype]).all()
+    else:
+        assert loss[4] == 0 and (d[4] == 0).all()
+
+
+@pytest.mark.parametrize("tail", [False, True])
+def test_distill_long_rows(voc, tail):
+    """Float32 rows of 2^20 columns: more than a cluster's shared memory holds, so the row is read twice."""
+    x = make(2, 1 << 20, torch.float32, 65, pad=3, shift=1)
+    ids, t = teacher(x, 40, tail, 7)
+    loss, d = voc.distill_topk(x, ids, t, tail=tail)
+    wl, wd, p, q = ref_distill(x, ids, t, 1.0, tail, None)
+    close(loss, wl, 4 * 7e-5)
+    assert ((d.double() - wd).abs() <= 1e-4 * (wd.abs() + p) + 1e-6 * p + 1e-9).all()
+
+
 @pytest.mark.parametrize("tail", [False, True])
 def test_distill_differences(voc, tail):
     x = make(2, 40, torch.float32, 71, scale=1.0)
