@@ -43,7 +43,7 @@ constexpr int kVGemmThreads = 64 + 32 * kVEpiWarps;
 
 // Row coefficients of dZ (RowCoef with the output scale applied by the reader).
 struct VRowCoef {
-  float A, B, lse, pad;
+  float A, B, lse2, pad;
 };
 
 constexpr int kVGroup = 16;  // columns per stored maximum
@@ -57,13 +57,12 @@ struct VGemmArgs {
   int units_m, units_n, units_s;  // units: M tiles x N parts x K parts
   int a_rows;  // rows of A's box (one CTA per tile: the rows there are, rounded up to 8; else 128)
   int n_fastest;                  // unit order: N parts innermost, else M tiles
+  float c2;  // log2(e) / temperature
   // kVStats: [M][units_n * 2] partials; group maxima [M][ldmax] or NULL
-  float c2;
   float4 *part;
   float *gmax;
   int64_t ldmax;
   // kVDz
-  float c;
   const VRowCoef *coef;
   int split;  // dZ as two 16-bit parts, the second `shift` elements on
   // kVDz, kVOut: dtype of the 16-bit output; bits of dZ's bound (vocab_scale), NULL: unscaled
@@ -344,7 +343,7 @@ __global__ void __launch_bounds__(kVGemmThreads, 1)
         if (live) {
           const VRowCoef v = a.coef[row];
           const float sc = vocab_scale(a.bound);
-          rc = RowCoef{v.A * sc, v.B * sc, v.lse};
+          rc = RowCoef{v.A * sc, v.B * sc, v.lse2};
         }
       }
       [[maybe_unused]] float unscale = 1.0f;
@@ -416,7 +415,7 @@ __global__ void __launch_bounds__(kVGemmThreads, 1)
             float d[32];
 #pragma unroll
             for (int k = 0; k < 32; k += 2) {
-              const float2 v = dense_grad2(make_float2(x[k], x[k + 1]), a.c, rc);
+              const float2 v = dense_grad2(make_float2(x[k], x[k + 1]), a.c2, rc);
               d[k] = v.x;
               d[k + 1] = v.y;
             }
@@ -540,8 +539,8 @@ struct VJoinArgs {
 template <bool TOP>
 __global__ void __launch_bounds__(kVocThreads) vocab_join_kernel(const VJoinArgs a) {
   __shared__ VStat s_warp[kVocWarps];
-  __shared__ float s_dot[kTeacherMax];
-  __shared__ TopShared s_top[1];
+  __shared__ float s_dot[kIdsMax];
+  __shared__ TopShared<kVocThreads> s_top[1];
   __shared__ float s_oval[kTopMax];
   __shared__ int s_ocol[kTopMax];
   __shared__ int s_on;
@@ -572,9 +571,9 @@ __global__ void __launch_bounds__(kVocThreads) vocab_join_kernel(const VJoinArgs
         m = VElem<IG_DT_F32>::hmax(m, VElem<IG_DT_F32>::hmax(VElem<IG_DT_F32>::hmax(v[j].x, v[j].y),
                                                              VElem<IG_DT_F32>::hmax(v[j].z, v[j].w)));
     }
-    if (tid == kLastThread && rp.last)
+    if (tid == last_thread(kVocThreads) && rp.last)
       for (int i = rv.col(rp.v1 - 1); i < a.ngroups; i++) m = VElem<IG_DT_F32>::hmax(m, __float_as_uint(rv.row[i]));
-    top_select<IG_DT_F32>(rv, rp, __uint_as_float(m), a.K, s_top[0], s_oval, s_ocol, &s_on);
+    top_select<IG_DT_F32, kVocThreads>(rv, rp, __uint_as_float(m), a.K, s_top[0], s_oval, s_ocol, &s_on);
   } else {
     if (tid == 0) s_on = 0;
   }
@@ -701,10 +700,10 @@ __global__ void vocab_coef_kernel(const VCoefArgs a) {
   const float gh = a.dentropy ? a.dentropy[row] : 0.0f, H = a.dentropy ? a.entropy[row] : 0.0f;
   const float lse = a.lse[row];
   const RowCoef k = row_coef(lse, H, G, gh, a.c);
-  a.coef[row] = VRowCoef{k.A, k.B, k.lse, 0.0f};
+  a.coef[row] = VRowCoef{k.A, k.B, k.lse2, 0.0f};
   // |dZ| <= c (sum |g| (1 + p) + |gH| p (|log p| + H)) <= c (2 sum |g| + |gH| (1 + H))
   const float b = a.c * (2.0f * size + fabsf(gh) * (1.0f + H));
-  if (a.bound && lse != -IG_INF && b > 0.0f && b < 3.0e38f) atomicMax(a.bound, __float_as_int(b));
+  if (a.bound && k.lse2 != IG_INF && b > 0.0f && b < 3.0e38f) atomicMax(a.bound, __float_as_int(b));
 }
 
 struct VTokenArgs {
@@ -712,7 +711,7 @@ struct VTokenArgs {
   int T, V, v0, v1, dtype;
   float c;
   const int32_t *ids;
-  const float *logprobs, *dlogprobs, *lse;
+  const float *logprobs, *dlogprobs;
   const VRowCoef *coef;
   const int *bound;
   void *dz;
@@ -728,10 +727,11 @@ __global__ void vocab_token_kernel(const VTokenArgs a) {
   if (i >= a.n) return;
   const int64_t row = i / a.T;
   const int id = a.ids[i];
-  if (id < a.v0 || id >= a.v1 || a.lse[row] == -IG_INF) return;
+  if (id < a.v0 || id >= a.v1) return;
   const VRowCoef k = a.coef[row];
-  const float t = max_nan(a.logprobs[i], kYMin);
-  float d = ex2(t * kLog2e) * fmaf(k.B, t, k.A) + token_grad(a.ids + row * a.T, a.dlogprobs + row * a.T, a.T, id, a.c);
+  if (k.lse2 == IG_INF) return;  // no distribution
+  const float y = max_nan(a.logprobs[i] * kLog2e, kYMin);
+  float d = ex2(y) * fmaf(k.B, y, k.A) + token_grad(a.ids + row * a.T, a.dlogprobs + row * a.T, a.T, id, a.c);
   d *= vocab_scale(a.bound);
   const int64_t at = row * a.ldz + id - a.v0;
   const uint32_t w = pack16(d, 0.0f, a.dtype);
@@ -1000,7 +1000,7 @@ static int run_vocab_grad(const VMatrices &x, const VPlan &p, const LogprobGradA
     a.units_m = p.units_m;
     a.units_n = (int)((vc + kVBN - 1) / kVBN);
     a.units_s = 1;
-    a.c = g.c;
+    a.c2 = g.c * kLog2e;
     a.coef = coef;
     a.split = p.split;
     a.shift = shift;
@@ -1010,7 +1010,7 @@ static int run_vocab_grad(const VMatrices &x, const VPlan &p, const LogprobGradA
                     : (launch_vgemm<2, false, false, kVDz>(mh, mw, mzs, a, st)));
     if (g.dlogprobs && g.T > 0) {
       VTokenArgs t{p.rows, p.rows * g.T, g.T, p.V, (int)v0, (int)(v0 + vc), x.dtype, g.c, g.ids, o.logprobs, g.dlogprobs,
-                   g.lse, coef, bound, dz, p.ldz, shift};
+                   coef, bound, dz, p.ldz, shift};
       IG_CU(launch_dep(vocab_token_kernel, dim3((unsigned)((t.n + 255) / 256)), dim3(256), 0, st, t));
     }
     IG_VMAP(&mz, dz, p.ldz, p.rows, p.ldz, kVBK, p.a_rows, x.dtype, false);

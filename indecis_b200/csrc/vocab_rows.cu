@@ -19,12 +19,11 @@
 
 namespace ig {
 
-constexpr int kVocThreads = 256;
+constexpr int kVocThreads = 256;  // most threads per CTA (NT below: 32 to 256)
 constexpr int kVocWarps = kVocThreads / 32;
 constexpr int kVocUnroll = 4;     // 16-byte vectors in flight per thread
 constexpr int kTopMax = 32;       // alternatives per row
-constexpr int kTopCap = 512;      // candidates a CTA collects
-constexpr int kTeacherMax = kVocThreads;  // teacher entries per row: one thread each
+constexpr int kIdsMax = 256;      // given tokens or teacher entries per row
 constexpr float kLog2e = 1.44269504088896340736f;
 constexpr float kLn2 = 0.69314718055994530942f;
 constexpr float kYMin = -1.0e4f;  // 2^kYMin = 0
@@ -199,7 +198,9 @@ struct RowPart {
     base = reinterpret_cast<const uint4 *>(rv.row + rv.col(w0));
   }
 };
-constexpr int kFirstThread = 0, kLastThread = 32;  // the threads that take the partial vectors
+// The threads of NT that take the partial vectors.
+constexpr int kFirstThread = 0;
+constexpr int last_thread(int NT) { return NT > 32 ? 32 : 16; }
 
 // ---- running statistics -----------------------------------------------------------
 
@@ -328,26 +329,29 @@ __device__ __forceinline__ bool top_before(float va, int ca, float vb, int cb) {
   return va > vb || (va == vb && ca < cb);
 }
 // The K first (value, column) of a CTA's part of a row, after the statistics'
-// pass has left each thread its own maximum. 64 bins of four neighbouring
-// threads: the K-th largest of the bins' maxima is a lower bound of the K-th
+// pass has left each thread its own maximum. Up to 64 bins of one to four
+// neighbouring threads: the K-th largest of the bins' maxima is a lower bound of the K-th
 // largest value (K bins hold a value at least as large), and only bins that
 // reach it (K, or a few more with ties) are read again, from L2. What reaches
 // the bound is collected and ranked. With too many equal values for the
 // buffer (a row of few distinct values) the K are found one by one instead.
-constexpr int kTopBins = 64;
+template <int NT>
 struct TopShared {
-  float bin[kTopBins];
-  int kept[kTopBins];
-  float val[kTopCap];
-  int col[kTopCap];
+  static constexpr int kBins = NT < 64 ? NT : 64;
+  static constexpr int kPer = NT / kBins;  // threads per bin
+  static constexpr int kCap = 2 * NT;      // candidates a CTA collects
+  float bin[kBins];
+  int kept[kBins];
+  float val[kCap];
+  int col[kCap];
   float tau;
   int nkept, n;
-  float wv[kVocWarps];
-  int wc[kVocWarps];
+  float wv[NT / 32];
+  int wc[NT / 32];
 };
 
-template <int DT>
-__device__ __noinline__ void top_one_by_one(const RowVecs<DT> rv, int v0, int v1, int K, TopShared &t, float *out_val,
+template <int DT, int NT>
+__device__ __noinline__ void top_one_by_one(const RowVecs<DT> rv, int v0, int v1, int K, TopShared<NT> &t, float *out_val,
                                             int *out_col, int *out_n) {
   using E = VElem<DT>;
   float lv = IG_INF;
@@ -355,7 +359,7 @@ __device__ __noinline__ void top_one_by_one(const RowVecs<DT> rv, int v0, int v1
   for (; n < K; n++) {
     float bv = -IG_INF;
     int bc = 0x7FFFFFFF;
-    for (int v = v0 + (int)threadIdx.x; v < v1; v += kVocThreads) {
+    for (int v = v0 + (int)threadIdx.x; v < v1; v += NT) {
       float x[E::kN];
       E::unpack(rv.load(v), x);
 #pragma unroll
@@ -382,7 +386,7 @@ __device__ __noinline__ void top_one_by_one(const RowVecs<DT> rv, int v0, int v1
       t.wc[threadIdx.x >> 5] = bc;
     }
     __syncthreads();
-    for (int w = 0; w < kVocWarps; w++)
+    for (int w = 0; w < NT / 32; w++)
       if (top_before(t.wv[w], t.wc[w], bv, bc)) {
         bv = t.wv[w];
         bc = t.wc[w];
@@ -398,8 +402,8 @@ __device__ __noinline__ void top_one_by_one(const RowVecs<DT> rv, int v0, int v1
   if (threadIdx.x == 0) *out_n = n;
 }
 
-template <int DT>
-__device__ __forceinline__ void top_scan(const uint4 &raw, int col, float tau, TopShared &t) {
+template <int DT, int NT>
+__device__ __forceinline__ void top_scan(const uint4 &raw, int col, float tau, TopShared<NT> &t) {
   using E = VElem<DT>;
   if (E::top(E::hmax(E::hmax(raw.x, raw.y), E::hmax(raw.z, raw.w))) < tau) return;
   float x[E::kN];
@@ -408,7 +412,7 @@ __device__ __forceinline__ void top_scan(const uint4 &raw, int col, float tau, T
   for (int i = 0; i < E::kN; i++)
     if (x[i] >= tau && x[i] > -IG_INF) {
       const int at = atomicAdd(&t.n, 1);
-      if (at < kTopCap) {
+      if (at < TopShared<NT>::kCap) {
         t.val[at] = x[i];
         t.col[at] = col + i;
       }
@@ -416,53 +420,55 @@ __device__ __forceinline__ void top_scan(const uint4 &raw, int col, float tau, T
 }
 
 // tmax: the thread's maximum over the part's whole vectors threadIdx.x + i
-// kVocThreads (and a partial one, which is read again in any case).
-template <int DT>
-__device__ __forceinline__ void top_select(const RowVecs<DT> &rv, const RowPart<DT> &rp, float tmax, int K, TopShared &t,
+// NT (and a partial one, which is read again in any case).
+template <int DT, int NT>
+__device__ __forceinline__ void top_select(const RowVecs<DT> &rv, const RowPart<DT> &rp, float tmax, int K, TopShared<NT> &t,
                                            float *out_val, int *out_col, int *out_n) {
   const int tid = (int)threadIdx.x;
-  float bm = fmaxf(tmax, __shfl_xor_sync(~0u, tmax, 1));
-  bm = fmaxf(bm, __shfl_xor_sync(~0u, bm, 2));
-  if ((tid & 3) == 0) t.bin[tid >> 2] = bm;
+  constexpr int kBins = TopShared<NT>::kBins, kPer = TopShared<NT>::kPer;
+  float bm = tmax;
+#pragma unroll
+  for (int o = 1; o < kPer; o *= 2) bm = fmaxf(bm, __shfl_xor_sync(~0u, bm, o));
+  if (tid % kPer == 0) t.bin[tid / kPer] = bm;
   if (tid == 0) t.nkept = t.n = 0;
   __syncthreads();
-  if (tid < kTopBins) {
+  if (tid < kBins) {
     const float b = t.bin[tid];
     int r = 0;
 #pragma unroll 8
-    for (int j = 0; j < kTopBins; j++) r += top_before(t.bin[j], j, b, tid);
+    for (int j = 0; j < kBins; j++) r += top_before(t.bin[j], j, b, tid);
     if (r == K - 1) t.tau = b;
   }
   __syncthreads();
   const float tau = t.tau;
-  if (tid < kTopBins && t.bin[tid] >= tau && t.bin[tid] > -IG_INF) t.kept[atomicAdd(&t.nkept, 1)] = tid;
+  if (tid < kBins && t.bin[tid] >= tau && t.bin[tid] > -IG_INF) t.kept[atomicAdd(&t.nkept, 1)] = tid;
   __syncthreads();
-  const int rounds = (rp.n + kVocThreads - 1) / kVocThreads;
-  const int items = t.nkept * rounds * 4;
+  const int rounds = (rp.n + NT - 1) / NT;
+  const int items = t.nkept * rounds * kPer;
   constexpr int kAhead = 4;  // loads in flight per thread
-  for (int it = tid; it < items; it += kAhead * kVocThreads) {
+  for (int it = tid; it < items; it += kAhead * NT) {
     uint4 raw[kAhead];
     int at[kAhead];
 #pragma unroll
     for (int j = 0; j < kAhead; j++) {
-      const int k = it + j * kVocThreads, r = k >> 2, b = r / rounds;
-      at[j] = k < items ? (r - b * rounds) * kVocThreads + t.kept[b] * 4 + (k & 3) : rp.n;
+      const int k = it + j * NT, r = k / kPer, b = r / rounds;
+      at[j] = k < items ? (r - b * rounds) * NT + t.kept[b] * kPer + k % kPer : rp.n;
       if (at[j] < rp.n) raw[j] = rp.base[at[j]];
     }
 #pragma unroll
     for (int j = 0; j < kAhead; j++)
-      if (at[j] < rp.n) top_scan<DT>(raw[j], rv.col(rp.w0 + at[j]), tau, t);
+      if (at[j] < rp.n) top_scan<DT, NT>(raw[j], rv.col(rp.w0 + at[j]), tau, t);
   }
-  if (tid == kFirstThread && rp.first) top_scan<DT>(rv.edge(rp.v0), rv.col(rp.v0), tau, t);
-  if (tid == kLastThread && rp.last) top_scan<DT>(rv.edge(rp.v1 - 1), rv.col(rp.v1 - 1), tau, t);
+  if (tid == kFirstThread && rp.first) top_scan<DT, NT>(rv.edge(rp.v0), rv.col(rp.v0), tau, t);
+  if (tid == last_thread(NT) && rp.last) top_scan<DT, NT>(rv.edge(rp.v1 - 1), rv.col(rp.v1 - 1), tau, t);
   __syncthreads();
   const int n = t.n;
-  if (n > kTopCap) {
-    top_one_by_one<DT>(rv, rp.v0, rp.v1, K, t, out_val, out_col, out_n);
+  if (n > TopShared<NT>::kCap) {
+    top_one_by_one<DT, NT>(rv, rp.v0, rp.v1, K, t, out_val, out_col, out_n);
     return;
   }
   // The order of arrival varies, the ranks do not.
-  for (int i = tid; i < n; i += kVocThreads) {
+  for (int i = tid; i < n; i += NT) {
     const float v = t.val[i];
     const int c = t.col[i];
     int r = 0;
@@ -506,11 +512,12 @@ __device__ __forceinline__ float row_logprob(float x, const VStat &a, float c, f
 
 // Merges `lists` sorted lists (list l: cnt[l] entries at val/col + l * stride)
 // into the first K, written to out_val/out_col; their number to *out_n.
+template <int NT>
 __device__ __forceinline__ void top_merge(const float *val, const int *col, const int *cnt, int lists, int stride, int K,
                                           float *out_val, int *out_col, int *out_n) {
   int total = 0;
   for (int l = 0; l < lists; l++) total += cnt[l];
-  for (int i = threadIdx.x; i < lists * K; i += kVocThreads) {
+  for (int i = threadIdx.x; i < lists * K; i += NT) {
     const int l = i / K, k = i % K;
     if (k >= cnt[l]) continue;
     const float v = val[l * stride + k];
@@ -540,21 +547,22 @@ __device__ __forceinline__ void top_merge(const float *val, const int *col, cons
   if (threadIdx.x == 0) *out_n = total < K ? total : K;
 }
 
-template <int DT, bool TOP>
-__global__ void __launch_bounds__(kVocThreads, 4) token_logprobs_kernel(const LogprobArgs a) {
+template <int DT, bool TOP, int NT>
+__global__ void __launch_bounds__(NT, 1024 / NT) token_logprobs_kernel(const LogprobArgs a) {
   using E = VElem<DT>;
   using T = typename E::T;
-  __shared__ VStat s_warp[kVocWarps];
+  __shared__ VStat s_warp[NT / 32];
   __shared__ VStat s_part[8];  // on rank 0, the cluster's statistics
-  __shared__ TopShared s_top[1];
-  __shared__ float s_oval[TOP ? 8 * kTopMax : 1];  // this CTA's list, and on rank 0 all the cluster's
-  __shared__ int s_ocol[TOP ? 8 * kTopMax : 1];
+  constexpr int kLists = NT == kVocThreads ? 8 : 1;  // smaller CTAs have their row alone
+  __shared__ TopShared<NT> s_top[1];
+  __shared__ float s_oval[TOP ? kLists * kTopMax : 1];  // this CTA's list, and on rank 0 all the cluster's
+  __shared__ int s_ocol[TOP ? kLists * kTopMax : 1];
   __shared__ int s_cnt[8], s_on;
   __shared__ float s_fval[TOP ? kTopMax : 1];
   __shared__ int s_fcol[TOP ? kTopMax : 1];
   __shared__ __align__(8) uint64_t s_bar;
 
-  const int cs = a.parts, rank = cs > 1 ? (int)cluster_ctarank() : 0;
+  const int cs = NT == kVocThreads ? a.parts : 1, rank = cs > 1 ? (int)cluster_ctarank() : 0;
   const int64_t row = blockIdx.x / cs;
   const RowVecs<DT> rv(static_cast<const T *>(a.x) + row * a.ld, a.V);
   const RowPart<DT> rp(rv, rank, cs);
@@ -570,7 +578,7 @@ __global__ void __launch_bounds__(kVocThreads, 4) token_logprobs_kernel(const Lo
     __syncwarp();
     cluster_announce();
   }
-  // The given tokens' logits, asked for early.
+  // The given tokens' logits (of the first NT), asked for early.
   int id = -1;
   float xt = 0.0f;
   if (rank == 0 && (int)threadIdx.x < a.T) {
@@ -579,16 +587,25 @@ __global__ void __launch_bounds__(kVocThreads, 4) token_logprobs_kernel(const Lo
   }
 
   VStat st{-IG_INF, 0.0f, 0.0f};
-  constexpr int kRound = kVocUnroll * kVocThreads;
+  constexpr int kRound = kVocUnroll * NT;
   const uint4 *p = rp.base + threadIdx.x;
   int i = 0;
-  for (; i + kRound <= rp.n; i += kRound) {
+  if (rp.n >= kRound) {
+    // Each round's vectors are asked for before the one before it is added.
     uint4 raw[kVocUnroll];
 #pragma unroll
-    for (int j = 0; j < kVocUnroll; j++) raw[j] = p[i + j * kVocThreads];
+    for (int j = 0; j < kVocUnroll; j++) raw[j] = p[j * NT];
+    for (i = kRound; i + kRound <= rp.n; i += kRound) {
+      uint4 cur[kVocUnroll];
+#pragma unroll
+      for (int j = 0; j < kVocUnroll; j++) cur[j] = raw[j];
+#pragma unroll
+      for (int j = 0; j < kVocUnroll; j++) raw[j] = p[i + j * NT];
+      vstat_add_raw<DT, true>(st, cur, c2);
+    }
     vstat_add_raw<DT, true>(st, raw, c2);
   }
-  for (i += threadIdx.x; i < rp.n; i += kVocThreads) {
+  for (i += threadIdx.x; i < rp.n; i += NT) {
     const uint4 raw[1] = {rp.base[i]};
     vstat_add_raw<DT, true>(st, raw, c2);
   }
@@ -596,16 +613,16 @@ __global__ void __launch_bounds__(kVocThreads, 4) token_logprobs_kernel(const Lo
     const uint4 raw[1] = {rv.edge(rp.v0)};
     vstat_add_raw<DT, true>(st, raw, c2);
   }
-  if (threadIdx.x == kLastThread && rp.last) {
+  if (threadIdx.x == last_thread(NT) && rp.last) {
     const uint4 raw[1] = {rv.edge(rp.v1 - 1)};
     vstat_add_raw<DT, true>(st, raw, c2);
   }
   const float tmax = st.m;
   st = vstat_warp<true>(st, c2);
   if (lane == 0) s_warp[warp] = st;
-  if constexpr (TOP) top_select<DT>(rv, rp, tmax, a.K, s_top[0], s_oval, s_ocol, &s_on);
+  if constexpr (TOP) top_select<DT, NT>(rv, rp, tmax, a.K, s_top[0], s_oval, s_ocol, &s_on);
   __syncthreads();
-  st = vstat_join<true>(s_warp, kVocWarps, c2);
+  st = vstat_join<true>(s_warp, NT / 32, c2);
   if (cs > 1) {
     cluster_ready();
     if (rank != 0) {
@@ -638,7 +655,11 @@ __global__ void __launch_bounds__(kVocThreads, 4) token_logprobs_kernel(const Lo
     if (a.lse) a.lse[row] = lse;
     if (a.entropy) a.entropy[row] = entropy;
   }
-  if ((int)threadIdx.x < a.T) {
+  for (int k = threadIdx.x; k < a.T; k += NT) {
+    if (k >= NT) {
+      id = a.ids[row * a.T + k];
+      if (id >= 0 && id < a.V) xt = E::get(rv.row[id]);
+    }
     float v = 0.0f;
     if (id >= a.V) {
       v = __int_as_float(0x7FC00000);
@@ -646,19 +667,19 @@ __global__ void __launch_bounds__(kVocThreads, 4) token_logprobs_kernel(const Lo
     } else if (id >= 0) {
       v = row_logprob(xt, st, a.c, log_s);
     }
-    a.logprobs[row * a.T + threadIdx.x] = v;
+    a.logprobs[row * a.T + k] = v;
   }
   if constexpr (TOP) {
     const float *fval = s_oval;
     const int *fcol = s_ocol;
     if (cs > 1) {
-      top_merge(s_oval, s_ocol, s_cnt, cs, kTopMax, a.K, s_fval, s_fcol, &s_on);
+      top_merge<NT>(s_oval, s_ocol, s_cnt, cs, kTopMax, a.K, s_fval, s_fcol, &s_on);
       __syncthreads();
       fval = s_fval;
       fcol = s_fcol;
     }
     const bool nan = st.s != st.s;
-    for (int k = threadIdx.x; k < a.K; k += kVocThreads) {
+    for (int k = threadIdx.x; k < a.K; k += NT) {
       const bool have = k < s_on && !nan;
       a.top_ids[row * a.K + k] = have ? fcol[k] : -1;
       a.top_logprobs[row * a.K + k] =
@@ -680,21 +701,21 @@ struct LogprobGradArgs {
   int64_t ldd;
 };
 
-// The row's gradient outside its given tokens is p (A + B t), t = z - lse:
-//   A = -c (sum of the tokens' gradients + gH H), B = -c gH.
+// The row's gradient outside its given tokens is p (A + B y) with
+// y = log2 p = x c log2(e) - lse log2(e):
+//   A = -c (sum of the tokens' gradients + gH H), B = -c gH ln 2.
 struct RowCoef {
-  float A, B, lse;
+  float A, B, lse2;
 };
-__device__ __forceinline__ float dense_grad(float x, float c, const RowCoef &k) {
-  const float t = max_nan(fmaf(x, c, -k.lse), kYMin);
-  return ex2(t * kLog2e) * fmaf(k.B, t, k.A);
+__device__ __forceinline__ float dense_grad(float x, float c2, const RowCoef &k) {
+  const float y = max_nan(fmaf(x, c2, -k.lse2), kYMin);
+  return ex2(y) * fmaf(k.B, y, k.A);
 }
-__device__ __forceinline__ float2 dense_grad2(float2 x, float c, const RowCoef &k) {
-  float2 t = __ffma2_rn(x, make_float2(c, c), make_float2(-k.lse, -k.lse));
-  t.x = max_nan(t.x, kYMin);
-  t.y = max_nan(t.y, kYMin);
-  const float2 y = __fmul2_rn(t, make_float2(kLog2e, kLog2e));
-  return __fmul2_rn(make_float2(ex2(y.x), ex2(y.y)), __ffma2_rn(make_float2(k.B, k.B), t, make_float2(k.A, k.A)));
+__device__ __forceinline__ float2 dense_grad2(float2 x, float c2, const RowCoef &k) {
+  float2 y = __ffma2_rn(x, make_float2(c2, c2), make_float2(-k.lse2, -k.lse2));
+  y.x = max_nan(y.x, kYMin);
+  y.y = max_nan(y.y, kYMin);
+  return __fmul2_rn(make_float2(ex2(y.x), ex2(y.y)), __ffma2_rn(make_float2(k.B, k.B), y, make_float2(k.A, k.A)));
 }
 // The gradient a given token adds in its own column: c times the sum over the
 // row's entries with the same id, in order.
@@ -719,12 +740,14 @@ __device__ __forceinline__ float given_grad_sum(const int32_t *ids, const float 
 }
 __device__ __forceinline__ RowCoef row_coef(float lse, float H, float G, float gh, float c) {
   RowCoef k;
-  k.B = -c * gh;
+  k.B = -c * gh * kLn2;
   k.A = -c * fmaf(gh, H, G);
-  k.lse = lse;
-  if (lse == -IG_INF) {  // no distribution: p = 0 everywhere
+  k.lse2 = lse * kLog2e;
+  // No distribution: nothing left, or all of it masked by the type's lowest
+  // value, whose lse cannot tell the columns apart.
+  if (k.lse2 < -1.0e38f) {
     k.A = k.B = 0.0f;
-    k.lse = IG_INF;
+    k.lse2 = IG_INF;
   }
   return k;
 }
@@ -751,12 +774,12 @@ __device__ __forceinline__ void store_edge(typename VElem<DT>::T *drow, const Ro
   }
 }
 
-template <int DT>
-__global__ void __launch_bounds__(kVocThreads, 4) token_logprobs_grad_kernel(const LogprobGradArgs a) {
+template <int DT, int NT>
+__global__ void __launch_bounds__(NT, 1024 / NT) token_logprobs_grad_kernel(const LogprobGradArgs a) {
   using E = VElem<DT>;
   using T = typename E::T;
   constexpr int kN = E::kN;
-  __shared__ float s_G;
+  __shared__ float s_G, s_xt[kIdsMax];
   const int64_t row = blockIdx.x / a.segs;
   const int seg = (int)(blockIdx.x - row * a.segs);
   const RowVecs<DT> rv(static_cast<const T *>(a.x) + row * a.ld, a.V);
@@ -765,15 +788,19 @@ __global__ void __launch_bounds__(kVocThreads, 4) token_logprobs_grad_kernel(con
   const RowPart<DT> rp(rv, seg, a.segs);
   const int32_t *ids = a.ids + row * a.T;
   const float *g = a.dlogprobs + row * a.T;
-  // One round of vectors per CTA, asked for before the row's scalars.
+  // Rounds of vectors, each asked for before the one before it is worked on,
+  // the first before the row's scalars.
   const uint4 *p = rp.base + threadIdx.x;
-  const int mine = rp.n - (int)threadIdx.x;  // vector j of the thread is there while j kVocThreads < mine
+  const int mine = rp.n - (int)threadIdx.x;  // the thread's vector i NT is there while i NT < mine
   uint4 raw[kVocUnroll], edge;
+  auto load = [&](int b) {
 #pragma unroll
-  for (int j = 0; j < kVocUnroll; j++)
-    if (j * kVocThreads < mine) raw[j] = __ldcs(p + j * kVocThreads);
+    for (int j = 0; j < kVocUnroll; j++)
+      if (b + j * NT < mine) raw[j] = p[b + j * NT];
+  };
+  load(0);
   if (threadIdx.x == kFirstThread && rp.first) edge = rv.edge(rp.v0);
-  if (threadIdx.x == kLastThread && rp.last) edge = rv.edge(rp.v1 - 1);
+  if (threadIdx.x == last_thread(NT) && rp.last) edge = rv.edge(rp.v1 - 1);
   const float lse = a.lse[row];
   const float gh = a.dentropy ? a.dentropy[row] : 0.0f, H = a.dentropy ? a.entropy[row] : 0.0f;
   if (threadIdx.x < 32) {
@@ -784,41 +811,53 @@ __global__ void __launch_bounds__(kVocThreads, 4) token_logprobs_grad_kernel(con
   }
   // The given tokens' logits are read before any store: dx may be x.
   const int cfirst = max(rv.col(rp.v0), 0), clast = min(rv.col(rp.v1), a.V);
-  float xt = 0.0f;
-  int id = -1;
-  if ((int)threadIdx.x < a.T && a.dlogprobs) {
-    id = ids[threadIdx.x];
-    if (id < cfirst || id >= clast) id = -1;
-    if (id >= 0) xt = E::get(rv.row[id]);
+  if (a.dlogprobs) {
+    for (int i = threadIdx.x; i < a.T; i += NT) {
+      const int id = ids[i];
+      if (id >= cfirst && id < clast) s_xt[i] = E::get(rv.row[id]);
+    }
   }
   __syncthreads();
   const RowCoef k = row_coef(lse, H, s_G, gh, a.c);
+  const float c2 = a.c * kLog2e;
   auto grad = [&](const uint4 &v, float *d) {
     float x[kN];
     E::unpack(v, x);
 #pragma unroll
     for (int i = 0; i < kN; i += 2) {
-      const float2 r = dense_grad2(make_float2(x[i], x[i + 1]), a.c, k);
+      const float2 r = dense_grad2(make_float2(x[i], x[i + 1]), c2, k);
       d[i] = r.x;
       d[i + 1] = r.y;
     }
   };
   T *dp = drow + rv.col(rp.w0) + (int64_t)threadIdx.x * kN;
+  constexpr int kRound = kVocUnroll * NT;
+  for (int b = 0; b < mine; b += kRound) {
+    uint4 cur[kVocUnroll];
 #pragma unroll
-  for (int j = 0; j < kVocUnroll; j++) {
-    if (j * kVocThreads >= mine) break;
-    float d[kN];
-    grad(raw[j], d);
-    store_whole<DT>(dp + j * kVocThreads * kN, same, d);
+    for (int j = 0; j < kVocUnroll; j++) cur[j] = raw[j];
+    load(b + kRound);
+#pragma unroll
+    for (int j = 0; j < kVocUnroll; j++) {
+      if (b + j * NT >= mine) break;
+      float d[kN];
+      grad(cur[j], d);
+      store_whole<DT>(dp + (int64_t)(b + j * NT) * kN, same, d);
+    }
   }
-  if ((threadIdx.x == kFirstThread && rp.first) || (threadIdx.x == kLastThread && rp.last)) {
+  if ((threadIdx.x == kFirstThread && rp.first) || (threadIdx.x == last_thread(NT) && rp.last)) {
     float d[kN];
     grad(edge, d);
     store_edge<DT>(drow, rv, threadIdx.x == kFirstThread ? rp.v0 : rp.v1 - 1, d);
   }
   if (a.T == 0 || !a.dlogprobs) return;
   __syncthreads();
-  if (id >= 0 && lse != -IG_INF) drow[id] = E::put(dense_grad(xt, a.c, k) + token_grad(ids, g, a.T, id, a.c));
+  if (k.lse2 == IG_INF) return;
+  for (int i = threadIdx.x; i < a.T; i += NT) {
+    const int id = ids[i];
+    if (id >= cfirst && id < clast)
+      drow[id] = E::put(dense_grad(s_xt[i], c2, k) + token_grad(ids, g, a.T, id, a.c));
+  }
 }
 
 // ---- divergence from a teacher's top logits ----------------------------------------------
@@ -854,21 +893,21 @@ __device__ __forceinline__ void bulk_load(void *dst, const void *src, uint32_t b
                : "memory");
 }
 
-template <int DT, bool TAIL, bool STAGED>
-__global__ void __launch_bounds__(kVocThreads, 4) distill_topk_kernel(const DistillArgs a) {
+template <int DT, bool TAIL, bool STAGED, int NT>
+__global__ void __launch_bounds__(NT, 1024 / NT) distill_topk_kernel(const DistillArgs a) {
   using E = VElem<DT>;
   using T = typename E::T;
   constexpr int kN = E::kN;
   constexpr int kR = 4;  // vectors per thread and step
   extern __shared__ uint4 s_dyn[];
-  __shared__ VStat s_warp[kVocWarps];
+  __shared__ VStat s_warp[NT / 32];
   __shared__ VStat s_part[8];  // every CTA's statistics
   __shared__ VStat s_list;     // with TAIL: the listed columns'
   __shared__ float s_mass[2];  // the sum of q, what is left of 1
-  __shared__ int s_ids[kTeacherMax], s_once[kTeacherMax];
-  __shared__ float s_q[kTeacherMax], s_xk[kTeacherMax];
+  __shared__ int s_ids[kIdsMax], s_once[kIdsMax];
+  __shared__ float s_q[kIdsMax], s_xk[kIdsMax];
   __shared__ __align__(8) uint64_t s_bar[kStageParts + 1];
-  const int cs = a.parts, rank = cs > 1 ? (int)cluster_ctarank() : 0;
+  const int cs = NT == kVocThreads ? a.parts : 1, rank = cs > 1 ? (int)cluster_ctarank() : 0;
   const int64_t row = blockIdx.x / cs;
   const RowVecs<DT> rv(static_cast<const T *>(a.x) + row * a.ld, a.V);
   const RowPart<DT> rp(rv, rank, cs);
@@ -876,7 +915,7 @@ __global__ void __launch_bounds__(kVocThreads, 4) distill_topk_kernel(const Dist
   const float c2 = a.c * kLog2e;
   uint8_t *s_mask = reinterpret_cast<uint8_t *>(s_dyn + (STAGED ? rp.n : 0));  // of vector v0 + i
   // Quarters of whole steps.
-  constexpr int kStep = kR * kVocThreads;
+  constexpr int kStep = kR * NT;
   const int quarter = ((rp.n + kStageParts - 1) / kStageParts + kStep - 1) / kStep * kStep;
   if (tid == 0) {
     for (int i = 0; i <= kStageParts; i++) mbar_init(&s_bar[i], 1);
@@ -896,7 +935,7 @@ __global__ void __launch_bounds__(kVocThreads, 4) distill_topk_kernel(const Dist
   if (cs > 1) cluster_announce();
   const uint4 *src = STAGED ? s_dyn : rp.base;
   uint4 edge;
-  const bool has_edge = (tid == kFirstThread && rp.first) || (tid == kLastThread && rp.last);
+  const bool has_edge = (tid == kFirstThread && rp.first) || (tid == last_thread(NT) && rp.last);
   const int edge_v = tid == kFirstThread ? rp.v0 : rp.v1 - 1;
   if (has_edge) edge = rv.edge(edge_v);
 
@@ -904,34 +943,33 @@ __global__ void __launch_bounds__(kVocThreads, 4) distill_topk_kernel(const Dist
   T *drow = a.dx ? static_cast<T *>(a.dx) + row * a.ldd : nullptr;
   const bool same = (reinterpret_cast<uintptr_t>(drow) & 15) == (reinterpret_cast<uintptr_t>(rv.row) & 15);
 
-  // The teacher's list: thread k brings entry k.
-  int id = -1;
-  if (tid < a.K) {
-    id = a.tids[row * a.K + tid];
-    if (id >= a.V) {
-      set_device_error(kDevBadId);
-      id = -1;
-    }
-    if (id < 0) id = -1;
-    s_ids[tid] = id;
-    s_q[tid] = id >= 0 ? a.tlogits[row * a.K + tid] : -IG_INF;
-    s_xk[tid] = id >= 0 ? E::get(rv.row[id]) : -IG_INF;
+  // The teacher's list.
+  bool some = false;
+  for (int k = tid; k < a.K; k += NT) {
+    int id = a.tids[row * a.K + k];
+    if (id >= a.V) set_device_error(kDevBadId);
+    if (id < 0 || id >= a.V) id = -1;
+    some |= id >= 0;
+    s_ids[k] = id;
+    s_q[k] = id >= 0 ? a.tlogits[row * a.K + k] : -IG_INF;
+    s_xk[k] = id >= 0 ? E::get(rv.row[id]) : -IG_INF;
   }
   if constexpr (TAIL) {
     const int nw = (rp.v1 - rp.v0 + 3) / 4;
-    for (int i = tid; i < nw; i += kVocThreads) reinterpret_cast<uint32_t *>(s_mask)[i] = 0;
+    for (int i = tid; i < nw; i += NT) reinterpret_cast<uint32_t *>(s_mask)[i] = 0;
   }
-  const int any = __syncthreads_or(id >= 0);
+  const int any = __syncthreads_or(some);
   const bool skip = !any || w == 0.0f;  // uniform over the cluster
   const int cfirst = max(rv.col(rp.v0), 0), clast = min(rv.col(rp.v1), a.V);
   VStat st{-IG_INF, 0.0f, 0.0f};
   if (!skip) {
     if constexpr (TAIL) {
-      if (tid < a.K) {
+      for (int k = tid; k < a.K; k += NT) {
+        const int id = s_ids[k];
         int once = id >= 0;  // the first entry with its id
-        for (int k = 0; k < tid; k++)
-          if (s_ids[k] == id) once = 0;
-        s_once[tid] = once;
+        for (int j = 0; j < k; j++)
+          if (s_ids[j] == id) once = 0;
+        s_once[k] = once;
         if (id >= cfirst && id < clast) {
           const int at = id + rv.mis - rp.v0 * kN, i = at / kN;
           atomicOr(reinterpret_cast<uint32_t *>(s_mask) + (i >> 2), 1u << ((i & 3) * 8 + at % kN));
@@ -996,13 +1034,13 @@ __global__ void __launch_bounds__(kVocThreads, 4) distill_topk_kernel(const Dist
       if constexpr (STAGED) mbar_wait(&s_bar[b / quarter], 0, kDevTimeoutFull);
       const int end = min(b + quarter, rp.n);
       int i = b + tid;
-      for (; i + kStep - kVocThreads < end; i += kStep) {
+      for (; i + kStep - NT < end; i += kStep) {
         uint4 raw[kR];
 #pragma unroll
-        for (int j = 0; j < kR; j++) raw[j] = unlisted(src[i + j * kVocThreads], rp.w0 + i + j * kVocThreads);
+        for (int j = 0; j < kR; j++) raw[j] = unlisted(src[i + j * NT], rp.w0 + i + j * NT);
         vstat_add_raw<DT, false>(st, raw, c2);
       }
-      for (; i < end; i += kVocThreads) {
+      for (; i < end; i += NT) {
         const uint4 raw[1] = {unlisted(src[i], rp.w0 + i)};
         vstat_add_raw<DT, false>(st, raw, c2);
       }
@@ -1014,7 +1052,7 @@ __global__ void __launch_bounds__(kVocThreads, 4) distill_topk_kernel(const Dist
     st = vstat_warp<false>(st, c2);
     if (lane == 0) s_warp[warp] = st;
     __syncthreads();
-    st = vstat_join<false>(s_warp, kVocWarps, c2);
+    st = vstat_join<false>(s_warp, NT / 32, c2);
   } else if constexpr (STAGED) {
     // The copies end before this CTA does.
     for (int i = 0; i < kStageParts; i++) mbar_wait(&s_bar[i], 0, kDevTimeoutFull);
@@ -1098,22 +1136,22 @@ __global__ void __launch_bounds__(kVocThreads, 4) distill_topk_kernel(const Dist
   T *dp = drow + rv.col(rp.w0);
   if (zero) {
     float d[kN] = {};
-    for (int i = tid; i < rp.n; i += kVocThreads) store_whole<DT>(dp + (int64_t)i * kN, same, d);
+    for (int i = tid; i < rp.n; i += NT) store_whole<DT>(dp + (int64_t)i * kN, same, d);
     if (has_edge) store_edge<DT>(drow, rv, edge_v, d);
   } else {
     int i = tid;
-    for (; i + kStep - kVocThreads < rp.n; i += kStep) {
+    for (; i + kStep - NT < rp.n; i += kStep) {
       uint4 raw[kR];
 #pragma unroll
-      for (int j = 0; j < kR; j++) raw[j] = src[i + j * kVocThreads];
+      for (int j = 0; j < kR; j++) raw[j] = src[i + j * NT];
 #pragma unroll
       for (int j = 0; j < kR; j++) {
         float d[kN];
         grad(raw[j], d);
-        store_whole<DT>(dp + (int64_t)(i + j * kVocThreads) * kN, same, d);
+        store_whole<DT>(dp + (int64_t)(i + j * NT) * kN, same, d);
       }
     }
-    for (; i < rp.n; i += kVocThreads) {
+    for (; i < rp.n; i += NT) {
       float d[kN];
       grad(src[i], d);
       store_whole<DT>(dp + (int64_t)i * kN, same, d);
@@ -1128,30 +1166,41 @@ __global__ void __launch_bounds__(kVocThreads, 4) distill_topk_kernel(const Dist
   __syncthreads();
   // The listed columns of this CTA's part; q of equal ids adds up (each of
   // their threads stores the same value).
-  if (id >= cfirst && id < clast) {
+  for (int i = tid; i < a.K; i += NT) {
+    const int id = s_ids[i];
+    if (id < cfirst || id >= clast) continue;
     float q = 0.0f;
     for (int k = 0; k < a.K; k++)
       if (s_ids[k] == id) q += s_q[k];
-    drow[id] = E::put(listed * ex2((s_xk[tid] - row_m) * c2 - row_l2) - w * a.c * q);
+    drow[id] = E::put(listed * ex2((s_xk[i] - row_m) * c2 - row_l2) - w * a.c * q);
   }
 }
 
 // ---- launches --------------------------------------------------------------------------
 
-// CTAs per row (a cluster): more than one while the rows alone do not give
-// every SM several CTAs and a part keeps at least one round of vectors.
-static int row_parts(int64_t rows, int V, int per_vec) {
-  const int64_t nv = (V + per_vec - 1) / per_vec;
-  int cs = 1;
-  while (cs < 8 && rows * cs < 4 * 4 * num_sms() && nv / (2 * cs) >= kVocThreads) cs *= 2;
-  return cs;
+// Threads per CTA and CTAs per row (a cluster).
+struct RowShape {
+  int threads, parts;
+};
+static RowShape row_shape(int64_t rows, int64_t nv) {
+  RowShape r{kVocThreads, 1};
+  // Many short rows: small CTAs, so that an SM has more rows on the way (a
+  // row's start and end cost as much as 16 vectors per thread), while the
+  // rows' threads fill the GPU.
+  while (r.threads > 32 && nv <= 8 * r.threads && rows * (r.threads / 2) >= num_sms() * 1024) r.threads /= 2;
+  // Few rows: several CTAs each, of a round of vectors at least.
+  while (r.threads == kVocThreads && r.parts < 8 && rows * r.parts < 2 * 4 * num_sms() &&
+         nv / (2 * r.parts) >= kVocThreads)
+    r.parts *= 2;
+  return r;
 }
 
 template <typename Args>
-static cudaError_t launch_rows(void (*kern)(Args), const Args &a, int64_t rows, int cs, size_t smem, cudaStream_t st) {
+static cudaError_t launch_rows(void (*kern)(Args), const Args &a, int64_t ctas, int threads, int cs, size_t smem,
+                               cudaStream_t st) {
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(rows * cs));
-  cfg.blockDim = dim3(kVocThreads);
+  cfg.gridDim = dim3((unsigned)ctas);
+  cfg.blockDim = dim3(threads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
   cudaLaunchAttribute attr[1];
@@ -1166,43 +1215,62 @@ static cudaError_t launch_rows(void (*kern)(Args), const Args &a, int64_t rows, 
   return cudaLaunchKernelEx(&cfg, kern, a);
 }
 
+#define IG_BY_THREADS(n, CALL) \
+  ((n) == 256 ? CALL(256) : (n) == 128 ? CALL(128) : (n) == 64 ? CALL(64) : CALL(32))
+
 template <int DT>
 static cudaError_t run_token_logprobs(LogprobArgs a, cudaStream_t st) {
-  const int cs = a.parts = row_parts(a.rows, a.V, VElem<DT>::kN);
-  return a.K > 0 ? launch_rows(token_logprobs_kernel<DT, true>, a, a.rows, cs, 0, st)
-                 : launch_rows(token_logprobs_kernel<DT, false>, a, a.rows, cs, 0, st);
+  const RowShape r = row_shape(a.rows, a.V / VElem<DT>::kN);
+  a.parts = r.parts;
+  const int64_t ctas = a.rows * r.parts;
+#define IG_CALL(NT)                                                                                   \
+  (a.K > 0 ? launch_rows(token_logprobs_kernel<DT, true, NT>, a, ctas, NT, r.parts, 0, st)            \
+           : launch_rows(token_logprobs_kernel<DT, false, NT>, a, ctas, NT, r.parts, 0, st))
+  return IG_BY_THREADS(r.threads, IG_CALL);
+#undef IG_CALL
 }
 
 template <int DT>
 static cudaError_t run_token_logprobs_grad(LogprobGradArgs a, cudaStream_t st) {
   const int64_t nv = (a.V + VElem<DT>::kN - 1) / VElem<DT>::kN + 1;  // a row off the boundary spans one more
-  const int64_t round = kVocUnroll * kVocThreads;
-  a.segs = (int)((nv + round - 1) / round);
-  return launch_rows(token_logprobs_grad_kernel<DT>, a, a.rows * a.segs, 1, 0, st);
+  const int nt = row_shape(a.rows, a.V / VElem<DT>::kN).threads;
+  const int64_t rounds = (nv + kVocUnroll * nt - 1) / (kVocUnroll * nt);
+  // Several rounds per CTA (a CTA's start costs about as much as a round)
+  // while there are CTAs enough to fill the GPU four times.
+  int64_t per = rounds;
+  while (per > 1 && a.rows * ((rounds + per - 1) / per) * nt < 4 * 1024 * num_sms()) per = (per + 1) / 2;
+  a.segs = (int)((rounds + per - 1) / per);
+  const int64_t ctas = a.rows * a.segs;
+  if (ctas > INT32_MAX) return cudaErrorInvalidConfiguration;
+#define IG_CALL(NT) launch_rows(token_logprobs_grad_kernel<DT, NT>, a, ctas, NT, 1, 0, st)
+  return IG_BY_THREADS(nt, IG_CALL);
+#undef IG_CALL
 }
 
-template <int DT, bool TAIL, bool STAGED>
-static cudaError_t launch_distill(const DistillArgs &a, int cs, size_t smem, cudaStream_t st) {
+template <int DT, bool TAIL, bool STAGED, int NT>
+static cudaError_t launch_distill(const DistillArgs &a, size_t smem, cudaStream_t st) {
   static SmemOptIn attr;
-  const cudaError_t e = attr.ensure((const void *)distill_topk_kernel<DT, TAIL, STAGED>, (int)smem);
+  const cudaError_t e = attr.ensure((const void *)distill_topk_kernel<DT, TAIL, STAGED, NT>, (int)smem);
   if (e != cudaSuccess) return e;
-  return launch_rows(distill_topk_kernel<DT, TAIL, STAGED>, a, a.rows, cs, smem, st);
+  return launch_rows(distill_topk_kernel<DT, TAIL, STAGED, NT>, a, a.rows * a.parts, NT, a.parts, smem, st);
 }
 
 template <int DT>
 static cudaError_t run_distill(DistillArgs a, bool tail, cudaStream_t st) {
   const int64_t nv = a.V / VElem<DT>::kN + 2;
-  int cs = row_parts(a.rows, a.V, VElem<DT>::kN);
+  RowShape r = row_shape(a.rows, a.V / VElem<DT>::kN);
   // Parts of at most 52 KB where the cluster allows it: four CTAs per SM.
-  while (cs < 8 && nv * 16 / cs > 52 * 1024) cs *= 2;
-  a.parts = cs;
-  const int64_t part = nv / cs + 1;
+  while (r.threads == kVocThreads && r.parts < 8 && nv * 16 / r.parts > 52 * 1024) r.parts *= 2;
+  a.parts = r.parts;
+  const int64_t part = nv / r.parts + 1;
   const bool staged = part * 16 <= kStageMax;
-  const size_t bits = tail ? (part / 4 + 1) * 4 : 0;
-  const size_t smem = bits + (staged ? part * 16 : 0);
-  if (staged)
-    return tail ? launch_distill<DT, true, true>(a, cs, smem, st) : launch_distill<DT, false, true>(a, cs, smem, st);
-  return tail ? launch_distill<DT, true, false>(a, cs, smem, st) : launch_distill<DT, false, false>(a, cs, smem, st);
+  const size_t smem = (tail ? (part / 4 + 1) * 4 : 0) + (staged ? part * 16 : 0);
+  if (!staged)
+    return tail ? launch_distill<DT, true, false, kVocThreads>(a, smem, st)
+                : launch_distill<DT, false, false, kVocThreads>(a, smem, st);
+#define IG_CALL(NT) (tail ? launch_distill<DT, true, true, NT>(a, smem, st) : launch_distill<DT, false, true, NT>(a, smem, st))
+  return IG_BY_THREADS(r.threads, IG_CALL);
+#undef IG_CALL
 }
 
 }  // namespace ig
