@@ -875,65 +875,44 @@ struct DistillArgs {
   int parts;  // CTAs per row (a cluster)
 };
 
-// One cluster per row. The row's part is copied to shared memory in four bulk
-// copies (STAGED), so the statistics' pass starts on the first quarter and the
-// gradient's pass reads no global memory; rows too long for that (over 8 x
-// kStageMax bytes) are read twice, the second time from L2. The teacher's list
-// is worked on by one warp while the others start on the row. With TAIL the
+// One cluster per row, in two passes over it: the statistics, then the
+// gradient while the row is still in L2. (Holding the row's part in shared
+// memory instead, by bulk copies, took 207 us for 4096 x 50021 bf16 against
+// 178: the copies' wait and the clusters that make room cost more than the
+// second read.) The teacher's list is worked on by one warp. With TAIL the
 // mass outside the list is summed on its own (1 - the list's mass would lose
 // it to cancellation): a byte per vector in shared memory marks its listed
 // columns.
-constexpr int kStageParts = 4;
-constexpr int kStageMax = 160 * 1024;
-
-__device__ __forceinline__ void bulk_load(void *dst, const void *src, uint32_t bytes, uint64_t *bar) {
-  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
-                   smem_u32(dst)),
-               "l"(src), "r"(bytes), "r"(smem_u32(bar))
-               : "memory");
-}
-
-template <int DT, bool TAIL, bool STAGED, int NT>
+template <int DT, bool TAIL, int NT>
 __global__ void __launch_bounds__(NT, 1024 / NT) distill_topk_kernel(const DistillArgs a) {
   using E = VElem<DT>;
   using T = typename E::T;
   constexpr int kN = E::kN;
-  constexpr int kR = 4;  // vectors per thread and step
-  extern __shared__ uint4 s_dyn[];
+  extern __shared__ uint32_t s_dyn[];
   __shared__ VStat s_warp[NT / 32];
   __shared__ VStat s_part[8];  // every CTA's statistics
   __shared__ VStat s_list;     // with TAIL: the listed columns'
   __shared__ float s_mass[2];  // the sum of q, what is left of 1
   __shared__ int s_ids[kIdsMax], s_once[kIdsMax];
   __shared__ float s_q[kIdsMax], s_xk[kIdsMax];
-  __shared__ __align__(8) uint64_t s_bar[kStageParts + 1];
+  __shared__ __align__(8) uint64_t s_bar;
   const int cs = NT == kVocThreads ? a.parts : 1, rank = cs > 1 ? (int)cluster_ctarank() : 0;
   const int64_t row = blockIdx.x / cs;
   const RowVecs<DT> rv(static_cast<const T *>(a.x) + row * a.ld, a.V);
   const RowPart<DT> rp(rv, rank, cs);
   const int tid = (int)threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const float c2 = a.c * kLog2e;
-  uint8_t *s_mask = reinterpret_cast<uint8_t *>(s_dyn + (STAGED ? rp.n : 0));  // of vector v0 + i
-  // Quarters of whole steps.
-  constexpr int kStep = kR * NT;
-  const int quarter = ((rp.n + kStageParts - 1) / kStageParts + kStep - 1) / kStep * kStep;
-  if (tid == 0) {
-    for (int i = 0; i <= kStageParts; i++) mbar_init(&s_bar[i], 1);
+  uint8_t *s_mask = reinterpret_cast<uint8_t *>(s_dyn);  // of vector v0 + i
+  if (tid == 0 && cs > 1) {
+    mbar_init(&s_bar, 1);
     fence_barrier_init();
-    mbar_arrive_expect_tx(&s_bar[kStageParts], (uint32_t)(cs - 1) * 8u);
-    if constexpr (STAGED) {
-      fence_proxy_async_smem();
-      for (int i = 0; i < kStageParts; i++) {
-        const int p0 = i * quarter, p1 = min(p0 + quarter, rp.n);
-        const uint32_t bytes = p1 > p0 ? (uint32_t)(p1 - p0) * 16u : 0u;
-        mbar_arrive_expect_tx(&s_bar[i], bytes);
-        if (bytes) bulk_load(s_dyn + p0, rp.base + p0, bytes, &s_bar[i]);
-      }
-    }
+    mbar_arrive_expect_tx(&s_bar, (uint32_t)(cs - 1) * 8u);
   }
   __syncwarp();
   if (cs > 1) cluster_announce();
-  const uint4 *src = STAGED ? s_dyn : rp.base;
+  const uint4 *src = rp.base + tid;
+  const int mine = rp.n - tid;  // the thread's vector i NT is there while i NT < mine
+  constexpr int kRound = kVocUnroll * NT;
   uint4 edge;
   const bool has_edge = (tid == kFirstThread && rp.first) || (tid == last_thread(NT) && rp.last);
   const int edge_v = tid == kFirstThread ? rp.v0 : rp.v1 - 1;
@@ -943,16 +922,17 @@ __global__ void __launch_bounds__(NT, 1024 / NT) distill_topk_kernel(const Disti
   T *drow = a.dx ? static_cast<T *>(a.dx) + row * a.ldd : nullptr;
   const bool same = (reinterpret_cast<uintptr_t>(drow) & 15) == (reinterpret_cast<uintptr_t>(rv.row) & 15);
 
-  // The teacher's list.
+  // The teacher's list is the first warp's: the ids now, the values and their
+  // logits asked for before the row's pass and worked on after its share of it.
   bool some = false;
-  for (int k = tid; k < a.K; k += NT) {
-    int id = a.tids[row * a.K + k];
-    if (id >= a.V) set_device_error(kDevBadId);
-    if (id < 0 || id >= a.V) id = -1;
-    some |= id >= 0;
-    s_ids[k] = id;
-    s_q[k] = id >= 0 ? a.tlogits[row * a.K + k] : -IG_INF;
-    s_xk[k] = id >= 0 ? E::get(rv.row[id]) : -IG_INF;
+  if (warp == 0) {
+    for (int k = lane; k < a.K; k += 32) {
+      int id = a.tids[row * a.K + k];
+      if (id >= a.V) set_device_error(kDevBadId);
+      if (id < 0 || id >= a.V) id = -1;
+      some |= id >= 0;
+      s_ids[k] = id;
+    }
   }
   if constexpr (TAIL) {
     const int nw = (rp.v1 - rp.v0 + 3) / 4;
@@ -963,6 +943,18 @@ __global__ void __launch_bounds__(NT, 1024 / NT) distill_topk_kernel(const Disti
   const int cfirst = max(rv.col(rp.v0), 0), clast = min(rv.col(rp.v1), a.V);
   VStat st{-IG_INF, 0.0f, 0.0f};
   if (!skip) {
+    constexpr int kHeld = 2;  // entries per lane in registers
+    float held_t[kHeld], held_x[kHeld];
+    auto entry = [&](int k, float &t, float &x) {
+      const int id = s_ids[k];
+      t = id >= 0 ? a.tlogits[row * a.K + k] : -IG_INF;
+      x = id >= 0 ? E::get(rv.row[id]) : -IG_INF;
+    };
+    if (warp == 0) {
+#pragma unroll
+      for (int j = 0; j < kHeld; j++)
+        if (lane + 32 * j < a.K) entry(lane + 32 * j, held_t[j], held_x[j]);
+    }
     if constexpr (TAIL) {
       for (int k = tid; k < a.K; k += NT) {
         const int id = s_ids[k];
@@ -976,44 +968,6 @@ __global__ void __launch_bounds__(NT, 1024 / NT) distill_topk_kernel(const Disti
         }
       }
       __syncthreads();
-    }
-    if (warp == 0) {
-      // q over the list, in place of the teacher's values.
-      float q_sum = 0.0f, q_rest = 0.0f;
-      if constexpr (TAIL) {
-        VStat l{-IG_INF, 0.0f, 0.0f};
-        for (int k = lane; k < a.K; k += 32) {
-          const float q = expf(s_q[k]);  // 0 for a missing entry
-          s_q[k] = q;
-          q_sum += q;
-          const float x = s_xk[k];
-          // A listed +inf or NaN: no distribution, s is NaN from here on.
-          const float one = x == -IG_INF ? 0.0f : (x < IG_INF ? 1.0f : __int_as_float(0x7FC00000));
-          if (s_once[k]) vstat_merge<false>(l, VStat{fmaxf(x, -IG_INF), one, 0.0f}, c2);
-        }
-        q_sum = warp_sum(q_sum);
-        q_rest = q_sum == q_sum ? fmaxf(1.0f - q_sum, 0.0f) : q_sum;
-        l = vstat_warp<false>(l, c2);
-        if (lane == 0) s_list = l;
-      } else {
-        float top = -IG_INF;
-        for (int k = lane; k < a.K; k += 32) top = max_nan(top, s_q[k]);
-        float nan = top != top ? top : 0.0f;
-        top = warp_max(top);
-        for (int k = lane; k < a.K; k += 32) {
-          const float e = top == -IG_INF ? 0.0f : expf((s_q[k] - top) * a.c);
-          s_q[k] = e;
-          q_sum += e;
-        }
-        q_sum = warp_sum(q_sum + nan);
-        const float inv = q_sum > 0.0f || q_sum != q_sum ? 1.0f / q_sum : 0.0f;
-        for (int k = lane; k < a.K; k += 32) s_q[k] *= inv;
-        q_sum = q_sum > 0.0f ? 1.0f : q_sum;
-      }
-      if (lane == 0) {
-        s_mass[0] = q_sum;
-        s_mass[1] = q_rest;
-      }
     }
     // A vector as the statistics see it: the listed columns are left out of the tail's.
     auto unlisted = [&](uint4 raw, int v) {
@@ -1030,20 +984,27 @@ __global__ void __launch_bounds__(NT, 1024 / NT) distill_topk_kernel(const Disti
       }
       return raw;
     };
-    for (int b = 0; b < rp.n; b += quarter) {
-      if constexpr (STAGED) mbar_wait(&s_bar[b / quarter], 0, kDevTimeoutFull);
-      const int end = min(b + quarter, rp.n);
-      int i = b + tid;
-      for (; i + kStep - NT < end; i += kStep) {
-        uint4 raw[kR];
+    int i = 0;
+    if (rp.n >= kRound) {
+      // Each round's vectors are asked for before the one before it is added.
+      uint4 raw[kVocUnroll];
 #pragma unroll
-        for (int j = 0; j < kR; j++) raw[j] = unlisted(src[i + j * NT], rp.w0 + i + j * NT);
-        vstat_add_raw<DT, false>(st, raw, c2);
+      for (int j = 0; j < kVocUnroll; j++) raw[j] = src[j * NT];
+      for (i = kRound; i <= rp.n; i += kRound) {
+        uint4 cur[kVocUnroll];
+#pragma unroll
+        for (int j = 0; j < kVocUnroll; j++) cur[j] = unlisted(raw[j], rp.w0 + i - kRound + j * NT + tid);
+        if (i + kRound <= rp.n) {
+#pragma unroll
+          for (int j = 0; j < kVocUnroll; j++) raw[j] = src[i + j * NT];
+        }
+        vstat_add_raw<DT, false>(st, cur, c2);
       }
-      for (; i < end; i += NT) {
-        const uint4 raw[1] = {unlisted(src[i], rp.w0 + i)};
-        vstat_add_raw<DT, false>(st, raw, c2);
-      }
+      i -= kRound;
+    }
+    for (; i < mine; i += NT) {
+      const uint4 raw[1] = {unlisted(src[i], rp.w0 + i + tid)};
+      vstat_add_raw<DT, false>(st, raw, c2);
     }
     if (has_edge) {
       const uint4 raw[1] = {unlisted(edge, edge_v)};
@@ -1051,11 +1012,59 @@ __global__ void __launch_bounds__(NT, 1024 / NT) distill_topk_kernel(const Disti
     }
     st = vstat_warp<false>(st, c2);
     if (lane == 0) s_warp[warp] = st;
+    if (warp == 0) {
+      // s_q: q over the list; s_mass: its sum, and what it leaves of 1.
+      float q_sum = 0.0f, q_rest = 0.0f, top = -IG_INF;
+      VStat l{-IG_INF, 0.0f, 0.0f};
+#pragma unroll
+      for (int j = 0; j < kIdsMax / 32; j++) {
+        const int k = lane + 32 * j;
+        if (k >= a.K) break;
+        float t, x;
+        if (j < kHeld) {
+          t = held_t[j < kHeld ? j : 0];
+          x = held_x[j < kHeld ? j : 0];
+        } else {
+          entry(k, t, x);
+        }
+        s_xk[k] = x;
+        if constexpr (TAIL) {
+          const float q = expf(t);  // 0 for a missing entry
+          s_q[k] = q;
+          q_sum += q;
+          // A listed +inf or NaN: no distribution, s is NaN from here on.
+          const float one = x == -IG_INF ? 0.0f : (x < IG_INF ? 1.0f : __int_as_float(0x7FC00000));
+          if (s_once[k]) vstat_merge<false>(l, VStat{fmaxf(x, -IG_INF), one, 0.0f}, c2);
+        } else {
+          s_q[k] = t;
+          top = max_nan(top, t);
+        }
+      }
+      if constexpr (TAIL) {
+        q_sum = warp_sum(q_sum);
+        q_rest = q_sum == q_sum ? fmaxf(1.0f - q_sum, 0.0f) : q_sum;
+        l = vstat_warp<false>(l, c2);
+        if (lane == 0) s_list = l;
+      } else {
+        const float nan = top != top ? top : 0.0f;
+        top = warp_max(top);
+        for (int k = lane; k < a.K; k += 32) {
+          const float e = top == -IG_INF ? 0.0f : expf((s_q[k] - top) * a.c);
+          s_q[k] = e;
+          q_sum += e;
+        }
+        q_sum = warp_sum(q_sum + nan);
+        const float inv = q_sum > 0.0f || q_sum != q_sum ? 1.0f / q_sum : 0.0f;
+        for (int k = lane; k < a.K; k += 32) s_q[k] *= inv;
+        q_sum = q_sum > 0.0f ? 1.0f : q_sum;
+      }
+      if (lane == 0) {
+        s_mass[0] = q_sum;
+        s_mass[1] = q_rest;
+      }
+    }
     __syncthreads();
     st = vstat_join<false>(s_warp, NT / 32, c2);
-  } else if constexpr (STAGED) {
-    // The copies end before this CTA does.
-    for (int i = 0; i < kStageParts; i++) mbar_wait(&s_bar[i], 0, kDevTimeoutFull);
   }
   if (cs > 1) {
     // Every CTA hands its statistics to every other one. (Each has its list's
@@ -1065,11 +1074,11 @@ __global__ void __launch_bounds__(NT, 1024 / NT) distill_topk_kernel(const Disti
       if (tid == rank) {
         s_part[rank] = st;
       } else {
-        st_async_f32(&s_part[rank].m, tid, st.m, &s_bar[kStageParts]);
-        st_async_f32(&s_part[rank].s, tid, st.s, &s_bar[kStageParts]);
+        st_async_f32(&s_part[rank].m, tid, st.m, &s_bar);
+        st_async_f32(&s_part[rank].s, tid, st.s, &s_bar);
       }
     }
-    mbar_wait_cluster(&s_bar[kStageParts], 0, kDevTimeoutFull);
+    mbar_wait_cluster(&s_bar, 0, kDevTimeoutFull);
     __syncthreads();
     st = vstat_join<false>(s_part, cs, c2);
   }
@@ -1133,28 +1142,31 @@ __global__ void __launch_bounds__(NT, 1024 / NT) distill_topk_kernel(const Disti
       d[e + 1] = r.y;
     }
   };
-  T *dp = drow + rv.col(rp.w0);
+  T *dp = drow + rv.col(rp.w0) + (int64_t)tid * kN;
   if (zero) {
     float d[kN] = {};
-    for (int i = tid; i < rp.n; i += NT) store_whole<DT>(dp + (int64_t)i * kN, same, d);
+    for (int i = 0; i < mine; i += NT) store_whole<DT>(dp + (int64_t)i * kN, same, d);
     if (has_edge) store_edge<DT>(drow, rv, edge_v, d);
   } else {
-    int i = tid;
-    for (; i + kStep - NT < rp.n; i += kStep) {
-      uint4 raw[kR];
+    uint4 raw[kVocUnroll];
+    auto load = [&](int b) {
 #pragma unroll
-      for (int j = 0; j < kR; j++) raw[j] = src[i + j * NT];
+      for (int j = 0; j < kVocUnroll; j++)
+        if (b + j * NT < mine) raw[j] = src[b + j * NT];
+    };
+    load(0);
+    for (int b = 0; b < mine; b += kRound) {
+      uint4 cur[kVocUnroll];
 #pragma unroll
-      for (int j = 0; j < kR; j++) {
+      for (int j = 0; j < kVocUnroll; j++) cur[j] = raw[j];
+      load(b + kRound);
+#pragma unroll
+      for (int j = 0; j < kVocUnroll; j++) {
+        if (b + j * NT >= mine) break;
         float d[kN];
-        grad(raw[j], d);
-        store_whole<DT>(dp + (int64_t)(i + j * NT) * kN, same, d);
+        grad(cur[j], d);
+        store_whole<DT>(dp + (int64_t)(b + j * NT) * kN, same, d);
       }
-    }
-    for (; i < rp.n; i += NT) {
-      float d[kN];
-      grad(src[i], d);
-      store_whole<DT>(dp + (int64_t)i * kN, same, d);
     }
     if (has_edge) {
       float d[kN];
@@ -1247,28 +1259,23 @@ static cudaError_t run_token_logprobs_grad(LogprobGradArgs a, cudaStream_t st) {
 #undef IG_CALL
 }
 
-template <int DT, bool TAIL, bool STAGED, int NT>
+template <int DT, bool TAIL, int NT>
 static cudaError_t launch_distill(const DistillArgs &a, size_t smem, cudaStream_t st) {
   static SmemOptIn attr;
-  const cudaError_t e = attr.ensure((const void *)distill_topk_kernel<DT, TAIL, STAGED, NT>, (int)smem);
+  const cudaError_t e = attr.ensure((const void *)distill_topk_kernel<DT, TAIL, NT>, (int)smem);
   if (e != cudaSuccess) return e;
-  return launch_rows(distill_topk_kernel<DT, TAIL, STAGED, NT>, a, a.rows * a.parts, NT, a.parts, smem, st);
+  return launch_rows(distill_topk_kernel<DT, TAIL, NT>, a, a.rows * a.parts, NT, a.parts, smem, st);
 }
 
 template <int DT>
 static cudaError_t run_distill(DistillArgs a, bool tail, cudaStream_t st) {
   const int64_t nv = a.V / VElem<DT>::kN + 2;
   RowShape r = row_shape(a.rows, a.V / VElem<DT>::kN);
-  // Parts of at most 52 KB where the cluster allows it: four CTAs per SM.
-  while (r.threads == kVocThreads && r.parts < 8 && nv * 16 / r.parts > 52 * 1024) r.parts *= 2;
+  // The rows on the way between their two passes have to stay in L2.
+  while (a.dx && r.threads == kVocThreads && r.parts < 8 && nv * 16 * (4 * num_sms() / r.parts) > (100ll << 20)) r.parts *= 2;
   a.parts = r.parts;
-  const int64_t part = nv / r.parts + 1;
-  const bool staged = part * 16 <= kStageMax;
-  const size_t smem = (tail ? (part / 4 + 1) * 4 : 0) + (staged ? part * 16 : 0);
-  if (!staged)
-    return tail ? launch_distill<DT, true, false, kVocThreads>(a, smem, st)
-                : launch_distill<DT, false, false, kVocThreads>(a, smem, st);
-#define IG_CALL(NT) (tail ? launch_distill<DT, true, true, NT>(a, smem, st) : launch_distill<DT, false, true, NT>(a, smem, st))
+  const size_t smem = tail ? ((nv / r.parts + 1) / 4 + 1) * 4 : 0;
+#define IG_CALL(NT) (tail ? launch_distill<DT, true, NT>(a, smem, st) : launch_distill<DT, false, NT>(a, smem, st))
   return IG_BY_THREADS(r.threads, IG_CALL);
 #undef IG_CALL
 }
