@@ -38,8 +38,18 @@ enum VEpi : int { kVStats = 0, kVDz = 1, kVOut = 2 };
 
 constexpr int kVBN = 256;   // tile columns
 constexpr int kVBK = 64;    // 16-bit elements of K per stage (128 bytes)
-constexpr int kVEpiWarps = 8;
-constexpr int kVGemmThreads = 64 + 32 * kVEpiWarps;
+// Epilogue warps: the plain stores keep up with eight; the exponentials need
+// sixteen (four per scheduler) to hide their latencies behind one another.
+// With eight, dZ of 8192 x 50021 x 768 took 544 us with the tensor pipe 59%
+// active, the statistics of 4096 x 262144 x 768 1202 us with 70%.
+template <int EPI>
+struct VEpiShape {
+  static constexpr int kWarps = EPI == kVOut ? 8 : 16;
+  static constexpr int kGroups = kWarps / 4;       // warps per TMEM lane quarter
+  static constexpr int kCols = kVBN / kGroups;     // tile columns of a warp
+  static constexpr int kThreads = 64 + 32 * kWarps;
+};
+constexpr int kVStatGroups = VEpiShape<kVStats>::kGroups;
 
 // Row coefficients of dZ (RowCoef with the output scale applied by the reader).
 struct VRowCoef {
@@ -58,7 +68,7 @@ struct VGemmArgs {
   int a_rows;  // rows of A's box (one CTA per tile: the rows there are, rounded up to 8; else 128)
   int n_fastest;                  // unit order: N parts innermost, else M tiles
   float c2;  // log2(e) / temperature
-  // kVStats: [M][units_n * 2] partials; group maxima [M][ldmax] or NULL
+  // kVStats: [M][units_n * kVStatGroups] partials; group maxima [M][ldmax] or NULL
   float4 *part;
   float *gmax;
   int64_t ldmax;
@@ -92,7 +102,7 @@ struct VSmem {
   static constexpr int kABytes = 128 * kVBK * 2;
   static constexpr int kBBytes = (kVBN / CG) * kVBK * 2;
   static constexpr int kStageBytes = kABytes + kBBytes;
-  static constexpr int kExtra = EPI == kVDz ? kVEpiWarps * 2 * 2048 : 0;  // two staging buffers per warp
+  static constexpr int kExtra = EPI == kVDz ? VEpiShape<EPI>::kWarps * 2 * 2048 : 0;  // two staging buffers per warp
   static constexpr int kRaw = (224 * 1024 - kExtra) / kStageBytes;
   static constexpr int kStages = kRaw > 6 ? 6 : kRaw;
   static constexpr int kExtraOff = kStages * kStageBytes;
@@ -190,7 +200,7 @@ __device__ __forceinline__ void store16(void *p, int64_t i, float v, int dtype) 
 }
 
 template <int CG, bool A_MN, bool B_MN, int EPI>
-__global__ void __launch_bounds__(kVGemmThreads, 1)
+__global__ void __launch_bounds__(VEpiShape<EPI>::kThreads, 1)
     vocab_gemm_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_constant__ CUtensorMap mapB,
                       const __grid_constant__ CUtensorMap mapC, const VGemmArgs a) {
   using S = VSmem<CG, EPI>;
@@ -218,7 +228,7 @@ __global__ void __launch_bounds__(kVGemmThreads, 1)
     }
     for (int b = 0; b < 2; b++) {
       mbar_init(&accf[b], 1);
-      mbar_init(&acce[b], CG * kVEpiWarps);
+      mbar_init(&acce[b], CG * VEpiShape<EPI>::kWarps);
     }
     fence_barrier_init();
   }
@@ -329,7 +339,9 @@ __global__ void __launch_bounds__(kVGemmThreads, 1)
       }
     }
   } else {
-    const int q4 = warp & 3, e = warp - 2, g = e >> 2;  // TMEM lane quarter; columns [128 g, 128 g + 128)
+    // TMEM lane quarter; columns [kCols g, kCols g + kCols).
+    constexpr int kCols = VEpiShape<EPI>::kCols;
+    const int q4 = warp & 3, e = warp - 2, g = e >> 2;
     int tile = 0;
     bool ok = true;
     [[maybe_unused]] int stores = 0;
@@ -372,19 +384,22 @@ __global__ void __launch_bounds__(kVGemmThreads, 1)
           continue;
         }
         const uint32_t tb = tmem + b * kVBN + ((uint32_t)(q4 * 32) << 16);
-        constexpr int kChunks = kVBN / 64;
-        uint32_t r[2][32];
+        constexpr int kChunks = kCols / 32;
+        // Two chunks in registers where a warp has few others beside it.
+        constexpr int kBufs = VEpiShape<EPI>::kWarps == 8 ? 2 : 1;
+        uint32_t r[kBufs][32];
         [[maybe_unused]] float gm[2 * kChunks];
-        tmem_ld_32x32b_x32(tb + g * 128, r[0]);
+        if constexpr (kBufs == 2) tmem_ld_32x32b_x32(tb + g * kCols, r[0]);
 #pragma unroll
         for (int i = 0; i < kChunks; i++) {
           __syncwarp();  // the branches below are per lane; the TMEM loads take the whole warp
+          if constexpr (kBufs == 1) tmem_ld_32x32b_x32(tb + g * kCols + 32 * i, r[0]);
           tmem_ld_wait();
-          if (i + 1 < kChunks)
-            tmem_ld_32x32b_x32(tb + g * 128 + 32 * (i + 1), r[(i + 1) & 1]);
-          else
+          if (i + 1 == kChunks)
             release();
-          const int col0 = n * kVBN + g * 128 + 32 * i;
+          else if constexpr (kBufs == 2)
+            tmem_ld_32x32b_x32(tb + g * kCols + 32 * (i + 1), r[(i + 1) & 1]);
+          const int col0 = n * kVBN + g * kCols + 32 * i;
           if constexpr (EPI != kVDz) {
             if (col0 >= a.N) {
               if constexpr (EPI == kVStats) gm[2 * i] = gm[2 * i + 1] = -IG_INF;
@@ -393,7 +408,7 @@ __global__ void __launch_bounds__(kVGemmThreads, 1)
           }
           float x[32];
 #pragma unroll
-          for (int k = 0; k < 32; k++) x[k] = __uint_as_float(r[i & 1][k]);
+          for (int k = 0; k < 32; k++) x[k] = __uint_as_float(r[i & (kBufs - 1)][k]);
           if constexpr (EPI == kVStats) {
             if (col0 + 32 > a.N) {
 #pragma unroll
@@ -486,14 +501,14 @@ __global__ void __launch_bounds__(kVGemmThreads, 1)
         }
         if constexpr (EPI == kVStats) {
           if (a.gmax && live) {
-            float4 *dst = reinterpret_cast<float4 *>(a.gmax + (int64_t)row * a.ldmax + n * (kVBN / kVGroup) + g * 8);
-            dst[0] = make_float4(gm[0], gm[1], gm[2], gm[3]);
-            dst[1] = make_float4(gm[4], gm[5], gm[6], gm[7]);
+            static_assert(kCols / kVGroup == 4, "one float4 of maxima");
+            *reinterpret_cast<float4 *>(a.gmax + (int64_t)row * a.ldmax + n * (kVBN / kVGroup) + g * 4) =
+                make_float4(gm[0], gm[1], gm[2], gm[3]);
           }
         }
       }
       if constexpr (EPI == kVStats) {
-        if (ok && live) a.part[(int64_t)row * (2 * a.units_n) + q.n * 2 + g] = make_float4(st.m, st.s, st.u, 0.0f);
+        if (ok && live) a.part[((int64_t)row * a.units_n + q.n) * kVStatGroups + g] = make_float4(st.m, st.s, st.u, 0.0f);
       }
     }
     if constexpr (EPI == kVDz) {
@@ -797,7 +812,7 @@ static int vgemm_slots() {
     at[0].val.clusterDim.y = 1;
     at[0].val.clusterDim.z = 1;
     cfg.gridDim = dim3(CG * (num_sms() / CG));
-    cfg.blockDim = dim3(kVGemmThreads);
+    cfg.blockDim = dim3(VEpiShape<EPI>::kThreads);
     cfg.dynamicSmemBytes = S::kTotal;
     cfg.attrs = at;
     cfg.numAttrs = 1;
@@ -819,7 +834,7 @@ static cudaError_t launch_vgemm(const CUtensorMap &ma, const CUtensorMap &mb, co
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute at[2];
   cfg.gridDim = dim3((unsigned)(CG * (units < slots ? units : slots)));
-  cfg.blockDim = dim3(kVGemmThreads);
+  cfg.blockDim = dim3(VEpiShape<EPI>::kThreads);
   cfg.dynamicSmemBytes = VSmem<CG, EPI>::kTotal;
   cfg.stream = st;
   if (CG > 1) {
@@ -856,7 +871,7 @@ static int best_parts(int64_t outer, int64_t tiles, int64_t slots, int64_t most,
   return (int)best;
 }
 
-constexpr int kVMaxParts = 256;        // column parts per M tile (two partials each)
+constexpr int kVMaxParts = 256;        // column parts per M tile
 constexpr int kVOneCtaRows = 128;      // at most this many rows: single CTAs
 constexpr int64_t kVDzBytes = 1ll << 30;  // dZ is formed in column chunks of at most this size
 
@@ -885,7 +900,7 @@ static VPlan vocab_plan(int64_t rows, int V, int H, int top_k) {
   p.units_m = (int)((rows + tm - 1) / tm);
   const int64_t tiles = ((int64_t)V + kVBN - 1) / kVBN;
   p.units_n = best_parts(p.units_m, tiles, slots, kVMaxParts, 0.25);
-  p.part_bytes = align_up((size_t)p.units_n * 2 * rows * sizeof(float4), 256);
+  p.part_bytes = align_up((size_t)p.units_n * kVStatGroups * rows * sizeof(float4), 256);
   p.ldmax = tiles * (kVBN / kVGroup);
   p.fwd_bytes = p.part_bytes + (top_k > 0 ? (size_t)rows * p.ldmax * 4 : 0);
   // With few rows, a given token's column or two carry most of the gradients,
@@ -946,7 +961,7 @@ static int run_vocab_logprobs(const VMatrices &x, const VPlan &p, const LogprobA
   j.H = p.H;
   j.T = o.T;
   j.K = o.K;
-  j.parts = 2 * p.units_n;
+  j.parts = kVStatGroups * p.units_n;
   j.dtype = x.dtype;
   j.c = o.c;
   j.ids = o.ids;
