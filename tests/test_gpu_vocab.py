@@ -86,6 +86,49 @@ def test_forward(voc, dtype, rows, V, pad, shift):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,V,pad", [(9600, 257, 0), (5000, 1023, 1), (2500, 2049, 0), (2400, 9001, 3)])
+def test_many_short_rows(voc, dtype, rows, V, pad):
+    """Enough rows for the CTAs of 32, 64 and 128 threads; more given tokens and teacher entries than threads."""
+    x = make(rows, V, dtype, 45 + V, pad)
+    g = torch.Generator(device="cuda").manual_seed(9)
+    T = 70
+    ids = torch.randint(-1, V, (rows, T), generator=g, device="cuda", dtype=torch.int32)
+    x[5] = 2.0  # all columns equal
+    r = voc.token_logprobs(x, ids, temperature=0.7, top_k=32)
+    lp, lse, ent, logp = ref_forward(x, ids, 0.7)
+    close(r.lse, lse, STAT_TOL, "lse")
+    close(r.logprobs, lp, STAT_TOL, "logprobs")
+    close(r.entropy, ent, STAT_TOL, "entropy")
+    i, _ = ref_top(x, 32)
+    assert torch.equal(r.top_ids.long(), i)
+    close(r.top_logprobs, logp.gather(1, i), STAT_TOL, "top")
+    del lp, logp
+    gl = torch.randn((rows, T), generator=g, device="cuda") / T
+    gh = torch.randn((rows,), generator=g, device="cuda")
+    d = voc.token_logprobs_backward(x, ids, r.lse, r.entropy, gl, gh, temperature=0.7)
+    want, p = ref_gradient(x, ids, gl, gh, 0.7)
+    size = gl.abs().sum(1, keepdim=True) + gh.abs()[:, None] * 40
+    tol = P_TOL * p * size + 2e-6 * gl.abs().sum(1, keepdim=True) / 0.7 * (want.abs() > p) + \
+        EPS[dtype] / 2 * want.abs() * 1.01 + TINY[dtype]
+    # Sums of up to T gradients in one column, in float32.
+    tol = tol + T * 2.0**-24 * gl.abs().amax(1, keepdim=True) / 0.7
+    assert ((d.double() - want).abs() <= tol).all()
+    for tail in (False, True):
+        tids, t = teacher(x, 100, tail, 7)
+        tids[3, 5] = -1
+        tids[4] = -1
+        loss, d = voc.distill_topk(x, tids, t, temperature=0.7, tail=tail)
+        wl, wd, p, q = ref_distill(x, tids, t, 0.7, tail, None)
+        close(loss, wl, 4 * STAT_TOL, "loss")
+        listed = torch.zeros_like(p, dtype=torch.bool).scatter_(1, tids.clamp(min=0).long(), tids >= 0)
+        mass = torch.where(listed, torch.zeros_like(p), p).sum(1).clamp(min=1e-300)
+        tol = (P_TOL * wd.abs() + 1e-6 * p / 0.7 + 4e-7) + EPS[dtype] / 2 * wd.abs() * 1.01 + TINY[dtype]
+        if tail:
+            tol = tol + (p * ((P_TOL * (1 - q.sum(1)).clamp(min=0) + 5e-7) / mass)[:, None]).clamp(max=1.0) / 0.7
+        assert ((d.double() - wd).abs() <= tol).all()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("V,rows", [(70, 2), (5000, 3), (70001, 1), (70001, 900)])
 def test_top_ties(voc, dtype, V, rows):
     """Few distinct values, constant rows: ties go to the lowest column."""
