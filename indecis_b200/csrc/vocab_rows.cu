@@ -202,6 +202,49 @@ struct RowPart {
 constexpr int kFirstThread = 0;
 constexpr int last_thread(int NT) { return NT > 32 ? 32 : 16; }
 
+// A thread's own vectors i NT of a part, read kAheadRounds rounds of
+// kVocUnroll ahead through slots in shared memory that no other thread
+// touches: asynchronous 16-byte copies need no registers while they are on
+// their way and, since each thread waits for its own, no barrier. Twelve
+// vectors a thread keep up to 192 KB per SM in flight (four in registers,
+// 64 KB: about 70% of the bandwidth).
+constexpr int kAheadRounds = 3;
+template <int NT, int ROUNDS = kAheadRounds>
+struct Ahead {
+  static constexpr int kRound = kVocUnroll * NT;
+  static constexpr int kBytes = ROUNDS * kRound * 16;
+  uint4 *slots;  // this thread's: [ROUNDS][kVocUnroll], NT apart
+  const uint4 *src;
+  int mine;  // vector i is there while i < mine (i in steps of NT)
+  __device__ __forceinline__ Ahead(void *smem, const uint4 *src_, int mine_)
+      : slots(static_cast<uint4 *>(smem) + threadIdx.x), src(src_), mine(mine_) {}
+  __device__ __forceinline__ void ask(int b, int stage) {
+#pragma unroll
+    for (int j = 0; j < kVocUnroll; j++)
+      if (b + j * NT < mine) cp_async16(slots + (stage * kVocUnroll + j) * NT, src + b + j * NT);
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  }
+  __device__ __forceinline__ void start() {
+#pragma unroll
+    for (int r = 0; r < ROUNDS; r++) ask(r * kRound, r);
+  }
+  // f(b, raw) for every round b of the thread's vectors, in order; raw[j] is
+  // there while b + j NT < mine.
+  template <typename F>
+  __device__ __forceinline__ void each(F f) {
+    int stage = 0;
+    for (int b = 0; b < mine; b += kRound) {
+      asm volatile("cp.async.wait_group %0;" ::"n"(ROUNDS - 1) : "memory");
+      uint4 raw[kVocUnroll];
+#pragma unroll
+      for (int j = 0; j < kVocUnroll; j++) raw[j] = slots[(stage * kVocUnroll + j) * NT];
+      ask(b + ROUNDS * kRound, stage);
+      stage = stage + 1 == ROUNDS ? 0 : stage + 1;
+      f(b, raw);
+    }
+  }
+};
+
 // ---- running statistics -----------------------------------------------------------
 
 struct VStat {
@@ -329,26 +372,31 @@ __device__ __forceinline__ bool top_before(float va, int ca, float vb, int cb) {
   return va > vb || (va == vb && ca < cb);
 }
 // The K first (value, column) of a CTA's part of a row, after the statistics'
-// pass has left each thread its own maximum. Up to 64 bins of one to four
-// neighbouring threads: the K-th largest of the bins' maxima is a lower bound of the K-th
-// largest value (K bins hold a value at least as large), and only bins that
-// reach it (K, or a few more with ties) are read again, from L2. What reaches
-// the bound is collected and ranked. With too many equal values for the
-// buffer (a row of few distinct values) the K are found one by one instead.
+// pass has left each thread its own maximum: the K-th largest of the threads'
+// maxima is a lower bound of the K-th largest value (K threads hold a value at
+// least as large), and only the vectors of threads that reach it (K, or a few
+// more) are read again, from L2. The bound is found bit by bit on the ordered
+// bits of the maxima, one counting barrier per bit. What reaches it is
+// collected and ranked. With too many equal values for the buffer (a row of
+// few distinct values) the K are found one by one instead.
 template <int NT>
 struct TopShared {
-  static constexpr int kBins = NT < 64 ? NT : 64;
-  static constexpr int kPer = NT / kBins;  // threads per bin
-  static constexpr int kCap = 2 * NT;      // candidates a CTA collects
-  float bin[kBins];
-  int kept[kBins];
+  static constexpr int kCap = NT < 128 ? 256 : 2 * NT;  // candidates a CTA collects
+  int kept[NT];
   float val[kCap];
   int col[kCap];
-  float tau;
   int nkept, n;
   float wv[NT / 32];
   int wc[NT / 32];
 };
+// Unsigned integers in the order of the floats (no NaN).
+__device__ __forceinline__ uint32_t order_key(float v) {
+  const uint32_t b = __float_as_uint(v);
+  return b & 0x80000000u ? ~b : b | 0x80000000u;
+}
+__device__ __forceinline__ float from_order_key(uint32_t k) {
+  return __uint_as_float(k & 0x80000000u ? k ^ 0x80000000u : ~k);
+}
 
 template <int DT, int NT>
 __device__ __noinline__ void top_one_by_one(const RowVecs<DT> rv, int v0, int v1, int K, TopShared<NT> &t, float *out_val,
@@ -425,34 +473,33 @@ template <int DT, int NT>
 __device__ __forceinline__ void top_select(const RowVecs<DT> &rv, const RowPart<DT> &rp, float tmax, int K, TopShared<NT> &t,
                                            float *out_val, int *out_col, int *out_n) {
   const int tid = (int)threadIdx.x;
-  constexpr int kBins = TopShared<NT>::kBins, kPer = TopShared<NT>::kPer;
-  float bm = tmax;
-#pragma unroll
-  for (int o = 1; o < kPer; o *= 2) bm = fmaxf(bm, __shfl_xor_sync(~0u, bm, o));
-  if (tid % kPer == 0) t.bin[tid / kPer] = bm;
   if (tid == 0) t.nkept = t.n = 0;
-  __syncthreads();
-  if (tid < kBins) {
-    const float b = t.bin[tid];
-    int r = 0;
-#pragma unroll 8
-    for (int j = 0; j < kBins; j++) r += top_before(t.bin[j], j, b, tid);
-    if (r == K - 1) t.tau = b;
+  const uint32_t key = order_key(tmax);
+  uint32_t bound = 0;
+  // Bits that tell widened values apart: sign, 8 of exponent and the type's mantissa.
+  constexpr int kBits = DT == IG_DT_BF16 ? 16 : DT == IG_DT_F16 ? 19 : 32;
+  for (int bit = 31; bit >= 32 - kBits; bit--) {
+    const uint32_t next = bound | (1u << bit);
+    const int n = __syncthreads_count(key >= next);
+    if (n >= K) {
+      bound = next;
+      if (n <= K + 2) break;
+    }
   }
-  __syncthreads();
-  const float tau = t.tau;
-  if (tid < kBins && t.bin[tid] >= tau && t.bin[tid] > -IG_INF) t.kept[atomicAdd(&t.nkept, 1)] = tid;
+  __syncthreads();  // nkept and n are set whatever the number of barriers above
+  const float tau = bound <= order_key(-IG_INF) ? -IG_INF : from_order_key(bound);
+  if (key >= bound && tmax > -IG_INF) t.kept[atomicAdd(&t.nkept, 1)] = tid;
   __syncthreads();
   const int rounds = (rp.n + NT - 1) / NT;
-  const int items = t.nkept * rounds * kPer;
+  const int items = t.nkept * rounds;
   constexpr int kAhead = 4;  // loads in flight per thread
   for (int it = tid; it < items; it += kAhead * NT) {
     uint4 raw[kAhead];
     int at[kAhead];
 #pragma unroll
     for (int j = 0; j < kAhead; j++) {
-      const int k = it + j * NT, r = k / kPer, b = r / rounds;
-      at[j] = k < items ? (r - b * rounds) * NT + t.kept[b] * kPer + k % kPer : rp.n;
+      const int k = it + j * NT, b = k / rounds;
+      at[j] = k < items ? (k - b * rounds) * NT + t.kept[b] : rp.n;
       if (at[j] < rp.n) raw[j] = rp.base[at[j]];
     }
 #pragma unroll
@@ -553,6 +600,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT) token_logprobs_kernel(const Log
   using T = typename E::T;
   __shared__ VStat s_warp[NT / 32];
   __shared__ VStat s_part[8];  // on rank 0, the cluster's statistics
+  extern __shared__ uint4 s_ahead[];
   constexpr int kLists = NT == kVocThreads ? 8 : 1;  // smaller CTAs have their row alone
   __shared__ TopShared<NT> s_top[1];
   __shared__ float s_oval[TOP ? kLists * kTopMax : 1];  // this CTA's list, and on rank 0 all the cluster's
@@ -568,6 +616,8 @@ __global__ void __launch_bounds__(NT, 1024 / NT) token_logprobs_kernel(const Log
   const RowPart<DT> rp(rv, rank, cs);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const float c2 = a.c * kLog2e;
+  Ahead<NT> ahead(s_ahead, rp.base + threadIdx.x, rp.n - (int)threadIdx.x);
+  ahead.start();
   if (cs > 1) {
     if (threadIdx.x == 0) {
       mbar_init(&s_bar, 1);
@@ -587,28 +637,18 @@ __global__ void __launch_bounds__(NT, 1024 / NT) token_logprobs_kernel(const Log
   }
 
   VStat st{-IG_INF, 0.0f, 0.0f};
-  constexpr int kRound = kVocUnroll * NT;
-  const uint4 *p = rp.base + threadIdx.x;
-  int i = 0;
-  if (rp.n >= kRound) {
-    // Each round's vectors are asked for before the one before it is added.
-    uint4 raw[kVocUnroll];
+  ahead.each([&](int b, const uint4(&raw)[kVocUnroll]) {
+    if (b + (kVocUnroll - 1) * NT < ahead.mine) {
+      vstat_add_raw<DT, true>(st, raw, c2);
+    } else {
 #pragma unroll
-    for (int j = 0; j < kVocUnroll; j++) raw[j] = p[j * NT];
-    for (i = kRound; i + kRound <= rp.n; i += kRound) {
-      uint4 cur[kVocUnroll];
-#pragma unroll
-      for (int j = 0; j < kVocUnroll; j++) cur[j] = raw[j];
-#pragma unroll
-      for (int j = 0; j < kVocUnroll; j++) raw[j] = p[i + j * NT];
-      vstat_add_raw<DT, true>(st, cur, c2);
+      for (int j = 0; j < kVocUnroll; j++)
+        if (b + j * NT < ahead.mine) {
+          const uint4 one[1] = {raw[j]};
+          vstat_add_raw<DT, true>(st, one, c2);
+        }
     }
-    vstat_add_raw<DT, true>(st, raw, c2);
-  }
-  for (i += threadIdx.x; i < rp.n; i += NT) {
-    const uint4 raw[1] = {rp.base[i]};
-    vstat_add_raw<DT, true>(st, raw, c2);
-  }
+  });
   if (threadIdx.x == kFirstThread && rp.first) {
     const uint4 raw[1] = {rv.edge(rp.v0)};
     vstat_add_raw<DT, true>(st, raw, c2);
@@ -788,17 +828,10 @@ __global__ void __launch_bounds__(NT, 1024 / NT) token_logprobs_grad_kernel(cons
   const RowPart<DT> rp(rv, seg, a.segs);
   const int32_t *ids = a.ids + row * a.T;
   const float *g = a.dlogprobs + row * a.T;
-  // Rounds of vectors, each asked for before the one before it is worked on,
-  // the first before the row's scalars.
-  const uint4 *p = rp.base + threadIdx.x;
-  const int mine = rp.n - (int)threadIdx.x;  // the thread's vector i NT is there while i NT < mine
-  uint4 raw[kVocUnroll], edge;
-  auto load = [&](int b) {
-#pragma unroll
-    for (int j = 0; j < kVocUnroll; j++)
-      if (b + j * NT < mine) raw[j] = p[b + j * NT];
-  };
-  load(0);
+  extern __shared__ uint4 s_ahead[];
+  Ahead<NT> ahead(s_ahead, rp.base + threadIdx.x, rp.n - (int)threadIdx.x);
+  ahead.start();  // before the row's scalars
+  uint4 edge;
   if (threadIdx.x == kFirstThread && rp.first) edge = rv.edge(rp.v0);
   if (threadIdx.x == last_thread(NT) && rp.last) edge = rv.edge(rp.v1 - 1);
   const float lse = a.lse[row];
@@ -831,20 +864,15 @@ __global__ void __launch_bounds__(NT, 1024 / NT) token_logprobs_grad_kernel(cons
     }
   };
   T *dp = drow + rv.col(rp.w0) + (int64_t)threadIdx.x * kN;
-  constexpr int kRound = kVocUnroll * NT;
-  for (int b = 0; b < mine; b += kRound) {
-    uint4 cur[kVocUnroll];
-#pragma unroll
-    for (int j = 0; j < kVocUnroll; j++) cur[j] = raw[j];
-    load(b + kRound);
+  ahead.each([&](int b, const uint4(&raw)[kVocUnroll]) {
 #pragma unroll
     for (int j = 0; j < kVocUnroll; j++) {
-      if (b + j * NT >= mine) break;
+      if (b + j * NT >= ahead.mine) break;
       float d[kN];
-      grad(cur[j], d);
+      grad(raw[j], d);
       store_whole<DT>(dp + (int64_t)(b + j * NT) * kN, same, d);
     }
-  }
+  });
   if ((threadIdx.x == kFirstThread && rp.first) || (threadIdx.x == last_thread(NT) && rp.last)) {
     float d[kN];
     grad(edge, d);
@@ -888,7 +916,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT) distill_topk_kernel(const Disti
   using E = VElem<DT>;
   using T = typename E::T;
   constexpr int kN = E::kN;
-  extern __shared__ uint32_t s_dyn[];
+  extern __shared__ uint4 s_dyn[];
   __shared__ VStat s_warp[NT / 32];
   __shared__ VStat s_part[8];  // every CTA's statistics
   __shared__ VStat s_list;     // with TAIL: the listed columns'
@@ -902,7 +930,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT) distill_topk_kernel(const Disti
   const RowPart<DT> rp(rv, rank, cs);
   const int tid = (int)threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const float c2 = a.c * kLog2e;
-  uint8_t *s_mask = reinterpret_cast<uint8_t *>(s_dyn);  // of vector v0 + i
+  uint8_t *s_mask = reinterpret_cast<uint8_t *>(s_dyn) + Ahead<NT, 2>::kBytes;  // of vector v0 + i
   if (tid == 0 && cs > 1) {
     mbar_init(&s_bar, 1);
     fence_barrier_init();
@@ -910,9 +938,8 @@ __global__ void __launch_bounds__(NT, 1024 / NT) distill_topk_kernel(const Disti
   }
   __syncwarp();
   if (cs > 1) cluster_announce();
-  const uint4 *src = rp.base + tid;
-  const int mine = rp.n - tid;  // the thread's vector i NT is there while i NT < mine
-  constexpr int kRound = kVocUnroll * NT;
+  Ahead<NT, 2> ahead(s_dyn, rp.base + tid, rp.n - tid);
+  ahead.start();
   uint4 edge;
   const bool has_edge = (tid == kFirstThread && rp.first) || (tid == last_thread(NT) && rp.last);
   const int edge_v = tid == kFirstThread ? rp.v0 : rp.v1 - 1;
@@ -984,32 +1011,27 @@ __global__ void __launch_bounds__(NT, 1024 / NT) distill_topk_kernel(const Disti
       }
       return raw;
     };
-    int i = 0;
-    if (rp.n >= kRound) {
-      // Each round's vectors are asked for before the one before it is added.
-      uint4 raw[kVocUnroll];
-#pragma unroll
-      for (int j = 0; j < kVocUnroll; j++) raw[j] = src[j * NT];
-      for (i = kRound; i <= rp.n; i += kRound) {
+    ahead.each([&](int b, const uint4(&raw)[kVocUnroll]) {
+      const int v = rp.w0 + b + tid;
+      if (b + (kVocUnroll - 1) * NT < ahead.mine) {
         uint4 cur[kVocUnroll];
 #pragma unroll
-        for (int j = 0; j < kVocUnroll; j++) cur[j] = unlisted(raw[j], rp.w0 + i - kRound + j * NT + tid);
-        if (i + kRound <= rp.n) {
-#pragma unroll
-          for (int j = 0; j < kVocUnroll; j++) raw[j] = src[i + j * NT];
-        }
+        for (int j = 0; j < kVocUnroll; j++) cur[j] = unlisted(raw[j], v + j * NT);
         vstat_add_raw<DT, false>(st, cur, c2);
+      } else {
+#pragma unroll
+        for (int j = 0; j < kVocUnroll; j++)
+          if (b + j * NT < ahead.mine) {
+            const uint4 one[1] = {unlisted(raw[j], v + j * NT)};
+            vstat_add_raw<DT, false>(st, one, c2);
+          }
       }
-      i -= kRound;
-    }
-    for (; i < mine; i += NT) {
-      const uint4 raw[1] = {unlisted(src[i], rp.w0 + i + tid)};
-      vstat_add_raw<DT, false>(st, raw, c2);
-    }
+    });
     if (has_edge) {
       const uint4 raw[1] = {unlisted(edge, edge_v)};
       vstat_add_raw<DT, false>(st, raw, c2);
     }
+    if (drow) ahead.start();  // the second pass's first vectors
     st = vstat_warp<false>(st, c2);
     if (lane == 0) s_warp[warp] = st;
     if (warp == 0) {
@@ -1128,7 +1150,10 @@ __global__ void __launch_bounds__(NT, 1024 / NT) distill_topk_kernel(const Disti
   } else if (rank == 0 && tid == 0) {
     a.loss[row] = 0.0f;
   }
-  if (!drow) return;
+  if (!drow) {
+    cp_async_wait_all();
+    return;
+  }
   if (cs == 1) __syncthreads();  // the list's logits are read before any store: dx may be x
   const float2 nm = make_float2(-mb, -mb), cc = make_float2(c2, c2), nl = make_float2(-l2, -l2);
   auto grad = [&](const uint4 &v, float *d) {
@@ -1144,30 +1169,20 @@ __global__ void __launch_bounds__(NT, 1024 / NT) distill_topk_kernel(const Disti
   };
   T *dp = drow + rv.col(rp.w0) + (int64_t)tid * kN;
   if (zero) {
+    cp_async_wait_all();
     float d[kN] = {};
-    for (int i = 0; i < mine; i += NT) store_whole<DT>(dp + (int64_t)i * kN, same, d);
+    for (int i = 0; i < ahead.mine; i += NT) store_whole<DT>(dp + (int64_t)i * kN, same, d);
     if (has_edge) store_edge<DT>(drow, rv, edge_v, d);
   } else {
-    uint4 raw[kVocUnroll];
-    auto load = [&](int b) {
-#pragma unroll
-      for (int j = 0; j < kVocUnroll; j++)
-        if (b + j * NT < mine) raw[j] = src[b + j * NT];
-    };
-    load(0);
-    for (int b = 0; b < mine; b += kRound) {
-      uint4 cur[kVocUnroll];
-#pragma unroll
-      for (int j = 0; j < kVocUnroll; j++) cur[j] = raw[j];
-      load(b + kRound);
+    ahead.each([&](int b, const uint4(&raw)[kVocUnroll]) {
 #pragma unroll
       for (int j = 0; j < kVocUnroll; j++) {
-        if (b + j * NT >= mine) break;
+        if (b + j * NT >= ahead.mine) break;
         float d[kN];
-        grad(cur[j], d);
+        grad(raw[j], d);
         store_whole<DT>(dp + (int64_t)(b + j * NT) * kN, same, d);
       }
-    }
+    });
     if (has_edge) {
       float d[kN];
       grad(edge, d);
@@ -1209,19 +1224,21 @@ static RowShape row_shape(int64_t rows, int64_t nv) {
 
 template <typename Args>
 static cudaError_t launch_rows(void (*kern)(Args), const Args &a, int64_t ctas, int threads, int cs, size_t smem,
-                               cudaStream_t st) {
+                               cudaStream_t st, SmemOptIn &attr) {
+  const cudaError_t e = attr.ensure((const void *)kern, (int)smem);
+  if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)ctas);
   cfg.blockDim = dim3(threads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
-  cudaLaunchAttribute attr[1];
+  cudaLaunchAttribute at[1];
   if (cs > 1) {
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = cs;
-    attr[0].val.clusterDim.y = 1;
-    attr[0].val.clusterDim.z = 1;
-    cfg.attrs = attr;
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = cs;
+    at[0].val.clusterDim.y = 1;
+    at[0].val.clusterDim.z = 1;
+    cfg.attrs = at;
     cfg.numAttrs = 1;
   }
   return cudaLaunchKernelEx(&cfg, kern, a);
@@ -1230,16 +1247,26 @@ static cudaError_t launch_rows(void (*kern)(Args), const Args &a, int64_t ctas, 
 #define IG_BY_THREADS(n, CALL) \
   ((n) == 256 ? CALL(256) : (n) == 128 ? CALL(128) : (n) == 64 ? CALL(64) : CALL(32))
 
+template <int DT, bool TOP, int NT>
+static cudaError_t launch_logprobs(const LogprobArgs &a, int64_t ctas, cudaStream_t st) {
+  static SmemOptIn attr;
+  return launch_rows(token_logprobs_kernel<DT, TOP, NT>, a, ctas, NT, a.parts, Ahead<NT>::kBytes, st, attr);
+}
+
 template <int DT>
 static cudaError_t run_token_logprobs(LogprobArgs a, cudaStream_t st) {
   const RowShape r = row_shape(a.rows, a.V / VElem<DT>::kN);
   a.parts = r.parts;
   const int64_t ctas = a.rows * r.parts;
-#define IG_CALL(NT)                                                                                   \
-  (a.K > 0 ? launch_rows(token_logprobs_kernel<DT, true, NT>, a, ctas, NT, r.parts, 0, st)            \
-           : launch_rows(token_logprobs_kernel<DT, false, NT>, a, ctas, NT, r.parts, 0, st))
+#define IG_CALL(NT) (a.K > 0 ? launch_logprobs<DT, true, NT>(a, ctas, st) : launch_logprobs<DT, false, NT>(a, ctas, st))
   return IG_BY_THREADS(r.threads, IG_CALL);
 #undef IG_CALL
+}
+
+template <int DT, int NT>
+static cudaError_t launch_grad(const LogprobGradArgs &a, int64_t ctas, cudaStream_t st) {
+  static SmemOptIn attr;
+  return launch_rows(token_logprobs_grad_kernel<DT, NT>, a, ctas, NT, 1, Ahead<NT>::kBytes, st, attr);
 }
 
 template <int DT>
@@ -1254,7 +1281,7 @@ static cudaError_t run_token_logprobs_grad(LogprobGradArgs a, cudaStream_t st) {
   a.segs = (int)((rounds + per - 1) / per);
   const int64_t ctas = a.rows * a.segs;
   if (ctas > INT32_MAX) return cudaErrorInvalidConfiguration;
-#define IG_CALL(NT) launch_rows(token_logprobs_grad_kernel<DT, NT>, a, ctas, NT, 1, 0, st)
+#define IG_CALL(NT) launch_grad<DT, NT>(a, ctas, st)
   return IG_BY_THREADS(nt, IG_CALL);
 #undef IG_CALL
 }
@@ -1262,9 +1289,8 @@ static cudaError_t run_token_logprobs_grad(LogprobGradArgs a, cudaStream_t st) {
 template <int DT, bool TAIL, int NT>
 static cudaError_t launch_distill(const DistillArgs &a, size_t smem, cudaStream_t st) {
   static SmemOptIn attr;
-  const cudaError_t e = attr.ensure((const void *)distill_topk_kernel<DT, TAIL, NT>, (int)smem);
-  if (e != cudaSuccess) return e;
-  return launch_rows(distill_topk_kernel<DT, TAIL, NT>, a, a.rows * a.parts, NT, a.parts, smem, st);
+  return launch_rows(distill_topk_kernel<DT, TAIL, NT>, a, a.rows * a.parts, NT, a.parts, Ahead<NT, 2>::kBytes + smem, st,
+                     attr);
 }
 
 template <int DT>
