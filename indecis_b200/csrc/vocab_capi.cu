@@ -108,7 +108,7 @@ int ig_distill_topk(const void *logits, int32_t dtype, int64_t ld, int64_t rows,
   if (!m) m = bad_matrix(logits, rows, vocab, ld, es);
   if (!m && dlogits) m = bad_matrix(dlogits, rows, vocab, ldd, es);
   if (!m && rows > 0 && !loss) m = "null argument";
-  if (!m && logits == dlogits && ld != ldd) m = "in place, both row strides must be the same";
+  if (!m && dlogits && logits == dlogits && ld != ldd) m = "in place, both row strides must be the same";
   if (m) return fail(IG_ERR_BAD_ARG, std::string("ig_distill_topk: ") + m);
   if (tail && vocab > (1 << 20))
     return fail(IG_ERR_UNSUPPORTED, "ig_distill_topk: with the tail, at most 1048576 columns");

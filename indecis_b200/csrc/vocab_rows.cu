@@ -1209,7 +1209,11 @@ __global__ void __launch_bounds__(NT, 1024 / NT) distill_topk_kernel(const Disti
 struct RowShape {
   int threads, parts;
 };
-static RowShape row_shape(int64_t rows, int64_t nv) {
+// again: the row's vectors are read a second time, so the rows on the way have
+// to stay near L2 (126 MB): 1024 x 262144 float32 with 20 alternatives takes
+// 282 us with 310 MB of rows on the way, 227 with 78; 4096 x 50021 float32
+// 188 with 118 MB and 223 with 59, where the clusters only cost.
+static RowShape row_shape(int64_t rows, int64_t nv, bool again) {
   RowShape r{kVocThreads, 1};
   // Many short rows: small CTAs, so that an SM has more rows on the way (a
   // row's start and end cost as much as 16 vectors per thread), while the
@@ -1218,6 +1222,8 @@ static RowShape row_shape(int64_t rows, int64_t nv) {
   // Few rows: several CTAs each, of a round of vectors at least.
   while (r.threads == kVocThreads && r.parts < 8 && rows * r.parts < 2 * 4 * num_sms() &&
          nv / (2 * r.parts) >= kVocThreads)
+    r.parts *= 2;
+  while (again && r.threads == kVocThreads && r.parts < 8 && nv * 16 * (4 * num_sms() / r.parts) > (140ll << 20))
     r.parts *= 2;
   return r;
 }
@@ -1255,7 +1261,7 @@ static cudaError_t launch_logprobs(const LogprobArgs &a, int64_t ctas, cudaStrea
 
 template <int DT>
 static cudaError_t run_token_logprobs(LogprobArgs a, cudaStream_t st) {
-  const RowShape r = row_shape(a.rows, a.V / VElem<DT>::kN);
+  const RowShape r = row_shape(a.rows, a.V / VElem<DT>::kN, a.K > 0);
   a.parts = r.parts;
   const int64_t ctas = a.rows * r.parts;
 #define IG_CALL(NT) (a.K > 0 ? launch_logprobs<DT, true, NT>(a, ctas, st) : launch_logprobs<DT, false, NT>(a, ctas, st))
@@ -1272,7 +1278,7 @@ static cudaError_t launch_grad(const LogprobGradArgs &a, int64_t ctas, cudaStrea
 template <int DT>
 static cudaError_t run_token_logprobs_grad(LogprobGradArgs a, cudaStream_t st) {
   const int64_t nv = (a.V + VElem<DT>::kN - 1) / VElem<DT>::kN + 1;  // a row off the boundary spans one more
-  const int nt = row_shape(a.rows, a.V / VElem<DT>::kN).threads;
+  const int nt = row_shape(a.rows, a.V / VElem<DT>::kN, false).threads;
   const int64_t rounds = (nv + kVocUnroll * nt - 1) / (kVocUnroll * nt);
   // Several rounds per CTA (a CTA's start costs about as much as a round)
   // while there are CTAs enough to fill the GPU four times.
@@ -1296,9 +1302,7 @@ static cudaError_t launch_distill(const DistillArgs &a, size_t smem, cudaStream_
 template <int DT>
 static cudaError_t run_distill(DistillArgs a, bool tail, cudaStream_t st) {
   const int64_t nv = a.V / VElem<DT>::kN + 2;
-  RowShape r = row_shape(a.rows, a.V / VElem<DT>::kN);
-  // The rows on the way between their two passes have to stay in L2.
-  while (a.dx && r.threads == kVocThreads && r.parts < 8 && nv * 16 * (4 * num_sms() / r.parts) > (100ll << 20)) r.parts *= 2;
+  const RowShape r = row_shape(a.rows, a.V / VElem<DT>::kN, a.dx != nullptr);
   a.parts = r.parts;
   const size_t smem = tail ? ((nv / r.parts + 1) / 4 + 1) * 4 : 0;
 #define IG_CALL(NT) (tail ? launch_distill<DT, true, NT>(a, smem, st) : launch_distill<DT, false, NT>(a, smem, st))
