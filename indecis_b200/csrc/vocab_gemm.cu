@@ -699,6 +699,7 @@ struct VCoefArgs {
 
 // One warp per row.
 __global__ void vocab_coef_kernel(const VCoefArgs a) {
+  dep_trigger();  // dZ's CTAs set themselves up meanwhile
   const int64_t row = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) >> 5;
   if (row >= a.rows) return;
   const int lane = threadIdx.x & 31;
@@ -738,6 +739,7 @@ struct VTokenArgs {
 // log probability plus the tokens' own gradients, rounded once.
 __global__ void vocab_token_kernel(const VTokenArgs a) {
   dep_wait();
+  dep_trigger();
   const int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
   if (i >= a.n) return;
   const int64_t row = i / a.T;
@@ -754,27 +756,44 @@ __global__ void vocab_token_kernel(const VTokenArgs a) {
   if (a.shift) store16(a.dz, at + a.shift, d - widen1((uint16_t)w, a.dtype), a.dtype);
 }
 
-// dhidden = sum over the K parts, in order, scaled back and rounded. One CTA
-// per row, four columns per thread.
-__global__ void __launch_bounds__(256) vocab_sum_kernel(const float *part, int parts, int64_t rows, int H, int64_t ldp,
-                                                        const int *bound, void *out, int64_t ldo, int dtype) {
+// dhidden = sum over the K parts, scaled back and rounded. One CTA per row,
+// four columns per thread; with many parts four groups of threads
+// (threadIdx.y) take every fourth part, and their sums are added in order (37
+// parts of 500 x 256: 11.2 us by one group, 7.9 by four; 3 parts of 8192 x
+// 768: 20 and 90).
+__global__ void __launch_bounds__(1024) vocab_sum_kernel(const float *part, int parts, int64_t rows, int H, int64_t ldp,
+                                                         const int *bound, void *out, int64_t ldo, int dtype) {
+  extern __shared__ float4 s_sum[];
   dep_wait();
+  dep_trigger();
   const int64_t row = blockIdx.x;
   const float unscale = 1.0f / vocab_scale(bound);
-  for (int col = 4 * threadIdx.x; col < H; col += 4 * blockDim.x) {
+  for (int c0 = 0; c0 < H; c0 += 4 * blockDim.x) {
+    const int col = c0 + 4 * threadIdx.x;
     float4 s = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    if (col < H) {
 #pragma unroll 8
-    for (int p = 0; p < parts; p++) {
-      const float4 v = *reinterpret_cast<const float4 *>(part + ((int64_t)p * rows + row) * ldp + col);
-      s = make_float4(s.x + v.x, s.y + v.y, s.z + v.z, s.w + v.w);
+      for (int p = threadIdx.y; p < parts; p += blockDim.y) {
+        const float4 v = *reinterpret_cast<const float4 *>(part + ((int64_t)p * rows + row) * ldp + col);
+        s = make_float4(s.x + v.x, s.y + v.y, s.z + v.z, s.w + v.w);
+      }
     }
-    const float v[4] = {s.x * unscale, s.y * unscale, s.z * unscale, s.w * unscale};
-    uint16_t *dst = static_cast<uint16_t *>(out) + row * ldo + col;
-    if (col + 4 <= H && (reinterpret_cast<uintptr_t>(dst) & 7) == 0) {
-      *reinterpret_cast<uint2 *>(dst) = make_uint2(pack16(v[0], v[1], dtype), pack16(v[2], v[3], dtype));
-    } else {
-      for (int k = 0; k < 4 && col + k < H; k++) store16(dst, k, v[k], dtype);
+    s_sum[threadIdx.y * blockDim.x + threadIdx.x] = s;
+    __syncthreads();
+    if (threadIdx.y == 0 && col < H) {
+      for (int g = 1; g < (int)blockDim.y; g++) {
+        const float4 v = s_sum[g * blockDim.x + threadIdx.x];
+        s = make_float4(s.x + v.x, s.y + v.y, s.z + v.z, s.w + v.w);
+      }
+      const float v[4] = {s.x * unscale, s.y * unscale, s.z * unscale, s.w * unscale};
+      uint16_t *dst = static_cast<uint16_t *>(out) + row * ldo + col;
+      if (col + 4 <= H && (reinterpret_cast<uintptr_t>(dst) & 7) == 0) {
+        *reinterpret_cast<uint2 *>(dst) = make_uint2(pack16(v[0], v[1], dtype), pack16(v[2], v[3], dtype));
+      } else {
+        for (int k = 0; k < 4 && col + k < H; k++) store16(dst, k, v[k], dtype);
+      }
     }
+    __syncthreads();
   }
 }
 
@@ -1057,8 +1076,9 @@ static int run_vocab_grad(const VMatrices &x, const VPlan &p, const LogprobGradA
                       : (launch_vgemm<2, false, true, kVOut>(mz, mw, mw, b, st)));
       if (!b.out16 && last) {
         const int threads = p.H >= 1024 ? 256 : (p.H + 127) / 128 * 32;
-        IG_CU(launch_dep(vocab_sum_kernel, dim3((unsigned)p.rows), dim3(threads), 0, st, (const float *)p32, parts, p.rows,
-                         p.H, p.ldp, (const int *)bound, o.dh, o.lddh, x.dtype));
+        const int groups = parts >= 16 ? 4 : 1;
+        IG_CU(launch_dep(vocab_sum_kernel, dim3((unsigned)p.rows), dim3(threads, groups), threads * groups * 16, st,
+                         (const float *)p32, parts, p.rows, p.H, p.ldp, (const int *)bound, o.dh, o.lddh, x.dtype));
       }
     }
     if (o.dw) {

@@ -165,6 +165,18 @@ def test_backward(voc, dtype, rows, V, H):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,V,H,T", [(40, 300, 64, 200), (300, 5003, 72, 17), (300, 5003, 72, 16), (130, 50, 64, 16)])
+def test_many_given_tokens(voc, dtype, rows, V, H, T):
+    """Many given tokens in a row, most of the columns given."""
+    h, w = make(rows, V, H, dtype, 15)
+    gen = torch.Generator(device="cuda").manual_seed(6)
+    ids = torch.randint(-1, V, (rows, T), generator=gen, device="cuda", dtype=torch.int32)
+    g = torch.randn((rows, T), generator=gen, device="cuda")
+    gh = torch.randn((rows,), generator=gen, device="cuda")
+    check_backward(voc, h, w, ids, g, gh, 0.8)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("rows,V,H", [(1, 5000, 256), (7, 33001, 72), (128, 1000, 136)])
 def test_few_rows_keep_more_bits(voc, dtype, rows, V, H):
     """At most 128 rows: dZ in two 16-bit parts, so the gradients are off by their own rounding and little else (the
