@@ -69,7 +69,7 @@ constexpr int kVGroup = 16;  // columns per stored maximum
 struct VGemmArgs {
   int M, N;
   int kblocks;  // blocks of kVBK of K
-  int kwrap;    // blocks from this one on read A's second part, `shift` elements further along its rows, and B from the start
+  int kparts;   // 2: blocks come in pairs, one of either part of A (`shift` elements apart along its rows) with one of B
   int shift;
   uint32_t idesc;
   int units_m, units_n, units_s;  // units: M tiles x N parts x K parts
@@ -110,7 +110,8 @@ struct VSmem {
   static constexpr int kABytes = 128 * kVBK * 2;
   static constexpr int kBBytes = (kVBN / CG) * kVBK * 2;
   static constexpr int kStageBytes = kABytes + kBBytes;
-  static constexpr int kExtra = EPI == kVDz ? VEpiShape<EPI>::kWarps * 2 * 2048 : 0;  // two staging buffers per warp
+  // Staging per warp: two buffers for dZ's bulk stores, one to turn rows for the plain 16-bit stores.
+  static constexpr int kExtra = EPI == kVDz ? VEpiShape<EPI>::kWarps * 2 * 2048 : EPI == kVOut ? VEpiShape<EPI>::kWarps * 2048 : 0;
   static constexpr int kRaw = (224 * 1024 - kExtra) / kStageBytes;
   static constexpr int kStages = kRaw > 6 ? 6 : kRaw;
   static constexpr int kExtraOff = kStages * kStageBytes;
@@ -278,8 +279,7 @@ __global__ void __launch_bounds__(VEpiShape<EPI>::kThreads, 1)
               else
                 tma_load_2d(map, dst, &full[s], c0, c1);
             };
-            const bool second = kb >= a.kwrap;
-            const int kc = (second ? kb - a.kwrap : kb) * kVBK, as = second ? a.shift : 0;
+            const int kc = (a.kparts == 2 ? kb >> 1 : kb) * kVBK, as = a.kparts == 2 && (kb & 1) ? a.shift : 0;
             if constexpr (A_MN) {
 #pragma unroll
               for (int i = 0; i < 2; i++) load(&mapA, sa + i * 8192, as + m0 + i * 64, kc);
@@ -475,21 +475,35 @@ __global__ void __launch_bounds__(VEpiShape<EPI>::kThreads, 1)
               stores++;
             }
           } else {
-            if (live && a.out16) {
+            if (a.out16) {
+              // A thread holds a row's 32 columns; through shared memory four
+              // lanes store a row's 64 bytes, whole sectors (a thread storing
+              // its own row 16 bytes at a time took 222 us for the 402 MB of
+              // one row's dweight, 262144 x 768).
+              uint8_t *buf = smem + S::kExtraOff + e * 2048;
+              __syncwarp();
 #pragma unroll
-              for (int k = 0; k < 32; k++) x[k] *= unscale;
-              const int64_t at = (int64_t)row * a.ldo + col0;
-              uint8_t *dst = static_cast<uint8_t *>(a.out16) + at * 2;
-              if (col0 + 32 <= a.N && (reinterpret_cast<uintptr_t>(dst) & 15) == 0) {
+              for (int j = 0; j < 4; j++)
+                *reinterpret_cast<uint4 *>(buf + lane * 64 + ((j ^ ((lane >> 1) & 3)) << 4)) =
+                    make_uint4(pack16(x[8 * j] * unscale, x[8 * j + 1] * unscale, a.dtype),
+                               pack16(x[8 * j + 2] * unscale, x[8 * j + 3] * unscale, a.dtype),
+                               pack16(x[8 * j + 4] * unscale, x[8 * j + 5] * unscale, a.dtype),
+                               pack16(x[8 * j + 6] * unscale, x[8 * j + 7] * unscale, a.dtype));
+              __syncwarp();
 #pragma unroll
-                for (int j = 0; j < 4; j++)
-                  reinterpret_cast<uint4 *>(dst)[j] =
-                      make_uint4(pack16(x[8 * j], x[8 * j + 1], a.dtype), pack16(x[8 * j + 2], x[8 * j + 3], a.dtype),
-                                 pack16(x[8 * j + 4], x[8 * j + 5], a.dtype), pack16(x[8 * j + 6], x[8 * j + 7], a.dtype));
-              } else {
+              for (int i8 = 0; i8 < 4; i8++) {
+                const int r8 = i8 * 8 + (lane >> 2), j = lane & 3, col = col0 + 8 * j;
+                if (row0 + r8 >= a.M || col >= a.N) continue;
+                const uint4 v = *reinterpret_cast<const uint4 *>(buf + r8 * 64 + ((j ^ ((r8 >> 1) & 3)) << 4));
+                uint16_t *dst = static_cast<uint16_t *>(a.out16) + (int64_t)(row0 + r8) * a.ldo + col;
+                if (col + 8 <= a.N && (reinterpret_cast<uintptr_t>(dst) & 15) == 0) {
+                  *reinterpret_cast<uint4 *>(dst) = v;
+                } else {
+                  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-                for (int k = 0; k < 32; k++)
-                  if (col0 + k < a.N) store16(a.out16, at + k, x[k], a.dtype);
+                  for (int k = 0; k < 8; k++)
+                    if (col + k < a.N) dst[k] = (uint16_t)(w[k >> 1] >> (16 * (k & 1)));
+                }
               }
             } else if (live) {
               // part32 rows are padded to a multiple of 4 floats.
@@ -968,7 +982,8 @@ static int run_vocab_logprobs(const VMatrices &x, const VPlan &p, const LogprobA
   a.M = (int)p.rows;
   a.N = p.V;
   a.a_rows = p.a_rows;
-  a.kblocks = a.kwrap = (p.H + kVBK - 1) / kVBK;
+  a.kblocks = (p.H + kVBK - 1) / kVBK;
+  a.kparts = 1;
   a.idesc = idesc_f16(128 * p.cg, kVBN, x.dtype, false, false);
   a.units_m = p.units_m;
   a.units_n = p.units_n;
@@ -1037,7 +1052,8 @@ static int run_vocab_grad(const VMatrices &x, const VPlan &p, const LogprobGradA
     a.M = (int)p.rows;
     a.N = (int)vc;
     a.a_rows = p.a_rows;
-    a.kblocks = a.kwrap = (p.H + kVBK - 1) / kVBK;
+    a.kblocks = (p.H + kVBK - 1) / kVBK;
+  a.kparts = 1;
     a.idesc = idesc_f16(tm, kVBN, x.dtype, false, false);
     a.units_m = p.units_m;
     a.units_n = (int)((vc + kVBN - 1) / kVBN);
@@ -1062,8 +1078,8 @@ static int run_vocab_grad(const VMatrices &x, const VPlan &p, const LogprobGradA
       b.M = (int)p.rows;
       b.N = p.H;
       b.a_rows = p.a_rows;
-      b.kwrap = (int)((vc + kVBK - 1) / kVBK);
-      b.kblocks = b.kwrap * (p.split ? 2 : 1);
+      b.kparts = p.split ? 2 : 1;
+      b.kblocks = (int)((vc + kVBK - 1) / kVBK) * b.kparts;
       b.shift = shift;
       b.idesc = idesc_f16(tm, kVBN, x.dtype, false, true);
       b.units_m = p.units_m;
@@ -1096,8 +1112,8 @@ static int run_vocab_grad(const VMatrices &x, const VPlan &p, const LogprobGradA
       b.M = (int)vc;
       b.N = p.H;
       b.a_rows = 128;  // of M: two boxes of 64
-      b.kwrap = (int)((p.rows + kVBK - 1) / kVBK);
-      b.kblocks = b.kwrap * (p.split ? 2 : 1);
+      b.kparts = p.split ? 2 : 1;
+      b.kblocks = (int)((p.rows + kVBK - 1) / kVBK) * b.kparts;
       b.shift = shift;
       b.idesc = idesc_f16(256, kVBN, x.dtype, true, true);
       b.units_m = (int)((vc + 255) / 256);
