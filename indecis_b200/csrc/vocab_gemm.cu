@@ -46,18 +46,15 @@ enum VEpi : int { kVStats = 0, kVDz = 1, kVOut = 2 };
 
 constexpr int kVBN = 256;   // tile columns
 constexpr int kVBK = 64;    // 16-bit elements of K per stage (128 bytes)
-// Epilogue warps: the plain stores keep up with eight; the exponentials take
-// sixteen, four per scheduler. With eight, 4096 x 65536 x 256 took 184 us
-// forward and 546 us backward, with sixteen 170 and 488; where K is 768 or
-// more the products cover either (within 1%).
-template <int EPI>
-struct VEpiShape {
-  static constexpr int kWarps = EPI == kVOut ? 8 : 16;
-  static constexpr int kGroups = kWarps / 4;       // warps per TMEM lane quarter
-  static constexpr int kCols = kVBN / kGroups;     // tile columns of a warp
-  static constexpr int kThreads = 64 + 32 * kWarps;
-};
-constexpr int kVStatGroups = VEpiShape<kVStats>::kGroups;
+// Sixteen epilogue warps, four per scheduler, a quarter of the tile's columns
+// each: with eight, 4096 x 65536 x 256 took 184 us forward and 546 us backward,
+// with sixteen 170 and 488, and one row's gradients at 262144 x 768 326 and 311;
+// where K is 768 or more and the rows are many the products cover either
+// (within 1%).
+constexpr int kVEpiWarps = 16;
+constexpr int kVEpiGroups = kVEpiWarps / 4;      // warps per TMEM lane quarter
+constexpr int kVEpiCols = kVBN / kVEpiGroups;    // tile columns of a warp
+constexpr int kVGemmThreads = 64 + 32 * kVEpiWarps;
 
 // Row coefficients of dZ (RowCoef with the output scale applied by the reader).
 struct VRowCoef {
@@ -76,7 +73,7 @@ struct VGemmArgs {
   int a_rows;  // rows of A's box (one CTA per tile: the rows there are, rounded up to 8; else 128)
   int n_fastest;                  // unit order: N parts innermost, else M tiles
   float c2;  // log2(e) / temperature
-  // kVStats: [M][units_n * kVStatGroups] partials; group maxima [M][ldmax] or NULL
+  // kVStats: [M][units_n * kVEpiGroups] partials; group maxima [M][ldmax] or NULL
   float4 *part;
   float *gmax;
   int64_t ldmax;
@@ -111,7 +108,7 @@ struct VSmem {
   static constexpr int kBBytes = (kVBN / CG) * kVBK * 2;
   static constexpr int kStageBytes = kABytes + kBBytes;
   // Staging per warp: two buffers for dZ's bulk stores, one to turn rows for the plain 16-bit stores.
-  static constexpr int kExtra = EPI == kVDz ? VEpiShape<EPI>::kWarps * 2 * 2048 : EPI == kVOut ? VEpiShape<EPI>::kWarps * 2048 : 0;
+  static constexpr int kExtra = EPI == kVDz ? kVEpiWarps * 2 * 2048 : EPI == kVOut ? kVEpiWarps * 2048 : 0;
   static constexpr int kRaw = (224 * 1024 - kExtra) / kStageBytes;
   static constexpr int kStages = kRaw > 6 ? 6 : kRaw;
   static constexpr int kExtraOff = kStages * kStageBytes;
@@ -209,7 +206,7 @@ __device__ __forceinline__ void store16(void *p, int64_t i, float v, int dtype) 
 }
 
 template <int CG, bool A_MN, bool B_MN, int EPI>
-__global__ void __launch_bounds__(VEpiShape<EPI>::kThreads, 1)
+__global__ void __launch_bounds__(kVGemmThreads, 1)
     vocab_gemm_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_constant__ CUtensorMap mapB,
                       const __grid_constant__ CUtensorMap mapC, const VGemmArgs a) {
   using S = VSmem<CG, EPI>;
@@ -237,7 +234,7 @@ __global__ void __launch_bounds__(VEpiShape<EPI>::kThreads, 1)
     }
     for (int b = 0; b < 2; b++) {
       mbar_init(&accf[b], 1);
-      mbar_init(&acce[b], CG * VEpiShape<EPI>::kWarps);
+      mbar_init(&acce[b], CG * kVEpiWarps);
     }
     fence_barrier_init();
   }
@@ -348,7 +345,7 @@ __global__ void __launch_bounds__(VEpiShape<EPI>::kThreads, 1)
     }
   } else {
     // TMEM lane quarter; columns [kCols g, kCols g + kCols).
-    constexpr int kCols = VEpiShape<EPI>::kCols;
+    constexpr int kCols = kVEpiCols;
     const int q4 = warp & 3, e = warp - 2, g = e >> 2;
     int tile = 0;
     bool ok = true;
@@ -393,20 +390,14 @@ __global__ void __launch_bounds__(VEpiShape<EPI>::kThreads, 1)
         }
         const uint32_t tb = tmem + b * kVBN + ((uint32_t)(q4 * 32) << 16);
         constexpr int kChunks = kCols / 32;
-        // Two chunks in registers where a warp has few others beside it.
-        constexpr int kBufs = VEpiShape<EPI>::kWarps == 8 ? 2 : 1;
-        uint32_t r[kBufs][32];
         [[maybe_unused]] float gm[2 * kChunks];
-        if constexpr (kBufs == 2) tmem_ld_32x32b_x32(tb + g * kCols, r[0]);
 #pragma unroll
         for (int i = 0; i < kChunks; i++) {
           __syncwarp();  // the branches below are per lane; the TMEM loads take the whole warp
-          if constexpr (kBufs == 1) tmem_ld_32x32b_x32(tb + g * kCols + 32 * i, r[0]);
+          uint32_t r[32];
+          tmem_ld_32x32b_x32(tb + g * kCols + 32 * i, r);
           tmem_ld_wait();
-          if (i + 1 == kChunks)
-            release();
-          else if constexpr (kBufs == 2)
-            tmem_ld_32x32b_x32(tb + g * kCols + 32 * (i + 1), r[(i + 1) & 1]);
+          if (i + 1 == kChunks) release();
           const int col0 = n * kVBN + g * kCols + 32 * i;
           if constexpr (EPI != kVDz) {
             if (col0 >= a.N) {
@@ -416,7 +407,7 @@ __global__ void __launch_bounds__(VEpiShape<EPI>::kThreads, 1)
           }
           float x[32];
 #pragma unroll
-          for (int k = 0; k < 32; k++) x[k] = __uint_as_float(r[i & (kBufs - 1)][k]);
+          for (int k = 0; k < 32; k++) x[k] = __uint_as_float(r[k]);
           if constexpr (EPI == kVStats) {
             if (col0 + 32 > a.N) {
 #pragma unroll
@@ -530,7 +521,7 @@ __global__ void __launch_bounds__(VEpiShape<EPI>::kThreads, 1)
         }
       }
       if constexpr (EPI == kVStats) {
-        if (ok && live) a.part[((int64_t)row * a.units_n + q.n) * kVStatGroups + g] = make_float4(st.m, st.s, st.u, 0.0f);
+        if (ok && live) a.part[((int64_t)row * a.units_n + q.n) * kVEpiGroups + g] = make_float4(st.m, st.s, st.u, 0.0f);
       }
     }
     if constexpr (EPI == kVDz) {
@@ -853,7 +844,7 @@ static int vgemm_slots() {
     at[0].val.clusterDim.y = 1;
     at[0].val.clusterDim.z = 1;
     cfg.gridDim = dim3(CG * (num_sms() / CG));
-    cfg.blockDim = dim3(VEpiShape<EPI>::kThreads);
+    cfg.blockDim = dim3(kVGemmThreads);
     cfg.dynamicSmemBytes = S::kTotal;
     cfg.attrs = at;
     cfg.numAttrs = 1;
@@ -875,7 +866,7 @@ static cudaError_t launch_vgemm(const CUtensorMap &ma, const CUtensorMap &mb, co
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute at[2];
   cfg.gridDim = dim3((unsigned)(CG * (units < slots ? units : slots)));
-  cfg.blockDim = dim3(VEpiShape<EPI>::kThreads);
+  cfg.blockDim = dim3(kVGemmThreads);
   cfg.dynamicSmemBytes = VSmem<CG, EPI>::kTotal;
   cfg.stream = st;
   if (CG > 1) {
@@ -941,7 +932,7 @@ static VPlan vocab_plan(int64_t rows, int V, int H, int top_k) {
   p.units_m = (int)((rows + tm - 1) / tm);
   const int64_t tiles = ((int64_t)V + kVBN - 1) / kVBN;
   p.units_n = best_parts(p.units_m, tiles, slots, kVMaxParts, 0.25);
-  p.part_bytes = align_up((size_t)p.units_n * kVStatGroups * rows * sizeof(float4), 256);
+  p.part_bytes = align_up((size_t)p.units_n * kVEpiGroups * rows * sizeof(float4), 256);
   p.ldmax = tiles * (kVBN / kVGroup);
   p.fwd_bytes = p.part_bytes + (top_k > 0 ? (size_t)rows * p.ldmax * 4 : 0);
   // With few rows, a given token's column or two carry most of the gradients,
@@ -1003,7 +994,7 @@ static int run_vocab_logprobs(const VMatrices &x, const VPlan &p, const LogprobA
   j.H = p.H;
   j.T = o.T;
   j.K = o.K;
-  j.parts = kVStatGroups * p.units_n;
+  j.parts = kVEpiGroups * p.units_n;
   j.dtype = x.dtype;
   j.c = o.c;
   j.ids = o.ids;
