@@ -486,6 +486,35 @@ def test_empty(voc):
     assert ((d.double() - want).abs() <= 1e-5 * (want.abs() + 1e-3)).all()
 
 
+@pytest.mark.parametrize("tail", [False, True])
+def test_distill_without_entries(voc, tail):
+    """Lists of length zero: no loss and no gradient, whatever the rows hold."""
+    x = make(3, 100, torch.bfloat16, 1)
+    x[1] = float("nan")
+    none = torch.empty((3, 0), dtype=torch.int32, device="cuda")
+    loss, d = voc.distill_topk(x, none, torch.empty((3, 0), device="cuda"), tail=tail)
+    assert (loss == 0).all() and (d == 0).all()
+
+
+def test_two_streams_at_once(voc):
+    """Calls in flight on two streams do not touch one another."""
+    xs = [make(600, 20011, torch.bfloat16, 83 + i) for i in range(2)]
+    ids = torch.randint(0, 20011, (600, 2), device="cuda", dtype=torch.int32)
+    want = [voc.token_logprobs(x, ids, top_k=8) for x in xs]
+    streams = [torch.cuda.Stream() for _ in xs]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(5):
+        for i, (st, x) in enumerate(zip(streams, xs)):
+            with torch.cuda.stream(st):
+                got[i].append(voc.token_logprobs(x, ids, top_k=8))
+    torch.cuda.synchronize()
+    for i in range(2):
+        for r in got[i]:
+            for a, b in zip(r, want[i]):
+                assert torch.equal(a, b)
+
+
 def test_bad_ids(voc):
     from indecis_b200 import ops
     ops.device_error()

@@ -260,6 +260,35 @@ def test_strides_streams_and_repeats(voc):
             assert torch.equal(a, b)
 
 
+def test_graph_capture(voc):
+    """Every operator recorded in one CUDA graph and replayed on new inputs."""
+    h, w = make(200, 3001, 72, torch.float16, 37)
+    ids = torch.randint(0, 3001, (200, 2), device="cuda", dtype=torch.int32)
+    g = torch.full((200, 2), -0.005, device="cuda")
+
+    def all_of_them():
+        r = voc.vocab_logprobs(h, w, ids, top_k=3)
+        dh, dw = voc.vocab_logprobs_backward(h, w, ids, r.logprobs, r.lse, r.entropy, g)
+        x = h @ w.T
+        s = voc.token_logprobs(x, ids, top_k=3)
+        d = voc.token_logprobs_backward(x, ids, s.lse, s.entropy, g)
+        loss, e = voc.distill_topk(x, s.top_ids, s.top_logprobs, tail=True)
+        return tuple(r) + (dh, dw) + tuple(s) + (d, loss, e)
+
+    st = torch.cuda.Stream()
+    st.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(st):
+        all_of_them()
+    torch.cuda.current_stream().wait_stream(st)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = all_of_them()
+    h.copy_(make(200, 3001, 72, torch.float16, 38)[0])
+    graph.replay()
+    for a, b in zip(out, all_of_them()):
+        assert torch.equal(a, b)
+
+
 def test_unaligned_gradients(voc):
     """The C entry point writes gradients at any stride and alignment."""
     from indecis_b200 import _capi
