@@ -904,7 +904,14 @@ static int best_parts(int64_t outer, int64_t tiles, int64_t slots, int64_t most,
 }
 
 constexpr int kVMaxParts = 256;        // column parts per M tile
-constexpr int kVOneCtaRows = 128;      // at most this many rows: single CTAs
+// At most this many rows: single CTAs (one row x 262144 x 768: 86 us, by pairs
+// 113; 128 rows 88 and 92).
+constexpr int kVOneCtaRows = 128;
+// At most this many rows: dZ in two 16-bit parts. In one part, a gradient's
+// error is 1.41 times its own rounding's in the median; the spread shrinks with
+// the rows (at 129 to 256 the 95th percentile is 1.48). Two parts cost 13 to
+// 32% there (256 x 262144 x 768: 385 us in one, 508 in two).
+constexpr int kVSplitRows = 128;
 constexpr int64_t kVDzBytes = 1ll << 30;  // dZ is formed in column chunks of at most this size
 
 struct VPlan {
@@ -938,7 +945,7 @@ static VPlan vocab_plan(int64_t rows, int V, int H, int top_k) {
   // With few rows, a given token's column or two carry most of the gradients,
   // and nothing averages the rounding of dZ: it is kept in two 16-bit parts
   // (16 or more bits), which doubles K where the weights' traffic bounds.
-  p.split = p.cg == 1;
+  p.split = rows <= kVSplitRows;
   int64_t chunk = kVDzBytes / (p.split ? 4 : 2) / (rows > 0 ? rows : 1) / kVBN * kVBN;
   if (chunk < kVBN) chunk = kVBN;
   if (chunk > tiles * kVBN) chunk = tiles * kVBN;
