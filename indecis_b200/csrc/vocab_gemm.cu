@@ -702,7 +702,7 @@ __global__ void __launch_bounds__(kVocThreads) vocab_join_kernel(const VJoinArgs
 
 struct VCoefArgs {
   int64_t rows;
-  int V, T, dtype;
+  int V, T;
   float c;
   const int32_t *ids;
   const float *lse, *entropy, *dlogprobs, *dentropy;
@@ -736,8 +736,8 @@ __global__ void vocab_coef_kernel(const VCoefArgs a) {
 }
 
 struct VTokenArgs {
-  int64_t rows, n;  // n = rows * T
-  int T, V, v0, v1, dtype;
+  int64_t n;  // rows * T
+  int T, v0, v1, dtype;
   float c;
   const int32_t *ids;
   const float *logprobs, *dlogprobs;
@@ -1032,7 +1032,7 @@ static int run_vocab_grad(const VMatrices &x, const VPlan &p, const LogprobGradA
   uint8_t *dz = ws + p.coef_bytes;
   float *p32 = reinterpret_cast<float *>(dz + p.dz_bytes);
   if (bound) IG_CU(cudaMemsetAsync(bound, 0, 4, st));
-  const VCoefArgs ca{p.rows, p.V, g.T, x.dtype, g.c, g.ids, g.lse, g.entropy, g.dlogprobs, g.dentropy, coef, bound};
+  const VCoefArgs ca{p.rows, p.V, g.T, g.c, g.ids, g.lse, g.entropy, g.dlogprobs, g.dentropy, coef, bound};
   vocab_coef_kernel<<<(unsigned)((p.rows + 7) / 8), 256, 0, st>>>(ca);
   IG_CU(cudaGetLastError());
   const int tm = 128 * p.cg, shift = p.split ? (int)p.chunk : 0;
@@ -1065,7 +1065,7 @@ static int run_vocab_grad(const VMatrices &x, const VPlan &p, const LogprobGradA
     IG_CU(p.cg == 1 ? (launch_vgemm<1, false, false, kVDz>(mh, mw, mzs, a, st))
                     : (launch_vgemm<2, false, false, kVDz>(mh, mw, mzs, a, st)));
     if (g.dlogprobs && g.T > 0) {
-      VTokenArgs t{p.rows, p.rows * g.T, g.T, p.V, (int)v0, (int)(v0 + vc), x.dtype, g.c, g.ids, o.logprobs, g.dlogprobs,
+      VTokenArgs t{p.rows * g.T, g.T, (int)v0, (int)(v0 + vc), x.dtype, g.c, g.ids, o.logprobs, g.dlogprobs,
                    coef, bound, dz, p.ldz, shift};
       IG_CU(launch_dep(vocab_token_kernel, dim3((unsigned)((t.n + 255) / 256)), dim3(256), 0, st, t));
     }

@@ -21,7 +21,7 @@ namespace ig {
 
 constexpr int kVocThreads = 256;  // most threads per CTA (NT below: 32 to 256)
 constexpr int kVocWarps = kVocThreads / 32;
-constexpr int kVocUnroll = 4;     // 16-byte vectors in flight per thread
+constexpr int kVocUnroll = 4;     // 16-byte vectors of a thread per round
 constexpr int kTopMax = 32;       // alternatives per row
 constexpr int kIdsMax = 256;      // given tokens or teacher entries per row
 constexpr float kLog2e = 1.44269504088896340736f;

@@ -260,6 +260,24 @@ def test_strides_streams_and_repeats(voc):
             assert torch.equal(a, b)
 
 
+@pytest.mark.parametrize("rows", [3, 300])
+def test_no_given_tokens(voc, rows):
+    """Entropy alone: no given tokens, forward and backward."""
+    h, w = make(rows, 500, 64, torch.bfloat16, 41)
+    none = torch.empty((rows, 0), dtype=torch.int32, device="cuda")
+    gh = torch.linspace(-1, 1, rows, device="cuda")
+    r = voc.vocab_logprobs(h, w, none, top_k=2)
+    assert r.logprobs.shape == (rows, 0)
+    dh, dw = voc.vocab_logprobs_backward(h, w, none, r.logprobs, r.lse, r.entropy, torch.empty((rows, 0), device="cuda"), gh)
+    one = torch.full((rows, 1), -1, dtype=torch.int32, device="cuda")
+    zero = torch.zeros((rows, 1), device="cuda")
+    s = voc.vocab_logprobs(h, w, one, top_k=2)
+    for a, b in zip(r[1:], s[1:]):
+        assert torch.equal(a, b)
+    eh, ew = voc.vocab_logprobs_backward(h, w, one, zero, s.lse, s.entropy, zero, gh)
+    assert torch.equal(dh, eh) and torch.equal(dw, ew) and (dw != 0).any()
+
+
 def test_graph_capture(voc):
     """Every operator recorded in one CUDA graph and replayed on new inputs."""
     h, w = make(200, 3001, 72, torch.float16, 37)
