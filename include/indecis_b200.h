@@ -352,7 +352,10 @@ IG_API int ig_token_logprobs(const void *logits, int32_t dtype, int64_t ld, int6
  * without dentropy): dlogits[r][j] = (sum_t dlogprobs[t] (1[j = ids[t]] - p_j)
  * - dentropy p_j (log p_j + entropy)) / temperature, rounded once to the
  * logits' type. Repeated ids add up; ids outside the vocabulary give nothing.
- * Zero for a row of -inf only. dlogits may be logits (with ldd = ld). */
+ * Zero for a row of -inf only. lse gives p as far as float32 holds it; for
+ * |lse| > 1024 (a row wholly masked by a finite value, a large offset, a very
+ * low temperature) the row's maximum and sum are formed again from the logits.
+ * dlogits may be logits (with ldd = ld). */
 IG_API int ig_token_logprobs_backward(const void *logits, int32_t dtype, int64_t ld, int64_t rows, int32_t vocab,
                                       double temperature, const int32_t *ids, int32_t nids, const float *lse,
                                       const float *entropy, const float *dlogprobs, const float *dentropy,
@@ -400,7 +403,10 @@ IG_API int ig_vocab_logprobs(const void *hidden, int64_t ldh, const void *weight
  * dweight = G^T . hidden, in the operands' type, strides free. G is formed
  * in the workspace in column chunks and rounded to the operands' type (for
  * float16 scaled by a power of two, so that small probabilities keep their
- * bits); the sums are float32 in a fixed order. */
+ * bits); the sums are float32 in a fixed order. p = exp(min(z - lse, 0)), off
+ * by |lse| 2^-24 of itself through lse's rounding; in a row whose lse float32
+ * does not resolve (wholly masked by a bias past 2^22, say) the columns within
+ * a step of the maximum have p = 1. */
 IG_API int ig_vocab_logprobs_backward(const void *hidden, int64_t ldh, const void *weight, int64_t ldw, int32_t dtype,
                                       int64_t rows, int32_t vocab, int32_t hidden_size, double temperature,
                                       const int32_t *ids, int32_t nids, const float *logprobs, const float *lse,

@@ -58,7 +58,7 @@ constexpr int kVGemmThreads = 64 + 32 * kVEpiWarps;
 
 // Row coefficients of dZ (RowCoef with the output scale applied by the reader).
 struct VRowCoef {
-  float A, B, lse2, pad;
+  float A, B, l, pad;
 };
 
 constexpr int kVGroup = 16;  // columns per stored maximum
@@ -72,7 +72,7 @@ struct VGemmArgs {
   int units_m, units_n, units_s;  // units: M tiles x N parts x K parts
   int a_rows;  // rows of A's box (one CTA per tile: the rows there are, rounded up to 8; else 128)
   int n_fastest;                  // unit order: N parts innermost, else M tiles
-  float c2;  // log2(e) / temperature
+  float c, c2;  // 1 / temperature, log2(e) / temperature
   // kVStats: [M][units_n * kVEpiGroups] partials; group maxima [M][ldmax] or NULL
   float4 *part;
   float *gmax;
@@ -360,7 +360,7 @@ __global__ void __launch_bounds__(kVGemmThreads, 1)
         if (live) {
           const VRowCoef v = a.coef[row];
           const float sc = vocab_scale(a.bound);
-          rc = RowCoef{v.A * sc, v.B * sc, v.lse2};
+          rc = RowCoef{v.A * sc, v.B * sc, v.l};
         }
       }
       [[maybe_unused]] float unscale = 1.0f;
@@ -429,7 +429,7 @@ __global__ void __launch_bounds__(kVGemmThreads, 1)
             float d[32];
 #pragma unroll
             for (int k = 0; k < 32; k += 2) {
-              const float2 v = dense_grad2(make_float2(x[k], x[k + 1]), a.c2, rc);
+              const float2 v = dense_grad2<true>(make_float2(x[k], x[k + 1]), a.c, rc);
               d[k] = v.x;
               d[k + 1] = v.y;
             }
@@ -729,10 +729,10 @@ __global__ void vocab_coef_kernel(const VCoefArgs a) {
   const float gh = a.dentropy ? a.dentropy[row] : 0.0f, H = a.dentropy ? a.entropy[row] : 0.0f;
   const float lse = a.lse[row];
   const RowCoef k = row_coef(lse, H, G, gh, a.c);
-  a.coef[row] = VRowCoef{k.A, k.B, k.lse2, 0.0f};
-  // |dZ| <= c (sum |g| (1 + p) + |gH| p (|log p| + H)) <= c (2 sum |g| + |gH| (1 + H))
+  a.coef[row] = VRowCoef{k.A, k.B, k.l, 0.0f};
+  // |dZ| <= c (sum |g| (1 + p) + |gH| p (|log p| + H)) <= c (2 sum |g| + |gH| (1 + H)), as p <= 1
   const float b = a.c * (2.0f * size + fabsf(gh) * (1.0f + H));
-  if (a.bound && k.lse2 != IG_INF && b > 0.0f && b < 3.0e38f) atomicMax(a.bound, __float_as_int(b));
+  if (a.bound && k.l != IG_INF && b > 0.0f && b < 3.0e38f) atomicMax(a.bound, __float_as_int(b));
 }
 
 struct VTokenArgs {
@@ -758,10 +758,10 @@ __global__ void vocab_token_kernel(const VTokenArgs a) {
   const int64_t row = i / a.T;
   const int id = a.ids[i];
   if (id < a.v0 || id >= a.v1) return;
-  const VRowCoef k = a.coef[row];
-  if (k.lse2 == IG_INF) return;  // no distribution
-  const float y = max_nan(a.logprobs[i] * kLog2e, kYMin);
-  float d = ex2(y) * fmaf(k.B, y, k.A) + token_grad(a.ids + row * a.T, a.dlogprobs + row * a.T, a.T, id, a.c);
+  const VRowCoef v = a.coef[row];
+  const RowCoef k{v.A, v.B, v.l};
+  if (k.l == IG_INF) return;  // no distribution
+  float d = dense_grad(log_prob<true>(a.logprobs[i]), k) + token_grad(a.ids + row * a.T, a.dlogprobs + row * a.T, a.T, id, a.c);
   d *= vocab_scale(a.bound);
   const int64_t at = row * a.ldz + id - a.v0;
   const uint32_t w = pack16(d, 0.0f, a.dtype);
@@ -1056,7 +1056,7 @@ static int run_vocab_grad(const VMatrices &x, const VPlan &p, const LogprobGradA
     a.units_m = p.units_m;
     a.units_n = (int)((vc + kVBN - 1) / kVBN);
     a.units_s = 1;
-    a.c2 = g.c * kLog2e;
+    a.c = g.c;
     a.coef = coef;
     a.split = p.split;
     a.shift = shift;

@@ -41,6 +41,12 @@ __device__ __forceinline__ float max_nan(float a, float b) {
   return r;
 }
 
+__device__ __forceinline__ float min_nan(float a, float b) {
+  float r;
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+
 // ---- element types --------------------------------------------------------------
 
 // unpack/pack: a 16-byte vector as floats; kNegInf: -inf in every element;
@@ -751,21 +757,29 @@ struct LogprobGradArgs {
   int64_t ldd;
 };
 
-// The row's gradient outside its given tokens is p (A + B y) with
-// y = log2 p = x c log2(e) - lse log2(e):
-//   A = -c (sum of the tokens' gradients + gH H), B = -c gH ln 2.
+// The row's gradient outside its given tokens is p (A + B t) with
+// t = log p = x c - l, l the row's logsumexp, in one multiply-add:
+//   A = -c (sum of the tokens' gradients + gH H), B = -c gH.
 struct RowCoef {
-  float A, B, lse2;
+  float A, B, l;
 };
-__device__ __forceinline__ float dense_grad(float x, float c2, const RowCoef &k) {
-  const float y = max_nan(fmaf(x, c2, -k.lse2), kYMin);
-  return ex2(y) * fmaf(k.B, y, k.A);
+constexpr float kTMin = -1.0e4f;  // e^kTMin = 0
+// A log probability; HOLD: at or below 0, where l may be one that float32 does
+// not resolve. NaN is kept.
+template <bool HOLD>
+__device__ __forceinline__ float log_prob(float t) {
+  t = max_nan(t, kTMin);
+  return HOLD ? min_nan(t, 0.0f) : t;
 }
-__device__ __forceinline__ float2 dense_grad2(float2 x, float c2, const RowCoef &k) {
-  float2 y = __ffma2_rn(x, make_float2(c2, c2), make_float2(-k.lse2, -k.lse2));
-  y.x = max_nan(y.x, kYMin);
-  y.y = max_nan(y.y, kYMin);
-  return __fmul2_rn(make_float2(ex2(y.x), ex2(y.y)), __ffma2_rn(make_float2(k.B, k.B), y, make_float2(k.A, k.A)));
+// From t = log_prob(..).
+__device__ __forceinline__ float dense_grad(float t, const RowCoef &k) { return ex2(t * kLog2e) * fmaf(k.B, t, k.A); }
+template <bool HOLD>
+__device__ __forceinline__ float2 dense_grad2(float2 x, float c, const RowCoef &k) {
+  float2 t = __ffma2_rn(x, make_float2(c, c), make_float2(-k.l, -k.l));
+  t.x = log_prob<HOLD>(t.x);
+  t.y = log_prob<HOLD>(t.y);
+  const float2 y = __fmul2_rn(t, make_float2(kLog2e, kLog2e));
+  return __fmul2_rn(make_float2(ex2(y.x), ex2(y.y)), __ffma2_rn(make_float2(k.B, k.B), t, make_float2(k.A, k.A)));
 }
 // The gradient a given token adds in its own column: c times the sum over the
 // row's entries with the same id, in order.
@@ -788,18 +802,9 @@ __device__ __forceinline__ float given_grad_sum(const int32_t *ids, const float 
   for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(~0u, s, o);
   return s;
 }
-__device__ __forceinline__ RowCoef row_coef(float lse, float H, float G, float gh, float c) {
-  RowCoef k;
-  k.B = -c * gh * kLn2;
-  k.A = -c * fmaf(gh, H, G);
-  k.lse2 = lse * kLog2e;
-  // No distribution: nothing left, or all of it masked by the type's lowest
-  // value, whose lse cannot tell the columns apart.
-  if (k.lse2 < -1.0e38f) {
-    k.A = k.B = 0.0f;
-    k.lse2 = IG_INF;
-  }
-  return k;
+__device__ __forceinline__ RowCoef row_coef(float l, float H, float G, float gh, float c) {
+  if (l == -IG_INF) return RowCoef{0.0f, 0.0f, IG_INF};  // no distribution
+  return RowCoef{-c * fmaf(gh, H, G), -c * gh, l};
 }
 
 // Writes the kN results of a whole vector: as one 16-byte store where the
@@ -824,17 +829,116 @@ __device__ __forceinline__ void store_edge(typename VElem<DT>::T *drow, const Ro
   }
 }
 
+// The given tokens' columns of a part, [cfirst, clast): their logits, read
+// before any store (dx may be x), and after the part their gradients.
+template <int DT, int NT>
+__device__ __forceinline__ void given_logits(const typename VElem<DT>::T *row, const int32_t *ids, int T, int cfirst,
+                                             int clast, float *s_xt) {
+  for (int i = threadIdx.x; i < T; i += NT) {
+    const int id = ids[i];
+    if (id >= cfirst && id < clast) s_xt[i] = VElem<DT>::get(row[id]);
+  }
+}
+// m: what l is counted from.
+template <int DT, int NT>
+__device__ __forceinline__ void given_grads(typename VElem<DT>::T *drow, const int32_t *ids, const float *g, int T, int cfirst,
+                                            int clast, const float *s_xt, float m, float c, const RowCoef &k) {
+  for (int i = threadIdx.x; i < T; i += NT) {
+    const int id = ids[i];
+    if (id >= cfirst && id < clast)
+      drow[id] = VElem<DT>::put(dense_grad(log_prob<false>(fmaf(s_xt[i] - m, c, -k.l)), k) + token_grad(ids, g, T, id, c));
+  }
+}
+
+// The largest |lse| that the gradient is formed from: float32 holds it to
+// |lse| 2^-24, 6e-5 at most, which is the relative error of p. Past it (a row
+// wholly masked by a finite value, logits at a large offset, a very low
+// temperature; also -inf, which the product with 1 / temperature gives for
+// large finite masks) one CTA takes the whole row and its maximum and sum
+// again, as the forward has them: 120 us where 2047 x 50021 bf16 takes 73 from
+// lse, 372 and 263 for 4096 x 50021 float32, 66 and 15 for 16 x 262144.
+constexpr float kLseMost = 1024.0f;
+
+template <int DT, int NT>
+__device__ __noinline__ void grad_whole_row(const LogprobGradArgs &a, int64_t row, float G, float H, float gh, void *slots,
+                                            float *s_xt, VStat *s_warp) {
+  using E = VElem<DT>;
+  using T = typename E::T;
+  constexpr int kN = E::kN;
+  const int tid = (int)threadIdx.x;
+  const RowVecs<DT> rv(static_cast<const T *>(a.x) + row * a.ld, a.V);
+  const RowPart<DT> rp(rv, 0, 1);
+  T *drow = static_cast<T *>(a.dx) + row * a.ldd;
+  const bool same = (reinterpret_cast<uintptr_t>(drow) & 15) == (reinterpret_cast<uintptr_t>(rv.row) & 15);
+  const float c2 = a.c * kLog2e;
+  Ahead<NT> ahead(slots, rp.base + tid, rp.n - tid);
+  ahead.start();
+  uint4 edge;
+  const bool has_edge = (tid == kFirstThread && rp.first) || (tid == last_thread(NT) && rp.last);
+  const int edge_v = tid == kFirstThread ? rp.v0 : rp.v1 - 1;
+  if (has_edge) edge = rv.edge(edge_v);
+  const int32_t *ids = a.ids + row * a.T;
+  if (a.dlogprobs) given_logits<DT, NT>(rv.row, ids, a.T, 0, a.V, s_xt);
+  VStat st{-IG_INF, 0.0f, 0.0f};
+  ahead.each([&](int b, const uint4(&raw)[kVocUnroll]) {
+#pragma unroll
+    for (int j = 0; j < kVocUnroll; j++)
+      if (b + j * NT < ahead.mine) {
+        const uint4 one[1] = {raw[j]};
+        vstat_add_raw<DT, false>(st, one, c2);
+      }
+  });
+  if (has_edge) {
+    const uint4 one[1] = {edge};
+    vstat_add_raw<DT, false>(st, one, c2);
+  }
+  ahead.start();
+  st = vstat_warp<false>(st, c2);
+  if ((tid & 31) == 0) s_warp[tid >> 5] = st;
+  __syncthreads();
+  st = vstat_join<false>(s_warp, NT / 32, c2);
+  const float m = st.s == 0.0f ? 0.0f : st.m;
+  const RowCoef k = row_coef(st.s == 0.0f ? -IG_INF : logf(st.s), H, G, gh, a.c);
+  auto grad = [&](const uint4 &v, float *d) {
+    float x[kN];
+    E::unpack(v, x);
+#pragma unroll
+    for (int i = 0; i < kN; i += 2) {
+      const float2 r = dense_grad2<false>(make_float2(x[i] - m, x[i + 1] - m), a.c, k);
+      d[i] = r.x;
+      d[i + 1] = r.y;
+    }
+  };
+  T *dp = drow + rv.col(rp.w0) + (int64_t)tid * kN;
+  ahead.each([&](int b, const uint4(&raw)[kVocUnroll]) {
+#pragma unroll
+    for (int j = 0; j < kVocUnroll; j++) {
+      if (b + j * NT >= ahead.mine) break;
+      float d[kN];
+      grad(raw[j], d);
+      store_whole<DT>(dp + (int64_t)(b + j * NT) * kN, same, d);
+    }
+  });
+  if (has_edge) {
+    float d[kN];
+    grad(edge, d);
+    store_edge<DT>(drow, rv, edge_v, d);
+  }
+  if (!a.dlogprobs || st.s == 0.0f) return;
+  __syncthreads();
+  given_grads<DT, NT>(drow, ids, a.dlogprobs + row * a.T, a.T, 0, a.V, s_xt, m, a.c, k);
+}
+
 // A CTA per part of a row, element by element from the row's saved lse and
 // entropy: bound by the bytes (each read once, written once). 2047 x 50021
-// bf16: 73 us, 5.6 TB/s, 87% of the measured copy bandwidth. The given tokens'
-// columns are written again after the part (their logits are read first: dx
-// may be x).
+// bf16: 73 us, 5.6 TB/s, 87% of the measured copy bandwidth.
 template <int DT, int NT>
-__global__ void __launch_bounds__(NT, 1024 / NT) token_logprobs_grad_kernel(const LogprobGradArgs a) {
+__global__ void __launch_bounds__(NT, 1024 / NT) token_logprobs_grad_kernel(const __grid_constant__ LogprobGradArgs a) {
   using E = VElem<DT>;
   using T = typename E::T;
   constexpr int kN = E::kN;
   __shared__ float s_G, s_xt[kIdsMax];
+  __shared__ VStat s_warp[NT / 32];
   const int64_t row = blockIdx.x / a.segs;
   const int seg = (int)(blockIdx.x - row * a.segs);
   const RowVecs<DT> rv(static_cast<const T *>(a.x) + row * a.ld, a.V);
@@ -857,23 +961,21 @@ __global__ void __launch_bounds__(NT, 1024 / NT) token_logprobs_grad_kernel(cons
     if (a.dlogprobs && bad) set_device_error(kDevBadId);
     if (threadIdx.x == 0) s_G = s;
   }
-  // The given tokens' logits are read before any store: dx may be x.
   const int cfirst = max(rv.col(rp.v0), 0), clast = min(rv.col(rp.v1), a.V);
-  if (a.dlogprobs) {
-    for (int i = threadIdx.x; i < a.T; i += NT) {
-      const int id = ids[i];
-      if (id >= cfirst && id < clast) s_xt[i] = E::get(rv.row[id]);
-    }
-  }
+  if (a.dlogprobs) given_logits<DT, NT>(rv.row, ids, a.T, cfirst, clast, s_xt);
   __syncthreads();
+  if (!(fabsf(lse) <= kLseMost)) {
+    cp_async_wait_all();
+    if (seg == 0) grad_whole_row<DT, NT>(a, row, s_G, H, gh, s_ahead, s_xt, s_warp);
+    return;
+  }
   const RowCoef k = row_coef(lse, H, s_G, gh, a.c);
-  const float c2 = a.c * kLog2e;
   auto grad = [&](const uint4 &v, float *d) {
     float x[kN];
     E::unpack(v, x);
 #pragma unroll
     for (int i = 0; i < kN; i += 2) {
-      const float2 r = dense_grad2(make_float2(x[i], x[i + 1]), c2, k);
+      const float2 r = dense_grad2<false>(make_float2(x[i], x[i + 1]), a.c, k);
       d[i] = r.x;
       d[i + 1] = r.y;
     }
@@ -895,12 +997,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT) token_logprobs_grad_kernel(cons
   }
   if (a.T == 0 || !a.dlogprobs) return;
   __syncthreads();
-  if (k.lse2 == IG_INF) return;
-  for (int i = threadIdx.x; i < a.T; i += NT) {
-    const int id = ids[i];
-    if (id >= cfirst && id < clast)
-      drow[id] = E::put(dense_grad(s_xt[i], c2, k) + token_grad(ids, g, a.T, id, a.c));
-  }
+  given_grads<DT, NT>(drow, ids, g, a.T, cfirst, clast, s_xt, 0.0f, a.c, k);
 }
 
 // ---- divergence from a teacher's top logits ----------------------------------------------

@@ -1,0 +1,140 @@
+"""Vocabulary operators where float32 or the inputs leave little room, against plain float64 forms.
+
+Tolerances as in test_gpu_vocab.py (STAT_TOL, P_TOL) and test_gpu_vocab_head.py (LOGIT).
+"""
+import math
+
+import pytest
+import torch
+
+from test_gpu_vocab import DTYPES, EPS, INF, P_TOL, STAT_TOL, TINY, close, make, ref_gradient
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def voc(igdev):
+    from indecis_b200 import vocab
+    return vocab
+
+
+# ---- gradients of rows far from zero ---------------------------------------------------------------------------------
+
+
+def gradient_close(d, x, ids, g, gh, temperature):
+    """d against float64, with the tolerances of test_gpu_vocab.test_backward."""
+    dtype = x.dtype
+    want, p = ref_gradient(x, ids, g, gh, temperature)
+    size = g.abs().sum(1, keepdim=True) + gh.abs()[:, None] * 40
+    tol = P_TOL * p * size + 2e-6 * g.abs().sum(1, keepdim=True) / temperature * (want.abs() > p) + \
+        EPS[dtype] / 2 * want.abs() * 1.01 + TINY[dtype]
+    assert d.isfinite().all()
+    assert ((d.double() - want).abs() <= tol).all()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,V,pad,shift", [(12, 37, 0, 0), (12, 5003, 3, 1), (12, 262145, 0, 0), (2400, 2049, 0, 0)])
+def test_gradient_of_masked_rows(voc, dtype, rows, V, pad, shift):
+    """Rows wholly masked by a finite value are uniform, forward and backward, whatever the value; zero gradients stay
+    zero there."""
+    x = make(rows, V, dtype, 131 + V, pad, shift)
+    values = [v for v in (-1e4, -1e9, -1e10, -1e30, torch.finfo(dtype).min) if abs(v) <= torch.finfo(dtype).max]
+    for i, v in enumerate(values):
+        x[2 * i] = v
+    zero = 2 * len(values)  # the last masked row again, with gradients of zero
+    x[zero] = values[-1]
+    gen = torch.Generator(device="cuda").manual_seed(6)
+    ids = torch.randint(-1, V, (rows, 5), generator=gen, device="cuda", dtype=torch.int32)
+    ids[:, 4] = ids[:, 0]
+    g = torch.randn((rows, 5), generator=gen, device="cuda")
+    gh = torch.randn((rows,), generator=gen, device="cuda")
+    g[zero] = 0
+    gh[zero] = 0
+    for temperature in (0.5, 1.0, 5.5, 8.0):
+        r = voc.token_logprobs(x, ids, temperature=temperature)
+        d = voc.token_logprobs_backward(x, ids, r.lse, r.entropy, g, gh, temperature=temperature)
+        gradient_close(d, x, ids, g, gh, temperature)
+        assert (d[zero] == 0).all()
+        y = x.contiguous().clone()
+        voc.token_logprobs_backward(y, ids, r.lse, r.entropy, g, gh, temperature=temperature, out=y)
+        gradient_close(y, x, ids, g, gh, temperature)
+
+
+@pytest.mark.parametrize("rows,V", [(7, 4099), (3, 262145), (2400, 1025)])
+@pytest.mark.parametrize("offset,temperature", [(-5000.0, 1.0), (20000.0, 1.0), (1e6, 3.0), (0.0, 0.005)])
+def test_gradient_far_from_zero(voc, rows, V, offset, temperature):
+    """float32 logits at a large offset, or scaled by a low temperature: the gradient does not lose the bits that the
+    absolute logsumexp has lost. (x - m) / temperature is up to 64 where it counts, so the temperature's own rounding
+    to float32 (2^-24 relative) is inside P_TOL."""
+    x = make(rows, V, torch.float32, 141, scale=1.0 if temperature > 0.1 else 0.03) + offset
+    if temperature < 0.1:
+        x += 10.0
+    gen = torch.Generator(device="cuda").manual_seed(6)
+    ids = torch.randint(-1, V, (rows, 3), generator=gen, device="cuda", dtype=torch.int32)
+    g = torch.randn((rows, 3), generator=gen, device="cuda")
+    gh = torch.randn((rows,), generator=gen, device="cuda")
+    r = voc.token_logprobs(x, ids, temperature=temperature)
+    d = voc.token_logprobs_backward(x, ids, r.lse, r.entropy, g, gh, temperature=temperature)
+    gradient_close(d, x, ids, g, gh, temperature)
+    # Rows that are no distribution, beside them.
+    x[0] = -INF
+    x[1, V // 2] = float("nan")
+    x[2, V // 3] = INF
+    ids[0, 1] = 5
+    r = voc.token_logprobs(x, ids, temperature=temperature)
+    y = x.clone()
+    voc.token_logprobs_backward(y, ids, r.lse, r.entropy, g, gh, temperature=temperature, out=y)
+    assert (y[0] == 0).all() and y[1].isnan().all() and y[2].isnan().all()
+    if rows > 3:
+        assert torch.equal(y[3:], d[3:])
+
+
+def biased(rows, V, H, dtype, seed, bias):
+    """hidden extended by a column of ones, weight by a column of the tokens' biases."""
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    h = torch.randn(rows, H, generator=g, device="cuda")
+    w = torch.randn(V, H, generator=g, device="cuda") * 0.1
+    h[:, H - 1] = 1.0
+    w[:, H - 1] = bias
+    return h.to(dtype), w.to(dtype)
+
+
+@pytest.mark.parametrize("dtype,bias", [(torch.bfloat16, -1e4), (torch.bfloat16, -1e9), (torch.bfloat16, -1e10),
+                                        (torch.bfloat16, -1e30), (torch.bfloat16, torch.finfo(torch.bfloat16).min),
+                                        (torch.float16, -6e4), (torch.float16, torch.finfo(torch.float16).min)])
+@pytest.mark.parametrize("rows", [5, 200])
+def test_head_gradient_of_masked_rows(voc, dtype, bias, rows):
+    """All tokens masked by a finite bias. Nothing is held of the states beside a bias of -1e9, but every probability is
+    at most 1: the gradients are finite and bounded, and zero where the incoming ones are."""
+    V, H = 999, 72
+    h, w = biased(rows, V, H, dtype, 151, bias)
+    gen = torch.Generator(device="cuda").manual_seed(6)
+    ids = torch.randint(0, V, (rows, 2), generator=gen, device="cuda", dtype=torch.int32)
+    g = torch.randn((rows, 2), generator=gen, device="cuda")
+    gh = torch.randn((rows,), generator=gen, device="cuda")
+    g[1] = 0
+    gh[1] = 0
+    for temperature in (0.5, 1.0, 5.5, 8.0):
+        r = voc.vocab_logprobs(h, w, ids, temperature=temperature)
+        dh, dw = voc.vocab_logprobs_backward(h, w, ids, r.logprobs, r.lse, r.entropy, g, gh, temperature=temperature)
+        dh, dw = dh[:, :H - 1], dw[:, :H - 1]  # the constant's own gradient is of the bias's size
+        assert dh.isfinite().all() and dw.isfinite().all()
+        assert (dh[1] == 0).all()
+        size = (2 * g.abs().sum(1) + gh.abs() * (1 + math.log(V) + 1)) / temperature
+        assert (dh.float().abs() <= 1.01 * size[:, None] * w[:, :H - 1].float().abs().sum(0)).all()
+        assert (dw.float().abs() <= 1.01 * (size[:, None] * h[:, :H - 1].float().abs()).sum(0)).all()
+        if r.lse.abs().max() < 1e5:
+            # The distribution is still there: p is off by lse's rounding (|lse| 2^-24) and the logits' (LOGIT of |bias|).
+            z = h.double() @ w.double().T / temperature
+            logp = torch.log_softmax(z, 1)
+            G = -g.double().sum(1, keepdim=True) * logp.exp()
+            ent = -(logp.exp() * logp).sum(1, keepdim=True)
+            G -= gh.double()[:, None] * logp.exp() * (logp + ent)
+            G.scatter_add_(1, ids.long(), g.double())
+            G /= temperature
+            off = 2 * (float(r.lse.abs().max()) * 2.0**-24 + abs(bias) * 2.0**-20 / temperature)
+            slack = (g.abs().sum(1) + gh.abs() * (1 + 2 * math.log(V)))[:, None].double() * logp.exp() / temperature
+            err = slack * (P_TOL + math.expm1(off)) + torch.finfo(dtype).eps * G.abs() + 1e-7
+            tol = err @ w[:, :H - 1].double().abs()
+            want = G @ w[:, :H - 1].double()
+            assert ((dh.double() - want).abs() <= tol + torch.finfo(dtype).eps * want.abs() + 1e-7).all()
