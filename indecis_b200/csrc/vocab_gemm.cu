@@ -719,11 +719,9 @@ __global__ void vocab_coef_kernel(const VCoefArgs a) {
   bool bad = false;
   float G = 0.0f, size = 0.0f;
   if (a.dlogprobs) {
-    G = given_grad_sum(a.ids + row * a.T, a.dlogprobs + row * a.T, a.T, a.V, bad);
+    G = given_grad_sum(a.ids + row * a.T, a.dlogprobs + row * a.T, a.T, a.V, bad, size);
     if (bad) set_device_error(kDevBadId);
-    for (int t = lane; t < a.T; t += 32) size += fabsf(a.dlogprobs[row * a.T + t]);
-#pragma unroll
-    for (int o = 16; o; o >>= 1) size += __shfl_xor_sync(~0u, size, o);
+    size = warp_sum(size);
   }
   if (lane) return;
   const float gh = a.dentropy ? a.dentropy[row] : 0.0f, H = a.dentropy ? a.entropy[row] : 0.0f;

@@ -789,14 +789,20 @@ __device__ __forceinline__ float token_grad(const int32_t *ids, const float *g, 
     if (ids[t] == id) s += g[t];
   return s * c;
 }
-// Sum over the row's given tokens (ids in the vocabulary), one warp, in a fixed order.
-__device__ __forceinline__ float given_grad_sum(const int32_t *ids, const float *g, int T, int V, bool &bad) {
+// Sum over the row's given tokens (ids in the vocabulary), one warp, in a fixed
+// order; size: of the absolute values, per lane. Entries that are not given
+// count for neither.
+__device__ __forceinline__ float given_grad_sum(const int32_t *ids, const float *g, int T, int V, bool &bad, float &size) {
   float s = 0.0f;
   bad = false;
+  size = 0.0f;
   for (int t = threadIdx.x & 31; t < T; t += 32) {
     const int id = ids[t];
     if (id >= V) bad = true;
-    if (id >= 0 && id < V) s += g[t];
+    if (id >= 0 && id < V) {
+      s += g[t];
+      size += fabsf(g[t]);
+    }
   }
 #pragma unroll
   for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(~0u, s, o);
@@ -957,7 +963,8 @@ __global__ void __launch_bounds__(NT, 1024 / NT) token_logprobs_grad_kernel(cons
   const float gh = a.dentropy ? a.dentropy[row] : 0.0f, H = a.dentropy ? a.entropy[row] : 0.0f;
   if (threadIdx.x < 32) {
     bool bad;
-    const float s = a.dlogprobs ? given_grad_sum(ids, g, a.T, a.V, bad) : 0.0f;
+    float size;
+    const float s = a.dlogprobs ? given_grad_sum(ids, g, a.T, a.V, bad, size) : 0.0f;
     if (a.dlogprobs && bad) set_device_error(kDevBadId);
     if (threadIdx.x == 0) s_G = s;
   }

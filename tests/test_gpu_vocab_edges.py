@@ -138,3 +138,38 @@ def test_head_gradient_of_masked_rows(voc, dtype, bias, rows):
             tol = err @ w[:, :H - 1].double().abs()
             want = G @ w[:, :H - 1].double()
             assert ((dh.double() - want).abs() <= tol + torch.finfo(dtype).eps * want.abs() + 1e-7).all()
+
+
+# ---- entries that are not given --------------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("rows", [40, 200])
+@pytest.mark.parametrize("value", [1e6, 1e30, INF, -INF, math.nan])
+def test_gradients_of_entries_not_given(voc, dtype, rows, value):
+    """Whatever the gradient of an entry that is not given (padded, or past the vocabulary), it changes no bit, the
+    scale of a float16 gradient included."""
+    from indecis_b200 import ops
+    V, H = 1003, 72
+    gen = torch.Generator(device="cuda").manual_seed(17)
+    h = torch.randn(rows, H, generator=gen, device="cuda").to(dtype)
+    w = (torch.randn(V, H, generator=gen, device="cuda") * 0.1).to(dtype)
+    ids = torch.randint(0, V, (rows, 4), generator=gen, device="cuda", dtype=torch.int32)
+    g = torch.randn((rows, 4), generator=gen, device="cuda") / rows
+    ids[3, 1] = -1
+    ids[7] = -5
+    ids[11, 3] = V
+    g[3] *= 100  # the row whose gradient sets the scale has an entry that is not given
+    gone = (ids < 0) | (ids >= V)
+    r = voc.vocab_logprobs(h, w, ids)
+    x = (h.float() @ w.float().T).to(dtype)
+    s = voc.token_logprobs(x, ids)
+    want = got = None
+    for v in (0.0, value):
+        gv = torch.where(gone, torch.full_like(g, v), g)
+        want, got = got, voc.vocab_logprobs_backward(h, w, ids, r.logprobs, r.lse, r.entropy, gv) + (
+            voc.token_logprobs_backward(x, ids, s.lse, s.entropy, gv),)
+    assert ops.device_error() == 5
+    for a, b in zip(got, want):
+        assert b.isfinite().all() and (b != 0).any()
+        assert torch.equal(a, b)
