@@ -398,9 +398,9 @@ struct TopShared {
   float wv[NT / 32];
   int wc[NT / 32];
 };
-// Unsigned integers in the order of the floats (no NaN).
+// Unsigned integers in the order of the floats (no NaN); -0 and +0 are one.
 __device__ __forceinline__ uint32_t order_key(float v) {
-  const uint32_t b = __float_as_uint(v);
+  const uint32_t b = v == 0.0f ? 0u : __float_as_uint(v);
   return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
 __device__ __forceinline__ float from_order_key(uint32_t k) {

@@ -173,3 +173,25 @@ def test_gradients_of_entries_not_given(voc, dtype, rows, value):
     for a, b in zip(got, want):
         assert b.isfinite().all() and (b != 0).any()
         assert torch.equal(a, b)
+
+
+# ---- alternatives ----------------------------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,V", [(2, 300), (3, 16384), (1, 70001), (9600, 257), (2400, 2049)])
+def test_top_ties_of_signed_zeros(voc, dtype, rows, V):
+    """-0 and +0 are the same value: the lowest column first."""
+    gen = torch.Generator(device="cuda").manual_seed(23)
+    none = torch.empty((rows, 0), dtype=torch.int32, device="cuda")
+    x = torch.full((rows, V), -1.0, device="cuda", dtype=dtype)
+    x[:, 0] = -0.0
+    x[:, 100] = 0.0
+    x[:, 200] = -0.0
+    assert voc.token_logprobs(x, none, top_k=1).top_ids[:, 0].tolist() == [0] * rows
+    assert voc.token_logprobs(x, none, top_k=3).top_ids.tolist() == [[0, 100, 200]] * rows
+    pick = torch.randint(0, 40, (rows, V), generator=gen, device="cuda")
+    x = torch.where(pick == 0, 0.0, torch.where(pick == 1, -0.0, -pick.float())).to(dtype)
+    for k in (1, 5, 32):
+        want = torch.sort(x.float() + 0.0, dim=1, descending=True, stable=True).indices[:, :k]
+        assert torch.equal(voc.token_logprobs(x, none, top_k=k).top_ids.long(), want)
