@@ -571,10 +571,11 @@ __global__ void __launch_bounds__(kVocThreads) vocab_join_kernel(const VJoinArgs
   __shared__ TopShared<kVocThreads> s_top[1];
   __shared__ float s_oval[kTopMax];
   __shared__ int s_ocol[kTopMax];
-  __shared__ int s_on;
+  __shared__ int s_on, s_left;
   const int64_t row = blockIdx.x;
   const int tid = (int)threadIdx.x, warp = tid >> 5, lane = tid & 31, nthreads = (int)blockDim.x;
   const float c2 = a.c * kLog2e;
+  if (tid == 0) s_left = 0;
   dep_wait();
   VStat st{-IG_INF, 0.0f, 0.0f};
   for (int p = tid; p < a.parts; p += nthreads) {
@@ -660,8 +661,11 @@ __global__ void __launch_bounds__(kVocThreads) vocab_join_kernel(const VJoinArgs
       if (d < a.T) {
         s_dot[d] = s;
       } else if (TOP && d < total) {
-        s_top[0].val[d - a.T] = id < a.V ? s : -IG_INF;
-        s_top[0].col[d - a.T] = id < a.V ? id : 0x7FFFFFFF;
+        // A masked column of a group is no alternative.
+        const bool left = id < a.V && s > -IG_INF;
+        s_top[0].val[d - a.T] = left ? s : -IG_INF;
+        s_top[0].col[d - a.T] = left ? id : 0x7FFFFFFF;
+        if (left) atomicAdd(&s_left, 1);
       }
     }
   }
@@ -690,8 +694,8 @@ __global__ void __launch_bounds__(kVocThreads) vocab_join_kernel(const VJoinArgs
         a.top_logprobs[row * a.K + r] = row_logprob(v, st, a.c, log_s);
       }
     }
-    // Past the columns (all groups are in the list then), or in a row that is no distribution.
-    for (int k = (nan ? 0 : min(cand, a.V)) + tid; k < a.K; k += nthreads) {
+    // Past the unmasked columns, or in a row that is no distribution.
+    for (int k = (nan ? 0 : s_left) + tid; k < a.K; k += nthreads) {
       a.top_ids[row * a.K + k] = -1;
       a.top_logprobs[row * a.K + k] = nan ? __int_as_float(0x7FC00000) : -IG_INF;
     }

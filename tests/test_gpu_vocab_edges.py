@@ -195,3 +195,31 @@ def test_top_ties_of_signed_zeros(voc, dtype, rows, V):
     for k in (1, 5, 32):
         want = torch.sort(x.float() + 0.0, dim=1, descending=True, stable=True).indices[:, :k]
         assert torch.equal(voc.token_logprobs(x, none, top_k=k).top_ids.long(), want)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("rows", [3, 150])
+@pytest.mark.parametrize("left", [[], [5], [19], [0, 17, 18], [3, 40, 41, 42, 43, 44, 45, 999], list(range(16))])
+def test_head_alternatives_of_masked_columns(voc, dtype, rows, left):
+    """Tokens masked by a bias of -inf are no alternatives: past the unmasked ones, -1 and -inf."""
+    V, H, K = 1000, 72, 8
+    bias = torch.full((V,), -INF)
+    bias[left] = 0.0
+    h, w = biased(rows, V, H, dtype, 171, bias.cuda())
+    h, w = h.contiguous(), w.contiguous()
+    ids = torch.tensor([[5, 700]] * rows, dtype=torch.int32, device="cuda")
+    for _ in range(2):
+        junk = torch.full((1 << 16,), 7, dtype=torch.int32, device="cuda")  # what a forgotten output would show
+        del junk
+        r = voc.vocab_logprobs(h, w, ids, top_k=K)
+        n = min(K, len(left))
+        if not left:
+            assert (r.lse == -INF).all() and (r.entropy == 0).all() and (r.logprobs == -INF).all()
+        else:
+            keep = torch.tensor(left, device="cuda")
+            logp = torch.log_softmax(h.double()[:, :H - 1] @ w.double()[keep][:, :H - 1].T, 1)
+            v, at = torch.sort(logp, dim=1, descending=True, stable=True)
+            assert torch.equal(r.top_ids[:, :n].long(), keep[at[:, :n]])
+            close(r.top_logprobs[:, :n], v[:, :n], STAT_TOL + 1e-4)
+            assert (r.logprobs[:, 1] == -INF).all()
+        assert (r.top_ids[:, n:] == -1).all() and (r.top_logprobs[:, n:] == -INF).all()
