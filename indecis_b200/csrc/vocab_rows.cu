@@ -1349,6 +1349,15 @@ static RowShape row_shape(int64_t rows, int64_t nv, bool again) {
   return r;
 }
 
+// The tail's marks, a byte per vector of a CTA's part: at most this many, with
+// which two CTAs of 256 threads share an SM beside their slots. With a gradient
+// the rule above leaves less in any case; for the loss alone the marks of a
+// whole row of 2^20 float32 columns are more than an SM has. Loss of 1184 rows,
+// one CTA each and by this rule: 450000 float32 columns (112 KB of marks) 386
+// and 332 us, 600000 (150 KB) 502 and 430; below it the clusters only cost
+// (262144 bf16 columns, 32 KB: 104 us, and 126 in two parts).
+constexpr int64_t kMarkBytes = 74 << 10;
+
 template <typename Args>
 static cudaError_t launch_rows(void (*kern)(Args), const Args &a, int64_t ctas, int threads, int cs, size_t smem,
                                cudaStream_t st, SmemOptIn &attr) {
@@ -1423,7 +1432,8 @@ static cudaError_t launch_distill(const DistillArgs &a, size_t smem, cudaStream_
 template <int DT>
 static cudaError_t run_distill(DistillArgs a, bool tail, cudaStream_t st) {
   const int64_t nv = a.V / VElem<DT>::kN + 2;
-  const RowShape r = row_shape(a.rows, a.V / VElem<DT>::kN, a.dx != nullptr);
+  RowShape r = row_shape(a.rows, a.V / VElem<DT>::kN, a.dx != nullptr);
+  while (tail && r.threads == kVocThreads && r.parts < 8 && nv / r.parts > kMarkBytes) r.parts *= 2;
   a.parts = r.parts;
   const size_t smem = tail ? ((nv / r.parts + 1) / 4 + 1) * 4 : 0;
 #define IG_CALL(NT) (tail ? launch_distill<DT, true, NT>(a, smem, st) : launch_distill<DT, false, NT>(a, smem, st))

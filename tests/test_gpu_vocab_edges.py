@@ -223,3 +223,38 @@ def test_head_alternatives_of_masked_columns(voc, dtype, rows, left):
             close(r.top_logprobs[:, :n], v[:, :n], STAT_TOL + 1e-4)
             assert (r.logprobs[:, 1] == -INF).all()
         assert (r.top_ids[:, n:] == -1).all() and (r.top_logprobs[:, n:] == -INF).all()
+
+
+# ---- distillation ----------------------------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("dtype,V", [(torch.float32, 1 << 20), (torch.float32, 300001), (torch.bfloat16, 1 << 20)])
+def test_tail_loss_of_many_long_rows(voc, dtype, V):
+    """The tail's loss without a gradient: rows enough that each would have one CTA, columns enough that their marks
+    do not fit into one CTA's shared memory."""
+    rows = 8 * torch.cuda.get_device_properties(0).multi_processor_count
+    gen = torch.Generator(device="cuda").manual_seed(29)
+    x = torch.empty((rows, V), dtype=dtype, device="cuda")
+    x.normal_(generator=gen)
+    ids = torch.randint(0, V, (rows, 40), generator=gen, device="cuda", dtype=torch.int32)
+    ids[3, 30:] = -1
+    ids[4] = -1
+    t = torch.log_softmax(torch.randn((rows, 41), generator=gen, device="cuda"), 1)[:, :40].contiguous()
+    loss, none = voc.distill_topk(x, ids, t, tail=True, grad=False)
+    assert none is None
+    for n in (0, 3, 4, rows - 1):
+        logp = torch.log_softmax(x[n].double(), 0)
+        at, first = {}, {}
+        for k, i in enumerate(ids[n].tolist()):
+            if i >= 0:
+                at.setdefault(i, []).append(float(t[n, k]))
+        if not at:
+            assert loss[n] == 0
+            continue
+        lp = logp[torch.tensor(list(at), device="cuda")].tolist()
+        want = sum(math.exp(v) * (v - l) for l, vs in zip(lp, at.values()) for v in vs)
+        rest = 1 - sum(math.exp(v) for vs in at.values() for v in vs)
+        want += rest * (math.log(rest) - math.log1p(-sum(math.exp(l) for l in lp)))
+        assert abs(float(loss[n]) - want) <= 4 * 7e-5 * (1 + abs(want))
+    more, _ = voc.distill_topk(x, ids, t, tail=True, out=x)
+    close(more, loss.double(), 4 * 7e-5)
