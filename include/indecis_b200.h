@@ -355,7 +355,8 @@ IG_API int ig_token_logprobs(const void *logits, int32_t dtype, int64_t ld, int6
  * Zero for a row of -inf only. lse gives p as far as float32 holds it; for
  * |lse| > 1024 (a row wholly masked by a finite value, a large offset, a very
  * low temperature) the row's maximum and sum are formed again from the logits.
- * dlogits may be logits (with ldd = ld). */
+ * dlogits may be logits (with ldd = ld); one that shares only some of its
+ * elements is refused. */
 IG_API int ig_token_logprobs_backward(const void *logits, int32_t dtype, int64_t ld, int64_t rows, int32_t vocab,
                                       double temperature, const int32_t *ids, int32_t nids, const float *lse,
                                       const float *entropy, const float *dlogprobs, const float *dentropy,
@@ -370,11 +371,11 @@ IG_API int ig_token_logprobs_backward(const void *logits, int32_t dtype, int64_t
  *   loss[r] = w (sum q (log q - log p) + q_rest (log q_rest - log p_rest))
  *   (left out where the row has no unmasked column outside the list).
  * w = weights[r] (NULL: 1), the row's share of the total: dlogits (NULL: loss
- * only; may be logits, with ldd = ld) is the gradient of sum_r loss[r]. A row
- * with weight 0 or without entries: loss 0 and gradient 0. A row of -inf
- * only: loss +inf, gradient 0; one with NaN or +inf: NaN. vocab <= 2^20 with
- * the tail (IG_ERR_UNSUPPORTED). Ids >= vocab count as missing and leave
- * device error 5. */
+ * only; may be logits, with ldd = ld, as above) is the gradient of
+ * sum_r loss[r]. A row with weight 0 or without entries: loss 0 and gradient
+ * 0. A row of -inf only: loss +inf, gradient 0; one with NaN or +inf: NaN.
+ * vocab <= 2^20 with the tail (IG_ERR_UNSUPPORTED). Ids >= vocab count as
+ * missing and leave device error 5. */
 IG_API int ig_distill_topk(const void *logits, int32_t dtype, int64_t ld, int64_t rows, int32_t vocab,
                            double temperature, const int32_t *teacher_ids, const float *teacher_logits, int32_t k,
                            int32_t tail, const float *weights, float *loss, void *dlogits, int64_t ldd, void *stream);
@@ -400,7 +401,8 @@ IG_API int ig_vocab_logprobs(const void *hidden, int64_t ldh, const void *weight
 /* Its gradient with respect to hidden and weight (either may be NULL), from
  * the forward's logprobs, lse and entropy: with G the gradient
  * ig_token_logprobs_backward gives for the logits, dhidden = G . weight and
- * dweight = G^T . hidden, in the operands' type, strides free. G is formed
+ * dweight = G^T . hidden, in the operands' type, strides free, apart from the
+ * operands and from one another. G is formed
  * in the workspace in column chunks and rounded to the operands' type (for
  * float16 scaled by a power of two, so that small probabilities keep their
  * bits); the sums are float32 in a fixed order. p = exp(min(z - lse, 0)), off

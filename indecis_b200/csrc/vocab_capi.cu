@@ -19,6 +19,44 @@ static const char *bad_matrix(const void *p, int64_t rows, int64_t cols, int64_t
   return nullptr;
 }
 
+// A matrix's rows as intervals of addresses: `width` bytes each, `stride` >= width apart.
+struct RowSpan {
+  uintptr_t at;
+  int64_t rows, stride, width;
+  RowSpan(const void *p, int64_t rows_, int64_t cols, int64_t ld, int es)
+      : at(reinterpret_cast<uintptr_t>(p)), rows(p ? rows_ : 0), stride(ld * es), width(cols * es) {}
+  uintptr_t end() const { return at + (uintptr_t)((rows - 1) * stride + width); }
+};
+// Whether two matrices share a byte (rows of one may lie between those of the other).
+static bool overlap(const RowSpan &p, const RowSpan &q) {
+  if (p.rows <= 0 || q.rows <= 0 || p.end() <= q.at || q.end() <= p.at) return false;
+  const RowSpan &a = p.at <= q.at ? p : q, &b = p.at <= q.at ? q : p;
+  if (a.stride == b.stride) {
+    // b's first row starts in a's row k, `r` bytes from its start; all later pairs of rows are alike.
+    const int64_t k = (int64_t)((b.at - a.at) / a.stride), r = (int64_t)((b.at - a.at) % a.stride);
+    return (k < a.rows && r < a.width) || (k + 1 < a.rows && r + b.width > a.stride);
+  }
+  uintptr_t x = a.at, y = b.at;
+  for (int64_t i = 0, j = 0; i < a.rows && j < b.rows;) {
+    if (x + a.width <= y) {
+      i++;
+      x += a.stride;
+    } else if (y + b.width <= x) {
+      j++;
+      y += b.stride;
+    } else {
+      return true;
+    }
+  }
+  return false;
+}
+// Logits' gradient in place of the logits, or apart from them.
+static const char *bad_in_place(const void *x, int64_t ld, const void *d, int64_t ldd, int64_t rows, int64_t cols, int es) {
+  if (x == d) return ld != ldd ? "in place, both row strides must be the same" : nullptr;
+  return overlap(RowSpan(x, rows, cols, ld, es), RowSpan(d, rows, cols, ldd, es))
+             ? "the gradient may replace the logits, but not overlap them" : nullptr;
+}
+
 static const char *bad_row_args(int64_t rows, int64_t vocab, int32_t nids, const void *ids, const float *io, double t) {
   if (rows < 0 || vocab < 1 || nids < 0) return "negative or empty size";
   if (vocab > (1 << 30) || rows > (int64_t)INT32_MAX / 8) return "too many rows or columns";
@@ -84,9 +122,8 @@ int ig_token_logprobs_backward(const void *logits, int32_t dtype, int64_t ld, in
   const char *m = bad_matrix(logits, rows, vocab, ld, es);
   if (!m) m = bad_matrix(dlogits, rows, vocab, ldd, es);
   if (!m && rows > 0 && (!lse || (dentropy && !entropy))) m = "null argument";
+  if (!m) m = bad_in_place(logits, ld, dlogits, ldd, rows, vocab, es);
   if (m) return fail(IG_ERR_BAD_ARG, std::string("ig_token_logprobs_backward: ") + m);
-  if (logits == dlogits && ld != ldd)
-    return fail(IG_ERR_BAD_ARG, "ig_token_logprobs_backward: in place, both row strides must be the same");
   if (rows == 0) return 0;
   LogprobGradArgs a{logits, ld, rows, vocab, nids, 1, (float)(1.0 / temperature), ids, lse, entropy,
                     nids > 0 ? dlogprobs : nullptr, dentropy, dlogits, ldd};
@@ -108,10 +145,11 @@ int ig_distill_topk(const void *logits, int32_t dtype, int64_t ld, int64_t rows,
   if (!m) m = bad_matrix(logits, rows, vocab, ld, es);
   if (!m && dlogits) m = bad_matrix(dlogits, rows, vocab, ldd, es);
   if (!m && rows > 0 && !loss) m = "null argument";
-  if (!m && dlogits && logits == dlogits && ld != ldd) m = "in place, both row strides must be the same";
   if (m) return fail(IG_ERR_BAD_ARG, std::string("ig_distill_topk: ") + m);
   if (tail && vocab > (1 << 20))
     return fail(IG_ERR_UNSUPPORTED, "ig_distill_topk: with the tail, at most 1048576 columns");
+  if (dlogits && (m = bad_in_place(logits, ld, dlogits, ldd, rows, vocab, es)))
+    return fail(IG_ERR_BAD_ARG, std::string("ig_distill_topk: ") + m);
   if (rows == 0) return 0;
   DistillArgs a{logits, ld, rows, vocab, k, (float)(1.0 / temperature), teacher_ids, teacher_logits, weights, loss,
                 dlogits, ldd, 1};
@@ -173,7 +211,12 @@ int ig_vocab_logprobs_backward(const void *hidden, int64_t ldh, const void *weig
   if (!m && dhidden) m = bad_matrix(dhidden, rows, hidden_size, lddh, 2);
   if (!m && dweight) m = bad_matrix(dweight, vocab, hidden_size, lddw, 2);
   if (!m && rows > 0 && (!lse || (nids > 0 && !logprobs) || (dentropy && !entropy))) m = "null argument";
-  if (!m && ((dhidden && dhidden == hidden) || (dweight && dweight == weight))) m = "the gradients cannot replace the operands";
+  if (!m) {
+    const RowSpan h(hidden, rows, hidden_size, ldh, 2), w(weight, vocab, hidden_size, ldw, 2),
+        dh(dhidden, rows, hidden_size, lddh, 2), dw(dweight, vocab, hidden_size, lddw, 2);
+    if (overlap(dh, h) || overlap(dh, w) || overlap(dw, h) || overlap(dw, w) || overlap(dh, dw))
+      m = "the gradients cannot overlap the operands or one another";
+  }
   if (m) return fail(IG_ERR_BAD_ARG, std::string("ig_vocab_logprobs_backward: ") + m);
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   if (!dhidden && !dweight) return 0;

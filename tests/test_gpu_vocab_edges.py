@@ -258,3 +258,29 @@ def test_tail_loss_of_many_long_rows(voc, dtype, V):
         assert abs(float(loss[n]) - want) <= 4 * 7e-5 * (1 + abs(want))
     more, _ = voc.distill_topk(x, ids, t, tail=True, out=x)
     close(more, loss.double(), 4 * 7e-5)
+
+
+# ---- where the gradient may go -----------------------------------------------------------------------------------------
+
+
+def test_gradient_between_the_logits_rows(voc):
+    """Rows of the output between those of the logits share nothing with them; an output that does is refused."""
+    from indecis_b200 import _capi
+    V = 1003
+    buf = torch.empty((70, 2 * V + 5), device="cuda")
+    x, out = buf[:, :V], buf[:, V + 2:2 * V + 2]
+    x.copy_(make(70, V, torch.float32, 181))
+    ids = torch.arange(70, dtype=torch.int32, device="cuda")[:, None].contiguous()
+    r = voc.token_logprobs(x, ids)
+    g = torch.ones_like(r.logprobs)
+    want = voc.token_logprobs_backward(x, ids, r.lse, r.entropy, g)
+    assert torch.equal(voc.token_logprobs_backward(x, ids, r.lse, r.entropy, g, out=out), want)
+    t = torch.zeros((70, 1), device="cuda")
+    want = voc.distill_topk(x, ids, t)[1]
+    assert torch.equal(voc.distill_topk(x, ids, t, out=out)[1], want)
+    for bad in (buf[:, 1:V + 1], buf[:, V - 1:2 * V - 1]):
+        for call in (lambda: voc.token_logprobs_backward(x, ids, r.lse, r.entropy, g, out=bad),
+                     lambda: voc.distill_topk(x, ids, t, out=bad)):
+            with pytest.raises(_capi.IgError) as e:
+                call()
+            assert e.value.code == _capi.IG_ERR_BAD_ARG
