@@ -7,7 +7,7 @@ import math
 import pytest
 import torch
 
-from test_gpu_vocab import DTYPES, EPS, INF, P_TOL, STAT_TOL, TINY, close, make, ref_gradient
+from test_gpu_vocab import DTYPES, EPS, INF, P_TOL, STAT_TOL, TINY, close, make, ref_distill, ref_gradient
 
 pytestmark = pytest.mark.gpu
 
@@ -284,3 +284,65 @@ def test_gradient_between_the_logits_rows(voc):
             with pytest.raises(_capi.IgError) as e:
                 call()
             assert e.value.code == _capi.IG_ERR_BAD_ARG
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("rows", [7, 300])
+def test_head_gradient_with_masked_columns(voc, dtype, rows):
+    """Tokens masked by a bias of -inf, given ones among them: no probability, no gradient but a given token's own. (The
+    bias column's own entry of dhidden is 0 times infinity.) Tolerances as in test_gpu_vocab_head.check_backward."""
+    V, H = 1500, 72
+    bias = torch.zeros(V)
+    bias[::3] = -INF
+    h, w = biased(rows, V, H, dtype, 191, bias.cuda())
+    gen = torch.Generator(device="cuda").manual_seed(6)
+    ids = torch.randint(0, V, (rows, 3), generator=gen, device="cuda", dtype=torch.int32)
+    g = torch.randn((rows, 3), generator=gen, device="cuda")
+    gh = torch.randn((rows,), generator=gen, device="cuda")
+    r = voc.vocab_logprobs(h, w, ids)
+    assert ((r.logprobs == -INF) == (ids % 3 == 0)).all()
+    dh, dw = voc.vocab_logprobs_backward(h, w, ids, r.logprobs, r.lse, r.entropy, g, gh)
+    hd, wd = h.double()[:, :H - 1], w.double()[:, :H - 1]
+    z = hd @ wd.T + bias.cuda().double()
+    logp = torch.log_softmax(z, 1)
+    p = logp.exp()
+    ent = torch.special.entr(p).sum(1, keepdim=True)
+    G = -g.double().sum(1, keepdim=True) * p
+    G -= gh.double()[:, None] * torch.where(p > 0, p * (logp + ent), torch.zeros_like(p))
+    G.scatter_add_(1, ids.long(), g.double())
+    slack = (g.double().abs().sum(1, keepdim=True) + gh.double().abs()[:, None] * 40) * p
+    off = 2 * 2.0**-20 * float((hd.abs() @ wd.abs().T).max())
+    u = torch.finfo(dtype).eps / 2
+    floor = float((2 * g.abs().sum(1) + gh.abs() * 10).max()) * 2.0**-39 if dtype == torch.float16 else 0.0
+    err = u * 1.01 * G.abs() + slack * (P_TOL + off) + floor
+    tiny = 3e-8 if dtype == torch.float16 else 0.0
+    want = G @ wd
+    tol = err @ wd.abs() + 2.0**-20 * (G.abs() @ wd.abs()) + u * 1.01 * want.abs() + tiny
+    assert ((dh[:, :H - 1].double() - want).abs() <= tol).all()
+    want = G.T @ h.double()
+    tol = err.T @ h.double().abs() + 2.0**-20 * (G.abs().T @ h.double().abs()) + u * 1.01 * want.abs() + tiny
+    assert ((dw.double() - want).abs() <= tol).all()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("tail", [False, True])
+@pytest.mark.parametrize("rows,V", [(8, 37), (8, 70001), (2400, 2049)])
+def test_distill_of_masked_rows(voc, dtype, tail, rows, V):
+    """Rows wholly masked by a finite value are uniform."""
+    x = make(rows, V, dtype, 201 + V)
+    values = [v for v in (-1e4, -1e9, -1e30, torch.finfo(dtype).min) if abs(v) <= torch.finfo(dtype).max]
+    for i, v in enumerate(values):
+        x[2 * i] = v
+    gen = torch.Generator(device="cuda").manual_seed(6)
+    ids = torch.rand((rows, V), generator=gen, device="cuda").topk(6, dim=1).indices.int().contiguous()
+    t = torch.log_softmax(torch.randn((rows, 7), generator=gen, device="cuda"), 1)[:, :6].contiguous()
+    for temperature in (0.5, 1.0, 8.0):
+        loss, d = voc.distill_topk(x, ids, t, temperature=temperature, tail=tail)
+        wl, wd, p, q = ref_distill(x, ids, t, temperature, tail, None)
+        close(loss, wl, 4 * STAT_TOL, "loss")
+        tol = (P_TOL * wd.abs() + 1e-6 * p + 4e-7) / min(temperature, 1.0) + EPS[dtype] / 2 * wd.abs() * 1.01 + TINY[dtype]
+        if tail:
+            listed = torch.zeros_like(p, dtype=torch.bool).scatter_(1, ids.long(), True)
+            mass = torch.where(listed, torch.zeros_like(p), p).sum(1).clamp(min=1e-300)
+            tol = tol + (p * ((P_TOL * (1 - q.sum(1)).clamp(min=0) + 5e-7) / mass)[:, None]).clamp(max=1.0) / temperature
+        assert ((d.double() - wd).abs() <= tol).all()
