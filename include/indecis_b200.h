@@ -341,7 +341,8 @@ IG_API int ig_attention_noalloc(const float *qkv, int32_t hidden, int32_t heads,
  * (either may be NULL), top_ids/top_logprobs[r][top_k] the columns of the
  * largest logits (ties: the lowest column first). A negative id is not given:
  * 0. An id >= vocab gives NaN and device error 5. -inf masks a column. A row
- * of -inf only: lse and logprobs -inf, entropy 0. Past the unmasked columns:
+ * of -inf only: lse and logprobs -inf, entropy 0 (lse is -FLT_MAX, not -inf,
+ * where other columns are left but z is past float32). Past the unmasked columns:
  * alternative -1, -inf. A row with NaN or +inf: NaN (alternatives -1). */
 IG_API int ig_token_logprobs(const void *logits, int32_t dtype, int64_t ld, int64_t rows, int32_t vocab,
                              double temperature, const int32_t *ids, int32_t nids, float *logprobs, float *lse,
@@ -408,7 +409,7 @@ IG_API int ig_vocab_logprobs(const void *hidden, int64_t ldh, const void *weight
  * bits); the sums are float32 in a fixed order. p = exp(min(z - lse, 0)), off
  * by |lse| 2^-24 of itself through lse's rounding; in a row whose lse float32
  * does not resolve (wholly masked by a bias past 2^22, say) the columns within
- * a step of the maximum have p = 1. */
+ * a step of the maximum have p = 1. Zero for a row with lse -inf or -FLT_MAX. */
 IG_API int ig_vocab_logprobs_backward(const void *hidden, int64_t ldh, const void *weight, int64_t ldw, int32_t dtype,
                                       int64_t rows, int32_t vocab, int32_t hidden_size, double temperature,
                                       const int32_t *ids, int32_t nids, const float *logprobs, const float *lse,

@@ -742,7 +742,8 @@ __global__ void vocab_coef_kernel(const VCoefArgs a) {
   if (lane) return;
   const float gh = a.dentropy ? a.dentropy[row] : 0.0f, H = a.dentropy ? a.entropy[row] : 0.0f;
   const float lse = a.lse[row];
-  const RowCoef k = row_coef(lse, H, G, gh, a.c);
+  // An lse at float32's end says nothing of the columns either.
+  const RowCoef k = row_coef(lse == -kFltMax ? -IG_INF : lse, H, G, gh, a.c);
   a.coef[row] = VRowCoef{k.A, k.B, k.l, 0.0f};
   // |dZ| <= c (sum |g| (1 + p) + |gH| p (|log p| + H)) <= c (2 sum |g| + |gH| (1 + H)), as p <= 1
   const float b = a.c * (2.0f * size + fabsf(gh) * (1.0f + H));

@@ -27,6 +27,7 @@ constexpr int kIdsMax = 256;      // given tokens or teacher entries per row
 constexpr float kLog2e = 1.44269504088896340736f;
 constexpr float kLn2 = 0.69314718055994530942f;
 constexpr float kYMin = -1.0e4f;  // 2^kYMin = 0
+constexpr float kFltMax = 3.402823466e38f;
 #define IG_INF __int_as_float(0x7f800000)
 
 __device__ __forceinline__ float ex2(float y) {
@@ -555,7 +556,8 @@ struct LogprobArgs {
 __device__ __forceinline__ void row_lse(const VStat &a, float c, float &log_s, float &lse, float &entropy) {
   const bool empty = a.s == 0.0f;
   log_s = logf(a.s);
-  lse = empty ? -IG_INF : fmaf(a.m, c, log_s);
+  // -inf stands for an empty row alone (NaN is kept).
+  lse = empty ? -IG_INF : max_nan(fmaf(a.m, c, log_s), -kFltMax);
   entropy = empty ? 0.0f : log_s - kLn2 * (a.u / a.s);
   if (entropy < 0.0f) entropy = 0.0f;
 }
@@ -859,10 +861,11 @@ __device__ __forceinline__ void given_grads(typename VElem<DT>::T *drow, const i
 // The largest |lse| that the gradient is formed from: float32 holds it to
 // |lse| 2^-24, 6e-5 at most, which is the relative error of p. Past it (a row
 // wholly masked by a finite value, logits at a large offset, a very low
-// temperature; also -inf, which the product with 1 / temperature gives for
-// large finite masks) one CTA takes the whole row and its maximum and sum
-// again, as the forward has them: 120 us where 2047 x 50021 bf16 takes 73 from
-// lse, 372 and 263 for 4096 x 50021 float32, 66 and 15 for 16 x 262144.
+// temperature) one CTA takes the whole row and its maximum and sum again, as
+// the forward has them: 111 us where 2047 x 50021 bf16 takes 70 from lse, 368
+// and 259 for 4096 x 50021 float32, 72 and 10 for 16 x 262144. (The row's CTAs
+// as a cluster take 19 us for the last, but the launch as clusters costs the
+// ordinary rows: 103 and 49 us for 16384 x 4096 bf16.)
 constexpr float kLseMost = 1024.0f;
 
 template <int DT, int NT>
@@ -971,7 +974,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT) token_logprobs_grad_kernel(cons
   const int cfirst = max(rv.col(rp.v0), 0), clast = min(rv.col(rp.v1), a.V);
   if (a.dlogprobs) given_logits<DT, NT>(rv.row, ids, a.T, cfirst, clast, s_xt);
   __syncthreads();
-  if (!(fabsf(lse) <= kLseMost)) {
+  if (fabsf(lse) > kLseMost && lse != -IG_INF) {
     cp_async_wait_all();
     if (seg == 0) grad_whole_row<DT, NT>(a, row, s_G, H, gh, s_ahead, s_xt, s_warp);
     return;
@@ -1002,7 +1005,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT) token_logprobs_grad_kernel(cons
     grad(edge, d);
     store_edge<DT>(drow, rv, threadIdx.x == kFirstThread ? rp.v0 : rp.v1 - 1, d);
   }
-  if (a.T == 0 || !a.dlogprobs) return;
+  if (a.T == 0 || !a.dlogprobs || k.l == IG_INF) return;
   __syncthreads();
   given_grads<DT, NT>(drow, ids, g, a.T, cfirst, clast, s_xt, 0.0f, a.c, k);
 }

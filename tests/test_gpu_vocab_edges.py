@@ -60,7 +60,7 @@ def test_gradient_of_masked_rows(voc, dtype, rows, V, pad, shift):
         gradient_close(y, x, ids, g, gh, temperature)
 
 
-@pytest.mark.parametrize("rows,V", [(7, 4099), (3, 262145), (2400, 1025)])
+@pytest.mark.parametrize("rows,V", [(7, 4099), (3, 10007), (5, 27001), (3, 262145), (2400, 1025)])
 @pytest.mark.parametrize("offset,temperature", [(-5000.0, 1.0), (20000.0, 1.0), (1e6, 3.0), (0.0, 0.005)])
 def test_gradient_far_from_zero(voc, rows, V, offset, temperature):
     """float32 logits at a large offset, or scaled by a low temperature: the gradient does not lose the bits that the
@@ -346,3 +346,28 @@ def test_distill_of_masked_rows(voc, dtype, tail, rows, V):
             mass = torch.where(listed, torch.zeros_like(p), p).sum(1).clamp(min=1e-300)
             tol = tol + (p * ((P_TOL * (1 - q.sum(1)).clamp(min=0) + 5e-7) / mass)[:, None]).clamp(max=1.0) / temperature
         assert ((d.double() - wd).abs() <= tol).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("top", [0, 3])
+def test_lse_says_whether_a_row_is_empty(voc, dtype, top):
+    """-inf for a row with nothing left alone, also where the product with 1 / temperature leaves float32."""
+    x = make(4, 3001, dtype, 211)
+    x[0] = -INF
+    x[1] = torch.finfo(dtype).min
+    x[2] = -INF
+    x[2, 7] = torch.finfo(dtype).min
+    ids = torch.tensor([[7, 8]] * 4, dtype=torch.int32, device="cuda")
+    r = voc.token_logprobs(x, ids, temperature=0.5, top_k=top)
+    assert r.lse[0] == -INF and r.lse[1:].isfinite().all()
+    assert r.logprobs[0].tolist() == [-INF, -INF] and r.logprobs[2].tolist() == [0.0, -INF]
+    g = torch.tensor([[1.0, 0.5]] * 4, device="cuda")
+    d = voc.token_logprobs_backward(x, ids, r.lse, r.entropy, g, temperature=0.5)
+    assert (d[0] == 0).all()
+    want = torch.full((3001,), -3.0 / 3001, device="cuda", dtype=torch.float64)
+    want[7] += 2.0
+    want[8] += 1.0
+    assert ((d[1].double() - want).abs() <= 4 * P_TOL / 3001 + EPS[dtype] * want.abs()).all()
+    want = torch.zeros(3001, device="cuda", dtype=torch.float64)
+    want[7], want[8] = -1.0, 1.0  # all of p in column 7: (1 - 1.5) / 0.5; the other given one has none
+    assert ((d[2].double() - want).abs() <= 1e-6 + EPS[dtype] * want.abs()).all()
