@@ -64,6 +64,27 @@ struct VRowCoef {
 };
 
 constexpr int kVGroup = 16;  // columns per stored maximum
+// At most this many given tokens a row: their logits are taken from the
+// accumulators, as the statistics are. The tensor cores' sums are cut off, not
+// rounded (a logit of 10 from 1000 terms comes out 1e-5 low), so a logit summed
+// in another way does not match them: the log probability of a token that
+// takes most of its row, -0.13 in the mean, was off by 6e-5 of itself.
+// More tokens' logits are dot products in the joining kernel, as a row's look-up
+// grows with their number: 4096 x 65536 x 256 takes 150 us with dot products,
+// 152 with one token caught, 160 with eight; with more, most are not the
+// likeliest of their row.
+constexpr int kVCaught = 8;
+// The lowest of a row's given tokens that is at least `from` and lies in the
+// columns of epilogue group g.
+__device__ __forceinline__ int next_given(const int32_t *ids, int T, int from, int g) {
+  int m = 0x7FFFFFFF;
+#pragma unroll
+  for (int t = 0; t < kVCaught; t++) {
+    const int id = t < T ? ids[t] : -1;
+    if (id >= from && id < m && id / kVEpiCols % kVEpiGroups == g) m = id;
+  }
+  return m;
+}
 
 struct VGemmArgs {
   int M, N;
@@ -79,6 +100,9 @@ struct VGemmArgs {
   float4 *part;
   float *gmax;
   int64_t ldmax;
+  const int32_t *ids;  // [M][T]: their logits go to xid [M][T]; T = 0: none
+  int T;
+  float *xid;
   // kVDz
   const VRowCoef *coef;
   int split;  // dZ as two 16-bit parts, the second `shift` elements on
@@ -357,6 +381,10 @@ __global__ void __launch_bounds__(kVGemmThreads, 1)
       const int row0 = q.m * (CG * 128) + rank * 128 + q4 * 32, row = row0 + lane;
       const bool warp_live = row0 < a.M, live = row < a.M;
       [[maybe_unused]] VStat st{-IG_INF, 0.0f, 0.0f};
+      [[maybe_unused]] int next = 0x7FFFFFFF;  // the row's next given column to catch
+      if constexpr (EPI == kVStats) {
+        if (live && a.T > 0) next = next_given(a.ids + (int64_t)row * a.T, a.T, q.n0 * kVBN, g);
+      }
       [[maybe_unused]] RowCoef rc{0.0f, 0.0f, 0.0f};
       [[maybe_unused]] bool hold = false;
       if constexpr (EPI == kVDz) {
@@ -419,6 +447,17 @@ __global__ void __launch_bounds__(kVGemmThreads, 1)
 #pragma unroll
               for (int k = 0; k < 32; k++)
                 if (col0 + k >= a.N) x[k] = -IG_INF;
+            }
+            while (next < col0 + 32) {  // seldom
+              const int32_t *ids = a.ids + (int64_t)row * a.T;
+              const int at = next - col0;
+              float v = x[0];
+#pragma unroll
+              for (int k = 1; k < 32; k++) v = at == k ? x[k] : v;
+#pragma unroll
+              for (int t = 0; t < kVCaught; t++)
+                if (t < a.T && ids[t] == next) a.xid[(int64_t)row * a.T + t] = v;
+              next = next_given(ids, a.T, next + 1, g);
             }
             float m4[4] = {x[0], x[1], x[16], x[17]};
 #pragma unroll
@@ -564,6 +603,7 @@ struct VJoinArgs {
   float c;
   const int32_t *ids;
   const float4 *part;
+  const float *xid;  // the given tokens' logits, or NULL: dot products here
   const float *gmax;
   int64_t ldmax;
   int ngroups;
@@ -573,9 +613,10 @@ struct VJoinArgs {
 };
 
 // One CTA per row: the statistics of the row's parts, then the dot products of
-// the given tokens and of the best groups' columns, eight lanes each (128
-// bytes of either operand a step). A logit summed here is float32 in another
-// order than the tensor core's.
+// the given tokens (where they are many) and of the best groups' columns, eight
+// lanes each (128 bytes of either operand a step). A logit summed here is
+// float32 in another order than the tensor core's, so the alternatives are
+// counted from the best of them, not from the statistics' maximum.
 template <bool TOP>
 __global__ void __launch_bounds__(kVocThreads) vocab_join_kernel(const VJoinArgs a) {
   __shared__ VStat s_warp[kVocWarps];
@@ -589,6 +630,8 @@ __global__ void __launch_bounds__(kVocThreads) vocab_join_kernel(const VJoinArgs
   const float c2 = a.c * kLog2e;
   if (tid == 0) s_left = 0;
   dep_wait();
+  float xid = 0.0f;  // asked for early
+  if (a.xid && tid < a.T) xid = a.xid[row * a.T + tid];
   VStat st{-IG_INF, 0.0f, 0.0f};
   for (int p = tid; p < a.parts; p += nthreads) {
     const float4 v = a.part[row * a.parts + p];
@@ -626,16 +669,17 @@ __global__ void __launch_bounds__(kVocThreads) vocab_join_kernel(const VJoinArgs
     if (a.lse) a.lse[row] = lse;
     if (a.entropy) a.entropy[row] = entropy;
   }
-  const int cand = s_on * kVGroup, total = a.T + cand;
+  const int given = a.xid ? 0 : a.T, cand = s_on * kVGroup, total = given + cand;
   const uint16_t *h = a.h + row * a.ldh;
   const int sub = tid & 7;
+  [[maybe_unused]] float best = -IG_INF;  // of the alternatives
   for (int d0 = 0; d0 < total; d0 += nthreads / 8) {
     const int d = d0 + (tid >> 3);
     int id = -1;
-    if (d < a.T)
+    if (d < given)
       id = a.ids[row * a.T + d];
     else if (d < total)
-      id = s_ocol[(d - a.T) / kVGroup] * kVGroup + (d - a.T) % kVGroup;
+      id = s_ocol[(d - given) / kVGroup] * kVGroup + (d - given) % kVGroup;
     float s = 0.0f;
     if (id >= 0 && id < a.V) {
       const uint16_t *w = a.w + (int64_t)id * a.ldw;
@@ -670,16 +714,23 @@ __global__ void __launch_bounds__(kVocThreads) vocab_join_kernel(const VJoinArgs
 #pragma unroll
     for (int o = 4; o; o >>= 1) s += __shfl_xor_sync(~0u, s, o);
     if (sub == 0) {
-      if (d < a.T) {
+      if (d < given) {
         s_dot[d] = s;
       } else if (TOP && d < total) {
         // A masked column of a group is no alternative.
         const bool left = id < a.V && s > -IG_INF;
-        s_top[0].val[d - a.T] = left ? s : -IG_INF;
-        s_top[0].col[d - a.T] = left ? id : 0x7FFFFFFF;
-        if (left) atomicAdd(&s_left, 1);
+        s_top[0].val[d - given] = left ? s : -IG_INF;
+        s_top[0].col[d - given] = left ? id : 0x7FFFFFFF;
+        if (left) {
+          atomicAdd(&s_left, 1);
+          best = fmaxf(best, s);
+        }
       }
     }
+  }
+  if constexpr (TOP) {
+    best = warp_max(best);
+    if (lane == 0) s_top[0].wv[warp] = best;
   }
   __syncthreads();
   for (int t = tid; t < a.T; t += nthreads) {
@@ -689,12 +740,13 @@ __global__ void __launch_bounds__(kVocThreads) vocab_join_kernel(const VJoinArgs
       v = __int_as_float(0x7FC00000);
       set_device_error(kDevBadId);
     } else if (id >= 0) {
-      v = row_logprob(s_dot[t], st, a.c, log_s);
+      v = row_logprob(a.xid ? xid : s_dot[t], st, a.c, log_s);
     }
     a.logprobs[row * a.T + t] = v;
   }
   if constexpr (TOP) {
     const bool nan = st.s != st.s;
+    for (int w = 0; w < kVocWarps; w++) best = fmaxf(best, s_top[0].wv[w]);
     for (int i = tid; i < cand && !nan; i += nthreads) {
       const float v = s_top[0].val[i];
       const int c = s_top[0].col[i];
@@ -703,7 +755,7 @@ __global__ void __launch_bounds__(kVocThreads) vocab_join_kernel(const VJoinArgs
       for (int j = 0; j < cand; j++) r += top_before(s_top[0].val[j], s_top[0].col[j], v, c);
       if (r < a.K) {
         a.top_ids[row * a.K + r] = c;
-        a.top_logprobs[row * a.K + r] = row_logprob(v, st, a.c, log_s);
+        a.top_logprobs[row * a.K + r] = row_logprob(v, VStat{best, st.s, st.u}, a.c, log_s);
       }
     }
     // Past the unmasked columns, or in a row that is no distribution.
@@ -935,7 +987,7 @@ struct VPlan {
   int cg, a_rows;
   int units_m, units_n;  // statistics
   int64_t ldmax;
-  size_t part_bytes, fwd_bytes;
+  size_t part_bytes, max_bytes, fwd_bytes;
   // backward
   bool split;
   int64_t chunk, ldz, ldp;
@@ -956,7 +1008,8 @@ static VPlan vocab_plan(int64_t rows, int V, int H, int top_k) {
   p.units_n = best_parts(p.units_m, tiles, slots, kVMaxParts, 0.25);
   p.part_bytes = align_up((size_t)p.units_n * kVEpiGroups * rows * sizeof(float4), 256);
   p.ldmax = tiles * (kVBN / kVGroup);
-  p.fwd_bytes = p.part_bytes + (top_k > 0 ? (size_t)rows * p.ldmax * 4 : 0);
+  p.max_bytes = top_k > 0 ? (size_t)rows * p.ldmax * 4 : 0;
+  p.fwd_bytes = p.part_bytes + p.max_bytes + (size_t)rows * kVCaught * 4;
   // With few rows, a given token's column or two carry most of the gradients,
   // and nothing averages the rounding of dZ: it is kept in two 16-bit parts
   // (16 or more bits), which doubles K where the weights' traffic bounds.
@@ -1005,6 +1058,11 @@ static int run_vocab_logprobs(const VMatrices &x, const VPlan &p, const LogprobA
   a.part = reinterpret_cast<float4 *>(ws);
   a.gmax = o.K > 0 ? reinterpret_cast<float *>(ws + p.part_bytes) : nullptr;
   a.ldmax = p.ldmax;
+  if (o.T <= kVCaught) {
+    a.ids = o.ids;
+    a.T = o.T;
+    a.xid = reinterpret_cast<float *>(ws + p.part_bytes + p.max_bytes);
+  }
   IG_CU(p.cg == 1 ? (launch_vgemm<1, false, false, kVStats>(ma, mb, mb, a, st))
                   : (launch_vgemm<2, false, false, kVStats>(ma, mb, mb, a, st)));
   VJoinArgs j{};
@@ -1021,6 +1079,7 @@ static int run_vocab_logprobs(const VMatrices &x, const VPlan &p, const LogprobA
   j.c = o.c;
   j.ids = o.ids;
   j.part = a.part;
+  j.xid = a.xid;
   j.gmax = a.gmax;
   j.ldmax = p.ldmax;
   j.ngroups = (p.V + kVGroup - 1) / kVGroup;

@@ -371,3 +371,30 @@ def test_lse_says_whether_a_row_is_empty(voc, dtype, top):
     want = torch.zeros(3001, device="cuda", dtype=torch.float64)
     want[7], want[8] = -1.0, 1.0  # all of p in column 7: (1 - 1.5) / 0.5; the other given one has none
     assert ((d[2].double() - want).abs() <= 1e-6 + EPS[dtype] * want.abs()).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("rows,V,H,T", [(1, 2985, 1024, 1), (40, 2985, 1024, 4), (300, 2985, 1000, 8), (300, 70001, 768, 2),
+                                        (129, 257, 520, 3)])
+def test_head_log_probability_of_a_likely_token(voc, dtype, rows, V, H, T):
+    """A token that takes nearly all of its row: its log probability is what the other columns leave, off by their own
+    relative errors (LOGIT of sum |h w| in every logit, P_TOL) and by the roundings of a sum near 1 (2^-24 each, (terms
+    per thread + 20) of them, at most 64), not by the difference of two ways to sum its logit."""
+    gen = torch.Generator(device="cuda").manual_seed(221)
+    w = (torch.randn(V, H, generator=gen, device="cuda") * 0.05).to(dtype)
+    ids = torch.randint(0, V, (rows, T), generator=gen, device="cuda", dtype=torch.int32)
+    h = torch.randn(rows, H, generator=gen, device="cuda")
+    h = (h + 8.0 * w[ids[:, T - 1].long()].float()).to(dtype)
+    z = (h.double() @ w.double().T) / 0.7
+    off = float((h.double().abs() @ w.double().abs().T).max()) * 2.0**-20 / 0.7
+    want = torch.log_softmax(z, 1).gather(1, ids.long())
+    r = voc.vocab_logprobs(h, w, ids, temperature=0.7, top_k=3)
+    likely = want[:, T - 1]
+    assert likely.max() > -1e-2 and likely.min() > -8
+    for got, lp in ((r.logprobs[:, T - 1], likely), (r.top_logprobs[:, 0], torch.log_softmax(z, 1).max(1).values)):
+        assert ((got.double() - lp).abs() <= lp.abs() * (2 * off + P_TOL) + 2.0**-18).all()
+    assert ((r.logprobs.double() - want).abs() <= (STAT_TOL + 2 * off) * (1 + want.abs())).all()
+    # More tokens than are taken from the accumulators: the same up to the logits' error.
+    many = torch.cat([ids, torch.randint(0, V, (rows, 9), generator=gen, device="cuda", dtype=torch.int32)], 1).contiguous()
+    s = voc.vocab_logprobs(h, w, many, temperature=0.7, top_k=3)
+    assert ((s.logprobs[:, :T] - r.logprobs).abs() <= 2 * off).all() and torch.equal(s.lse, r.lse)
