@@ -370,7 +370,8 @@ IG_API int ig_token_logprobs_backward(const void *logits, int32_t dtype, int64_t
  * tail != 0: teacher_logits are log probabilities, q = exp of them, and what
  *   is left of 1 is one more outcome against the mass of p outside the list:
  *   loss[r] = w (sum q (log q - log p) + q_rest (log q_rest - log p_rest))
- *   (left out where the row has no unmasked column outside the list).
+ *   (left out where the row has no unmasked column outside the list, or where
+ *   q_rest is less than 2^-21, the rounding of the list's sum).
  * w = weights[r] (NULL: 1), the row's share of the total: dlogits (NULL: loss
  * only; may be logits, with ldd = ld, as above) is the gradient of
  * sum_r loss[r]. A row with weight 0 or without entries: loss 0 and gradient

@@ -1025,6 +1025,12 @@ struct DistillArgs {
   int parts;  // CTAs per row (a cluster)
 };
 
+// Less than this left of 1 by the list is the rounding of its sum (3e-7 at
+// most over lists of up to 256 that hold everything): no outcome. Against
+// columns that are masked by a finite value it would count with their whole
+// depth (2e30 nats for the lowest value, 2e-3 for -1e4 at temperature 0.3).
+constexpr float kRestLeast = 4.76837158e-7f;  // 2^-21
+
 // A CTA or a cluster per row, in two passes over it: the statistics, then the
 // gradient while the row is still in L2 (the row is fetched from DRAM once).
 // 4096 x 50021 bf16: 157 us, 5.2 TB/s of its 820 MB, 81% of the measured copy
@@ -1188,7 +1194,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT) distill_topk_kernel(const Disti
       }
       if constexpr (TAIL) {
         q_sum = warp_sum(q_sum);
-        q_rest = q_sum == q_sum ? fmaxf(1.0f - q_sum, 0.0f) : q_sum;
+        q_rest = q_sum < 1.0f - kRestLeast ? 1.0f - q_sum : (q_sum == q_sum ? 0.0f : q_sum);
         l = vstat_warp<false>(l, c2);
         if (lane == 0) s_list = l;
       } else {

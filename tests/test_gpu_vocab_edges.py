@@ -398,3 +398,26 @@ def test_head_log_probability_of_a_likely_token(voc, dtype, rows, V, H, T):
     many = torch.cat([ids, torch.randint(0, V, (rows, 9), generator=gen, device="cuda", dtype=torch.int32)], 1).contiguous()
     s = voc.vocab_logprobs(h, w, many, temperature=0.7, top_k=3)
     assert ((s.logprobs[:, :T] - r.logprobs).abs() <= 2 * off).all() and torch.equal(s.lse, r.lse)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,V,K", [(3, 40, 7), (6, 20011, 100), (2400, 2049, 33)])
+def test_tail_of_a_list_that_holds_everything(voc, dtype, rows, V, K):
+    """The teacher's list and the student's unmasked columns are the same: what float32 leaves of 1 does not count against
+    columns masked by a finite value, however deep (the lowest value, -1e4)."""
+    gen = torch.Generator(device="cuda").manual_seed(231)
+    ids = torch.rand((rows, V), generator=gen, device="cuda").topk(K, dim=1).indices.int().contiguous()
+    y = torch.randn((rows, K), generator=gen, device="cuda") * 2
+    t = torch.log_softmax(torch.randn((rows, K), generator=gen, device="cuda").double() * 2, 1).float().contiguous()
+    for mask in (-1e4, torch.finfo(dtype).min):
+        x = torch.full((rows, V), mask, device="cuda").scatter_(1, ids.long(), y).to(dtype)
+        for temperature in (0.3, 1.0):
+            loss, d = voc.distill_topk(x, ids, t, temperature=temperature, tail=True)
+            z = x.double() / temperature
+            logp = torch.log_softmax(z, 1)
+            q = t.double().exp()
+            wl = (q * (t.double() - logp.gather(1, ids.long()))).sum(1)
+            wd = (logp.exp() * q.sum(1, keepdim=True)).scatter_add_(1, ids.long(), -q) / temperature
+            close(loss, wl, 4 * STAT_TOL, "loss")
+            tol = (P_TOL * logp.exp() + P_TOL * wd.abs() + 1e-6) / temperature + EPS[dtype] / 2 * wd.abs() * 1.01 + TINY[dtype]
+            assert ((d.double() - wd).abs() <= tol).all()
