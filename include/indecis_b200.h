@@ -393,7 +393,10 @@ IG_API int64_t ig_vocab_workspace(int64_t rows, int32_t vocab, int32_t hidden_si
  * IG_DT_F16, float32 accumulation), which are never stored. Rows of both
  * matrices start at multiples of 16 bytes (strides ldh, ldw in elements,
  * multiples of 8); hidden_size is free. A bias per token is one more column:
- * hidden extended by 1, weight by the bias. rows <= 2^24. */
+ * hidden extended by 1, weight by the bias. rows <= 2^24. The tensor cores cut
+ * their sums off: the logits behind lse and entropy are low by up to 2^-20 of
+ * sum |h w|. Log probabilities (of up to eight given tokens a row, and of the
+ * alternatives) take back what a likely token's logit is short there. */
 IG_API int ig_vocab_logprobs(const void *hidden, int64_t ldh, const void *weight, int64_t ldw, int32_t dtype,
                              int64_t rows, int32_t vocab, int32_t hidden_size, double temperature, const int32_t *ids,
                              int32_t nids, float *logprobs, float *lse, float *entropy, int32_t top_k,
@@ -404,13 +407,19 @@ IG_API int ig_vocab_logprobs(const void *hidden, int64_t ldh, const void *weight
  * the forward's logprobs, lse and entropy: with G the gradient
  * ig_token_logprobs_backward gives for the logits, dhidden = G . weight and
  * dweight = G^T . hidden, in the operands' type, strides free, apart from the
- * operands and from one another. G is formed
- * in the workspace in column chunks and rounded to the operands' type (for
- * float16 scaled by a power of two, so that small probabilities keep their
- * bits); the sums are float32 in a fixed order. p = exp(min(z - lse, 0)), off
- * by |lse| 2^-24 of itself through lse's rounding; in a row whose lse float32
- * does not resolve (wholly masked by a bias past 2^22, say) the columns within
- * a step of the maximum have p = 1. Zero for a row with lse -inf or -FLT_MAX. */
+ * operands and from one another.
+ * G is formed in the workspace in column chunks and rounded to the operands'
+ * type (for float16 scaled by a power of two, so that small probabilities keep
+ * their bits; for at most 128 rows kept in two parts of that type); the sums
+ * are float32 in a fixed order. The rounding of G is of the size of the
+ * gradients' own: for more than 128 rows their error is 1.4 times (at most 1.5
+ * times) what it would be without.
+ * p = exp(min(z - lse, 0)), off by |lse| 2^-24 of itself through lse's
+ * rounding; in a row whose lse float32 does not resolve (wholly masked by a
+ * bias past 2^22, say) the columns within a step of the maximum have p = 1.
+ * Zero for a row with lse -inf or -FLT_MAX. A bias column that holds -inf
+ * masks its tokens here too, but its own entry of dhidden is then NaN (0 times
+ * infinity). */
 IG_API int ig_vocab_logprobs_backward(const void *hidden, int64_t ldh, const void *weight, int64_t ldw, int32_t dtype,
                                       int64_t rows, int32_t vocab, int32_t hidden_size, double temperature,
                                       const int32_t *ids, int32_t nids, const float *logprobs, const float *lse,

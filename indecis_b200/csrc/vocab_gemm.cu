@@ -64,15 +64,15 @@ struct VRowCoef {
 };
 
 constexpr int kVGroup = 16;  // columns per stored maximum
-// At most this many given tokens a row: their logits are taken from the
-// accumulators, as the statistics are. The tensor cores' sums are cut off, not
-// rounded (a logit of 10 from 1000 terms comes out 1e-5 low), so a logit summed
-// in another way does not match them: the log probability of a token that
-// takes most of its row, -0.13 in the mean, was off by 6e-5 of itself.
-// More tokens' logits are dot products in the joining kernel, as a row's look-up
-// grows with their number: 4096 x 65536 x 256 takes 150 us with dot products,
-// 152 with one token caught, 160 with eight; with more, most are not the
-// likeliest of their row.
+// The tensor cores' sums are cut off, not rounded: a logit of 10 from 1000
+// terms comes out 1e-5 low, and lse by that times the column's probability.
+// Against a logit summed with rounding, the log probability of a token that
+// takes most of its row (-0.13 in the mean) was off by 6e-5 of itself. For at
+// most this many given tokens a row the accumulator's own logit is kept too,
+// and the row's lse is corrected by what it is short. More tokens make it less
+// likely that one is the likeliest of the row, and a row's look-up grows with
+// their number: 4096 x 65536 x 256 takes 150 us without, 155 with one token and
+// 162 with eight.
 constexpr int kVCaught = 8;
 // The lowest of a row's given tokens that is at least `from` and lies in the
 // columns of epilogue group g.
@@ -603,7 +603,7 @@ struct VJoinArgs {
   float c;
   const int32_t *ids;
   const float4 *part;
-  const float *xid;  // the given tokens' logits, or NULL: dot products here
+  const float *xid;  // the given tokens' logits as accumulated, or NULL
   const float *gmax;
   int64_t ldmax;
   int ngroups;
@@ -613,10 +613,14 @@ struct VJoinArgs {
 };
 
 // One CTA per row: the statistics of the row's parts, then the dot products of
-// the given tokens (where they are many) and of the best groups' columns, eight
-// lanes each (128 bytes of either operand a step). A logit summed here is
-// float32 in another order than the tensor core's, so the alternatives are
-// counted from the best of them, not from the statistics' maximum.
+// the given tokens and of the best groups' columns, eight lanes each (128
+// bytes of either operand a step). A logit summed here is float32 in another
+// order than the tensor core's: `full` against `cut`, lse is short by
+// p c (full - cut) of the column's probability p, which a log probability of
+// that column, or of one beside the row's best, takes back.
+__device__ __forceinline__ float back(float x, float p, float full, float cut) {
+  return p > 0.0f ? fmaf(-p, full - cut, x) : x;
+}
 template <bool TOP>
 __global__ void __launch_bounds__(kVocThreads) vocab_join_kernel(const VJoinArgs a) {
   __shared__ VStat s_warp[kVocWarps];
@@ -669,17 +673,17 @@ __global__ void __launch_bounds__(kVocThreads) vocab_join_kernel(const VJoinArgs
     if (a.lse) a.lse[row] = lse;
     if (a.entropy) a.entropy[row] = entropy;
   }
-  const int given = a.xid ? 0 : a.T, cand = s_on * kVGroup, total = given + cand;
+  const int cand = s_on * kVGroup, total = a.T + cand;
   const uint16_t *h = a.h + row * a.ldh;
   const int sub = tid & 7;
   [[maybe_unused]] float best = -IG_INF;  // of the alternatives
   for (int d0 = 0; d0 < total; d0 += nthreads / 8) {
     const int d = d0 + (tid >> 3);
     int id = -1;
-    if (d < given)
+    if (d < a.T)
       id = a.ids[row * a.T + d];
     else if (d < total)
-      id = s_ocol[(d - given) / kVGroup] * kVGroup + (d - given) % kVGroup;
+      id = s_ocol[(d - a.T) / kVGroup] * kVGroup + (d - a.T) % kVGroup;
     float s = 0.0f;
     if (id >= 0 && id < a.V) {
       const uint16_t *w = a.w + (int64_t)id * a.ldw;
@@ -714,13 +718,13 @@ __global__ void __launch_bounds__(kVocThreads) vocab_join_kernel(const VJoinArgs
 #pragma unroll
     for (int o = 4; o; o >>= 1) s += __shfl_xor_sync(~0u, s, o);
     if (sub == 0) {
-      if (d < given) {
+      if (d < a.T) {
         s_dot[d] = s;
       } else if (TOP && d < total) {
         // A masked column of a group is no alternative.
         const bool left = id < a.V && s > -IG_INF;
-        s_top[0].val[d - given] = left ? s : -IG_INF;
-        s_top[0].col[d - given] = left ? id : 0x7FFFFFFF;
+        s_top[0].val[d - a.T] = left ? s : -IG_INF;
+        s_top[0].col[d - a.T] = left ? id : 0x7FFFFFFF;
         if (left) {
           atomicAdd(&s_left, 1);
           best = fmaxf(best, s);
@@ -740,7 +744,9 @@ __global__ void __launch_bounds__(kVocThreads) vocab_join_kernel(const VJoinArgs
       v = __int_as_float(0x7FC00000);
       set_device_error(kDevBadId);
     } else if (id >= 0) {
-      v = row_logprob(a.xid ? xid : s_dot[t], st, a.c, log_s);
+      float x = s_dot[t];
+      if (a.xid) x = back(x, expf(row_logprob(xid, st, a.c, log_s)), x, xid);
+      v = row_logprob(x, st, a.c, log_s);
     }
     a.logprobs[row * a.T + t] = v;
   }
@@ -755,7 +761,7 @@ __global__ void __launch_bounds__(kVocThreads) vocab_join_kernel(const VJoinArgs
       for (int j = 0; j < cand; j++) r += top_before(s_top[0].val[j], s_top[0].col[j], v, c);
       if (r < a.K) {
         a.top_ids[row * a.K + r] = c;
-        a.top_logprobs[row * a.K + r] = row_logprob(v, VStat{best, st.s, st.u}, a.c, log_s);
+        a.top_logprobs[row * a.K + r] = row_logprob(back(v, 1.0f / st.s, best, st.m), st, a.c, log_s);
       }
     }
     // Past the unmasked columns, or in a row that is no distribution.
@@ -974,10 +980,14 @@ constexpr int kVMaxParts = 256;        // column parts per M tile
 // At most this many rows: single CTAs (one row x 262144 x 768: 86 us, by pairs
 // 113; 128 rows 88 and 92).
 constexpr int kVOneCtaRows = 128;
-// At most this many rows: dZ in two 16-bit parts. In one part, a gradient's
-// error is 1.41 times its own rounding's in the median; the spread shrinks with
-// the rows (at 129 to 256 the 95th percentile is 1.48). Two parts cost 13 to
-// 32% there (256 x 262144 x 768: 385 us in one, 508 in two).
+// At most this many rows: dZ in two 16-bit parts, and the gradients as exact as
+// their own type. With more rows dZ is held in the operands' type, as a caller
+// that stored the logits' gradient for its products would hold it: its rounding
+// adds to the gradients' own one of the same size, so they are off by 1.4 times
+// what they would be with dZ in 32 bits (0.0024 against 0.0017 in the norm in
+// bfloat16, 0.00030 against 0.00021 in float16; at 129 rows up to 1.5 times,
+// as few rows do not average). Two parts for all rows would double K in two of
+// the three products (256 x 262144 x 768: 385 us in one, 508 in two).
 constexpr int kVSplitRows = 128;
 constexpr int64_t kVDzBytes = 1ll << 30;  // dZ is formed in column chunks of at most this size
 
@@ -1125,7 +1135,7 @@ static int run_vocab_grad(const VMatrices &x, const VPlan &p, const LogprobGradA
     a.N = (int)vc;
     a.a_rows = p.a_rows;
     a.kblocks = (p.H + kVBK - 1) / kVBK;
-  a.kparts = 1;
+    a.kparts = 1;
     a.idesc = idesc_f16(tm, kVBN, x.dtype, false, false);
     a.units_m = p.units_m;
     a.units_n = (int)((vc + kVBN - 1) / kVBN);

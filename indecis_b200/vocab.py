@@ -6,6 +6,9 @@ Thin wrappers over the C ABI: each checks shapes, types and strides, allocates
 the outputs, enqueues the kernels on the current stream of the inputs' device
 and raises on a non-zero status. Logits are [rows, vocab] float32, bfloat16 or
 float16 with a unit column stride and any row stride.
+
+No call records anything for torch's autograd, whatever its inputs require:
+gradients come from the *_backward functions and from distill_topk.
 """
 from __future__ import annotations
 
@@ -22,6 +25,7 @@ _DT = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 
 
 class TokenLogProbs(NamedTuple):
+    """Pieces of one allocation: clone() what is kept on its own."""
     logprobs: torch.Tensor                # float32 [rows, given]
     lse: torch.Tensor                     # float32 [rows]
     entropy: torch.Tensor                 # float32 [rows]
@@ -105,7 +109,7 @@ def token_logprobs(logits, ids, temperature=1.0, top_k=0) -> TokenLogProbs:
 def token_logprobs_backward(logits, ids, lse, entropy, dlogprobs, dentropy=None, temperature=1.0, out=None):
     """Gradient with respect to the logits, in their type, from the gradients
     of token_logprobs' logprobs and entropy. out: where to write it (may be
-    logits itself)."""
+    logits itself, but not overlap it otherwise)."""
     ld = _matrix(logits, "logits")
     N, V = logits.shape
     if ids.dim() != 2:
@@ -137,7 +141,7 @@ def distill_topk(logits, teacher_ids, teacher_logits, temperature=1.0, tail=Fals
     log probabilities, and the mass they leave is one more outcome. Returns
     (loss float32 [rows], already weighted by `weights`; the gradient of its
     sum with respect to the logits, or None with grad=False). out: where to
-    write the gradient (may be logits itself)."""
+    write the gradient (may be logits itself, but not overlap it otherwise)."""
     ld = _matrix(logits, "logits")
     N, V = logits.shape
     if teacher_ids.dim() != 2:
@@ -210,7 +214,9 @@ def vocab_logprobs_backward(hidden, weight, ids, logprobs, lse, entropy, dlogpro
                             need_hidden=True, need_weight=True):
     """Gradients with respect to hidden and weight, in their type (None where
     not needed), from the gradients of vocab_logprobs' logprobs and entropy and
-    its results."""
+    its results. The logits' gradient in between is held in the operands' type
+    for more than 128 rows, which adds an error of the gradients' own rounding's
+    size."""
     hidden, ldh, weight, ldw = _operands(hidden, weight)
     N, H = hidden.shape
     V = weight.shape[0]
