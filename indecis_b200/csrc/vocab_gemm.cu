@@ -18,11 +18,11 @@
 // TMA boxes are then 64 (M or N) x 64 (K) and the matrix descriptors
 // MN-major, so nothing is transposed in memory.
 //
-// 4096 x 65536 x 768 bf16: the forward takes 337 us (1,220 TFLOP/s) where the
-// library's product alone takes 312 and stores the logits; the backward 988 us
-// for its three products (1,250 TFLOP/s). The power limit sets the rate of long
-// runs: 1.40 ms for 4096 x 262144 x 768 back to back (1,180 TFLOP/s, 84% of the
-// measured sustained rate), 1.17 ms one at a time.
+// 4096 x 65536 x 768 bf16, one call at a time: the forward takes 323 us (1,280
+// TFLOP/s) where the library's product alone takes 297 and stores the logits;
+// the backward 966 us for its three products (1,280 TFLOP/s). The power limit
+// sets the rate of long runs: 1.38 ms for 4096 x 262144 x 768 back to back
+// (1,190 TFLOP/s, 85% of the measured sustained rate), 1.21 ms one at a time.
 //
 // Tiles are 256 x 256 on a CTA pair (cta_group::2: each CTA holds half of
 // either operand, 32 KB per 64 of K, where one CTA alone would fetch 48 KB
