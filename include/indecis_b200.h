@@ -434,8 +434,8 @@ IG_API int ig_vocab_logprobs_backward(const void *hidden, int64_t ldh, const voi
  * elements, rows starting at any multiple of the element size. Statistics and
  * sums are float32 in a fixed order, results rounded once. IG_ERR_BAD_ARG, before any
  * GPU work, for null pointers, negative sizes, strides shorter than a row,
- * outputs that share memory with an operand or one another (but for those that
- * may replace an operand). */
+ * outputs or a workspace that share memory with an operand or one another (but
+ * for outputs that may replace an operand). */
 
 /* Layer norm of rows of n: y = (x - mean) * rstd * weight + bias, rstd = 1 /
  * sqrt(mean of (x - mean)^2 + eps). y has x's type, or 16 bits for float32 x;

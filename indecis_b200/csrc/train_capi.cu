@@ -1,6 +1,7 @@
 // C entry points of the operators that blocks are trained with (layer_norm.cu, gated_ff.cu, adamw.cu).
 #include <algorithm>
 #include <cmath>
+#include <initializer_list>
 #include <new>
 #include <string>
 #include <utility>
@@ -16,6 +17,19 @@ namespace ig {
 static const char *bad_in_place_of(const RowSpan &in, const RowSpan &out, bool same_type) {
   if (same_type && in.at == out.at && in.stride == out.stride) return nullptr;
   return overlap(in, out) ? "an output may replace an operand of its type and stride, but not overlap one otherwise" : nullptr;
+}
+
+// A dense vector of n; a null pointer or no elements: nothing.
+static RowSpan vector_span(const void *p, int64_t n, int es) { return RowSpan(n > 0 ? p : nullptr, 1, n, n, es); }
+// Outputs against operands and one another.
+static const char *bad_shared(std::initializer_list<RowSpan> out, std::initializer_list<RowSpan> in) {
+  for (auto o = out.begin(); o != out.end(); ++o) {
+    for (const RowSpan &i : in)
+      if (overlap(*o, i)) return "outputs and the workspace cannot share memory with an operand or one another";
+    for (auto q = out.begin(); q != o; ++q)
+      if (overlap(*o, *q)) return "outputs and the workspace cannot share memory with an operand or one another";
+  }
+  return nullptr;
 }
 
 static const char *bad_norm_args(int32_t x_dtype, int32_t y_dtype, int64_t rows, int32_t n, const void *weight,
@@ -62,7 +76,13 @@ int ig_layer_norm(const void *x, int32_t x_dtype, int64_t ldx, int64_t rows, int
   if (!m && (!(eps >= 0.0) || !std::isfinite((float)eps))) m = "eps must be finite and not negative";
   if (!m) m = bad_matrix(x, rows, n, ldx, ex);
   if (!m) m = bad_matrix(y, rows, n, ldy, ey);
-  if (!m) m = bad_in_place_of(RowSpan(x, rows, n, ldx, ex), RowSpan(y, rows, n, ldy, ey), ex == ey);
+  if (!m) {
+    const RowSpan in(x, rows, n, ldx, ex), out(y, rows, n, ldy, ey), s0 = vector_span(mean, rows, 4), s1 = vector_span(rstd, rows, 4);
+    const int ew = vocab_elem_size(weight_dtype);
+    m = bad_in_place_of(in, out, ex == ey);
+    if (!m) m = bad_shared({out, s0, s1}, {vector_span(weight, n, ew), vector_span(bias, n, ew)});
+    if (!m) m = bad_shared({s0, s1}, {in});
+  }
   if (m) return fail(IG_ERR_BAD_ARG, std::string("ig_layer_norm: ") + m);
   if (rows == 0) return 0;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
@@ -92,9 +112,12 @@ int ig_layer_norm_backward(const void *dy, int32_t y_dtype, int64_t lddy, const 
   if (!m) m = bad_matrix(dx, rows, n, lddx, ex);
   if (!m && rows > 0 && (!mean || !rstd)) m = "null argument";
   if (!m) {
-    const RowSpan out(dx, rows, n, lddx, ex);
-    m = bad_in_place_of(RowSpan(x, rows, n, ldx, ex), out, true);
-    if (!m) m = bad_in_place_of(RowSpan(dy, rows, n, lddy, ey), out, x_dtype == y_dtype);
+    const RowSpan out(dx, rows, n, lddx, ex), in(x, rows, n, ldx, ex), up(dy, rows, n, lddy, ey), sw = vector_span(dweight, n, ew),
+        sb = vector_span(dbias, n, ew), ws = vector_span(workspace, sums ? layer_norm_workspace(rows, n) : 0, 1);
+    m = bad_in_place_of(in, out, true);
+    if (!m) m = bad_in_place_of(up, out, x_dtype == y_dtype);
+    if (!m) m = bad_shared({out, sw, sb, ws}, {vector_span(weight, n, ew), vector_span(mean, rows, 4), vector_span(rstd, rows, 4)});
+    if (!m) m = bad_shared({sw, sb, ws}, {in, up});
   }
   if (m) return fail(IG_ERR_BAD_ARG, std::string("ig_layer_norm_backward: ") + m);
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
