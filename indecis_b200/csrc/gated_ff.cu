@@ -923,10 +923,12 @@ static FfCut ff_cut(const FfShapeOf *p, int count) {
   return best;
 }
 
+static size_t ff_h_bytes(int64_t rows, int I) { return align_up((size_t)rows * ff_ld(I) * 2, 256); }
+static size_t ff_z_bytes(int64_t rows, int I) { return (size_t)ff_up(rows, 32) * ff_up(I, 32) * 8; }
 static FfPlan ff_plan(const FfSizes &s, bool backward) {
   FfPlan p{};
-  p.h_bytes = align_up((size_t)s.rows * ff_ld(s.I) * 2, 256);
-  p.z_bytes = (size_t)ff_up(s.rows, 32) * ff_up(s.I, 32) * 8;
+  p.h_bytes = ff_h_bytes(s.rows, s.I);
+  p.z_bytes = ff_z_bytes(s.rows, s.I);
   const int64_t rows[4] = {s.rows, 2 * (int64_t)s.I, s.O, s.rows}, cols[4] = {s.H, s.H, s.I, s.O};
   for (int i = 0; i < 4; i++) {
     p.off[i] = p.pack_bytes;

@@ -149,8 +149,7 @@ int ig_layer_norm_backward(const void *dy, int32_t y_dtype, int64_t lddy, const 
 
 int64_t ig_gated_ff_saved(int64_t rows, int32_t inner) {
   if (rows <= 0 || rows > (1 << 24) || inner < 1 || inner > (1 << 20)) return 0;
-  const FfPlan p = ff_plan(FfSizes{rows, 1, inner, 1, 0}, false);
-  return (int64_t)(p.h_bytes + p.z_bytes);
+  return (int64_t)(ff_h_bytes(rows, inner) + ff_z_bytes(rows, inner));
 }
 
 int64_t ig_gated_ff_workspace(int64_t rows, int32_t hidden, int32_t inner, int32_t out_size, int32_t unaligned, int32_t pass) {
@@ -168,20 +167,18 @@ int ig_gated_ff(const void *x, int64_t ldx, const void *w_in, int64_t ldi, const
   if (!m) m = bad_matrix(w_in, 2 * (int64_t)inner, hidden, ldi, 2);
   if (!m) m = bad_matrix(w_out, out_size, inner, ldw, 2);
   if (!m) m = bad_matrix(y, rows, out_size, ldy, 2);
-  if (!m) {
-    const RowSpan o(y, rows, out_size, ldy, 2);
-    if (overlap(o, RowSpan(x, rows, hidden, ldx, 2)) || overlap(o, RowSpan(w_in, 2 * (int64_t)inner, hidden, ldi, 2)) ||
-        overlap(o, RowSpan(w_out, out_size, inner, ldw, 2)))
-      m = "the result cannot overlap the operands";
-  }
   if (!m && (reinterpret_cast<uintptr_t>(saved) & 255)) m = "what is saved must start at a multiple of 256 bytes";
   if (m) return fail(IG_ERR_BAD_ARG, std::string("ig_gated_ff: ") + m);
   if (rows == 0) return 0;
   const FfMatrix mx = ff_matrix(x, ldx, rows, hidden), mi = ff_matrix(w_in, ldi, 2, hidden), mo = ff_matrix(w_out, ldw, out_size, inner);
   const FfSizes s{rows, hidden, inner, out_size, ff_pack_bits(mx, mi, mo, FfMatrix{})};
   const FfPlan p = ff_plan(s, false);
-  if (bad_workspace(workspace, workspace_bytes, ff_bytes(s, p, saved ? 1 : 0)))
+  const size_t need = ff_bytes(s, p, saved ? 1 : 0);
+  if (bad_workspace(workspace, workspace_bytes, need))
     return fail(IG_ERR_BAD_ARG, "ig_gated_ff: workspace missing, too small or not aligned to 256 bytes");
+  m = bad_shared({RowSpan(y, rows, out_size, ldy, 2), vector_span(saved, (int64_t)(p.h_bytes + p.z_bytes), 1), vector_span(workspace, (int64_t)need, 1)},
+                 {RowSpan(x, rows, hidden, ldx, 2), RowSpan(w_in, 2 * (int64_t)inner, hidden, ldi, 2), RowSpan(w_out, out_size, inner, ldw, 2)});
+  if (m) return fail(IG_ERR_BAD_ARG, std::string("ig_gated_ff: ") + m);
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   ProfScope ps("gated_ff", 2.0 * ((double)rows * (hidden + out_size) + (double)inner * (2.0 * hidden + out_size)),
                2.0 * rows * inner * (2.0 * hidden + out_size), 2, st);
@@ -204,21 +201,13 @@ int ig_gated_ff_backward(const void *dy, int64_t lddy, const void *x, int64_t ld
   if (!m && dw_out) m = bad_matrix(dw_out, out_size, inner, lddw, 2);
   if (!m && rows > 0 && (!saved || (reinterpret_cast<uintptr_t>(saved) & 255)))
     m = "what the forward saved is missing or does not start at a multiple of 256 bytes";
-  if (!m) {
-    const RowSpan in[4] = {RowSpan(dy, rows, out_size, lddy, 2), RowSpan(x, rows, hidden, ldx, 2), RowSpan(w_in, i2, hidden, ldi, 2),
-                           RowSpan(w_out, out_size, inner, ldw, 2)};
-    const RowSpan out[3] = {RowSpan(dx, rows, hidden, lddx, 2), RowSpan(dw_in, i2, hidden, lddi, 2),
-                            RowSpan(dw_out, out_size, inner, lddw, 2)};
-    for (int i = 0; i < 3 && !m; i++) {
-      for (int j = 0; j < 4; j++)
-        if (overlap(out[i], in[j])) m = "the gradients cannot overlap the operands or one another";
-      for (int j = 0; j < i; j++)
-        if (overlap(out[i], out[j])) m = "the gradients cannot overlap the operands or one another";
-    }
-  }
   if (m) return fail(IG_ERR_BAD_ARG, std::string("ig_gated_ff_backward: ") + m);
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   if (!dx && !dw_in && !dw_out) return 0;
+  const RowSpan sdx(dx, rows, hidden, lddx, 2), sdi(dw_in, i2, hidden, lddi, 2), sdo(dw_out, out_size, inner, lddw, 2), sy(dy, rows, out_size, lddy, 2),
+      sx(x, rows, hidden, ldx, 2), si(w_in, i2, hidden, ldi, 2), so(w_out, out_size, inner, ldw, 2),
+      sv = vector_span(saved, ig_gated_ff_saved(rows, inner), 1);
+  if ((m = bad_shared({sdx, sdi, sdo}, {sy, sx, si, so, sv}))) return fail(IG_ERR_BAD_ARG, std::string("ig_gated_ff_backward: ") + m);
   if (rows == 0) {
     if (dw_in) IG_CU(cudaMemset2DAsync(dw_in, (size_t)lddi * 2, 0, (size_t)hidden * 2, i2, st));
     if (dw_out) IG_CU(cudaMemset2DAsync(dw_out, (size_t)lddw * 2, 0, (size_t)inner * 2, out_size, st));
@@ -228,8 +217,11 @@ int ig_gated_ff_backward(const void *dy, int64_t lddy, const void *x, int64_t ld
                  mo = ff_matrix(w_out, ldw, out_size, inner);
   const FfSizes s{rows, hidden, inner, out_size, ff_pack_bits(mx, mi, mo, md)};
   const FfPlan p = ff_plan(s, true);
-  if (bad_workspace(workspace, workspace_bytes, ff_bytes(s, p, 2)))
+  const size_t need = ff_bytes(s, p, 2);
+  if (bad_workspace(workspace, workspace_bytes, need))
     return fail(IG_ERR_BAD_ARG, "ig_gated_ff_backward: workspace missing, too small or not aligned to 256 bytes");
+  if ((m = bad_shared({vector_span(workspace, (int64_t)need, 1)}, {sdx, sdi, sdo, sy, sx, si, so, sv})))
+    return fail(IG_ERR_BAD_ARG, std::string("ig_gated_ff_backward: ") + m);
   const int products = (dx || dw_in) + 2 * (dx != nullptr) + 2 * (dw_in != nullptr) + (dw_out != nullptr);
   ProfScope ps("gated_ff_backward", 4.0 * ((double)rows * (hidden + out_size) + (double)inner * (2.0 * hidden + out_size)),
                2.0 * products * rows * inner * hidden, 4, st);

@@ -88,3 +88,41 @@ def test_layer_norm_backward_without_rows(lib):
     apart(call, base)
     for kw in (dict(dw=M), dict(db=2 * M), dict(dw=3 * M - 4), dict(db=M + VECTOR - 4)):
         refused(call, base, "ig_layer_norm_backward", **kw)
+
+
+H, I, O = 64, 32, 48
+
+
+def test_gated_ff(lib):
+    def call(x, wi, wo, y, saved, ws):
+        return lib.ig_gated_ff(x, H, wi, H, wo, I, 1, ROWS, H, I, O, 0, y, O, saved, ws, M // 2, None)
+    names = ("x", "wi", "wo", "y", "saved", "ws")
+    base = {k: (i + 1) * M for i, k in enumerate(names)}
+    apart(call, base)
+    for saved in (base["saved"], None):  # 4 rows or fewer without it take another workspace
+        size = dict(x=2 * ROWS * H, wi=4 * I * H, wo=2 * O * I, y=2 * ROWS * O, saved=lib.ig_gated_ff_saved(ROWS, I),
+                    ws=lib.ig_gated_ff_workspace(ROWS, H, I, O, 0, int(saved is not None)))
+        at = dict(base, saved=saved)
+        for out in ("y", "saved", "ws"):
+            for other in names:
+                if other == out or at[other] is None or size[out] == 0 or size[other] == 0 or at[out] is None:
+                    continue
+                for spot in (at[other], (at[other] + size[other] - 2) // 256 * 256, at[other] - (size[out] - 1) // 256 * 256):
+                    if spot + size[out] > at[other]:
+                        refused(call, at, "ig_gated_ff", **{out: spot})
+
+
+def test_gated_ff_backward(lib):
+    names = ("dy", "x", "wi", "wo", "saved", "dx", "dwi", "dwo", "ws")
+
+    def call(dy, x, wi, wo, saved, dx, dwi, dwo, ws):
+        return lib.ig_gated_ff_backward(dy, O, x, H, wi, H, wo, I, 1, ROWS, H, I, O, 0, saved, dx, H, dwi, H, dwo, I, ws, M // 2, None)
+    base = {k: (i + 1) * M for i, k in enumerate(names)}
+    apart(call, base)
+    size = dict(dy=2 * ROWS * O, x=2 * ROWS * H, wi=4 * I * H, wo=2 * O * I, saved=lib.ig_gated_ff_saved(ROWS, I), dx=2 * ROWS * H,
+                dwi=4 * I * H, dwo=2 * O * I, ws=lib.ig_gated_ff_workspace(ROWS, H, I, O, 0, 2))
+    for out in ("dx", "dwi", "dwo", "ws"):
+        for other in names:
+            if other != out:
+                for spot in (base[other], (base[other] + size[other] - 2) // 256 * 256, base[other] - (size[out] - 1) // 256 * 256):
+                    refused(call, base, "ig_gated_ff_backward", **{out: spot})
