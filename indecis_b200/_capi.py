@@ -10,6 +10,7 @@ import os
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libindecis_b200.so")
+TORCH_OPS_PATH = os.path.join(_HERE, "_torch_ops.so")
 
 IG_OK = 0
 IG_ERR_BAD_ARG = 1
@@ -129,6 +130,24 @@ _lib = None
 
 class LibraryMissing(RuntimeError):
     pass
+
+
+class _TorchOps:
+    """The functions of _torch_ops.so (the training operators' calls), loaded with the first that is asked for, so that
+    importing the modules around it needs nothing built."""
+
+    def __getattr__(self, name):
+        if name.startswith("__"):
+            raise AttributeError(name)
+        if not os.path.exists(TORCH_OPS_PATH):
+            raise LibraryMissing(f"{TORCH_OPS_PATH} is not built: run `python -m indecis_b200.build` (no CPU fallback exists)")
+        from . import _torch_ops
+        fn = getattr(_torch_ops, name)
+        setattr(self, name, fn)  # later calls find it there
+        return fn
+
+
+torch_ops = _TorchOps()
 
 
 def load() -> C.CDLL:

@@ -15,7 +15,7 @@ from typing import NamedTuple
 
 import torch
 
-from . import _torch_ops
+from ._capi import torch_ops as _torch_ops
 from .vocab import _DT
 
 

@@ -11,7 +11,7 @@ from typing import NamedTuple
 
 import torch
 
-from . import _torch_ops
+from ._capi import torch_ops as _torch_ops
 
 BLOCK = 256  # elements of a tensor that share a scale in 8 bits
 
