@@ -33,7 +33,7 @@ static const char *bad_shared(std::initializer_list<RowSpan> out, std::initializ
 }
 
 static const char *bad_norm_args(int32_t x_dtype, int32_t y_dtype, int64_t rows, int32_t n, const void *weight,
-                                 const void *bias, int32_t weight_dtype) {
+                                 const void *bias, int32_t weight_dtype, const float *mean, const float *rstd) {
   const int wes = vocab_elem_size(weight_dtype);
   if (!vocab_elem_size(x_dtype) || !vocab_elem_size(y_dtype)) return "dtype must be float32, bfloat16 or float16";
   if (x_dtype != y_dtype && x_dtype != IG_DT_F32) return "the result of 16-bit rows has their type";
@@ -42,6 +42,7 @@ static const char *bad_norm_args(int32_t x_dtype, int32_t y_dtype, int64_t rows,
   if ((weight || bias) && !wes) return "dtype must be float32, bfloat16 or float16";
   if (wes && ((reinterpret_cast<uintptr_t>(weight) | reinterpret_cast<uintptr_t>(bias)) % wes))
     return "weight or bias not aligned to its element size";
+  if ((reinterpret_cast<uintptr_t>(mean) | reinterpret_cast<uintptr_t>(rstd)) & 3) return "mean or rstd not aligned to 4 bytes";
   return nullptr;
 }
 
@@ -71,7 +72,7 @@ int ig_layer_norm(const void *x, int32_t x_dtype, int64_t ldx, int64_t rows, int
                   const void *bias, int32_t weight_dtype, double eps, void *y, int32_t y_dtype, int64_t ldy, float *mean,
                   float *rstd, void *stream) {
   t_last_error.clear();
-  const char *m = bad_norm_args(x_dtype, y_dtype, rows, n, weight, bias, weight_dtype);
+  const char *m = bad_norm_args(x_dtype, y_dtype, rows, n, weight, bias, weight_dtype, mean, rstd);
   const int ex = vocab_elem_size(x_dtype), ey = vocab_elem_size(y_dtype);
   if (!m && (!(eps >= 0.0) || !std::isfinite((float)eps))) m = "eps must be finite and not negative";
   if (!m) m = bad_matrix(x, rows, n, ldx, ex);
@@ -101,7 +102,7 @@ int ig_layer_norm_backward(const void *dy, int32_t y_dtype, int64_t lddy, const 
                            const float *rstd, void *dx, int64_t lddx, void *dweight, void *dbias, void *workspace,
                            int64_t workspace_bytes, void *stream) {
   t_last_error.clear();
-  const char *m = bad_norm_args(x_dtype, y_dtype, rows, n, weight, nullptr, weight_dtype);
+  const char *m = bad_norm_args(x_dtype, y_dtype, rows, n, weight, nullptr, weight_dtype, mean, rstd);
   const int ex = vocab_elem_size(x_dtype), ey = vocab_elem_size(y_dtype), ew = vocab_elem_size(weight_dtype);
   const bool sums = dweight || dbias;
   if (!m && sums && !ew) m = "dtype must be float32, bfloat16 or float16";
