@@ -7,6 +7,7 @@ operators through, and links torch. Run ``python -m indecis_b200.build`` or call
 """
 from __future__ import annotations
 
+import importlib.metadata
 import importlib.util
 import os
 import subprocess
@@ -18,6 +19,7 @@ ROOT = os.path.dirname(HERE)
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libindecis_b200.so")
 TORCH_OPS = os.path.join(HERE, "_torch_ops.so")  # the training operators' calls from Python (torch_ops.cpp)
+TORCH_OPS_STAMP = os.path.join(HERE, "_build", "torch_ops.txt")  # the torch and Python it was built for
 SOURCES = ["libindecis_b200.cu", "adamw.cu", "spans.cpp", "batcher.cpp"]
 HEADERS = ["common.cuh", "exactmath.cuh", "internal.h", "gemm_i8.cu", "gemm_persist.cu", "gemm_pair.cu", "rows_fast.cu", "rows.cu", "rows_ln.cu", "attention.cu", "attention_tc.cu", "attention_short.cu", "siglip.cu", "encoder_f32.cu", "capi.cu", "multi.cu", "siglip_capi.cu", "spans_device.cu", "noalloc.cu", "selfcheck.cu",
            "vocab_rows.cu", "vocab_gemm.cu", "vocab_capi.cu", "train.h", "layer_norm.cu", "gated_ff.cu", "train_capi.cu"]
@@ -43,6 +45,19 @@ def _stale(target: str, deps: list[str]) -> bool:
         return True
     t = os.path.getmtime(target)
     return any(os.path.getmtime(d) > t for d in deps)
+
+
+def _torch_and_python() -> str:
+    return f"torch {importlib.metadata.version('torch')}, {sysconfig.get_config_var('SOABI')}"
+
+
+def _torch_ops_stale() -> bool:
+    if _stale(TORCH_OPS, [os.path.join(CSRC, "torch_ops.cpp"), os.path.join(ROOT, "include", "indecis_b200.h")]):
+        return True
+    if not os.path.exists(TORCH_OPS_STAMP):
+        return True
+    with open(TORCH_OPS_STAMP) as f:
+        return f.read() != _torch_and_python()
 
 
 def _torch_ops_command() -> list[str]:
@@ -80,11 +95,13 @@ def build(verbose: bool = False, force: bool = False, extra: list[str] | None = 
         if verbose:
             print(" ".join(cmd), flush=True)
         subprocess.run(cmd, check=True)
-    if force or _stale(TORCH_OPS, [os.path.join(CSRC, "torch_ops.cpp"), os.path.join(ROOT, "include", "indecis_b200.h")]):
+    if force or _torch_ops_stale():
         cmd = _torch_ops_command()
         if verbose:
             print(" ".join(cmd), flush=True)
         subprocess.run(cmd, check=True)
+        with open(TORCH_OPS_STAMP, "w") as f:
+            f.write(_torch_and_python())
     return LIB
 
 
