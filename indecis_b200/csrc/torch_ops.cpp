@@ -103,6 +103,11 @@ at::Tensor scratch(const Matrix &x, int64_t bytes) {
 }
 void *address(const at::Tensor &t) { return t.defined() ? t.data_ptr() : nullptr; }
 
+// Autograd notices that what it may have kept is another value now.
+void written(const at::Tensor &t) {
+  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
 struct On {  // x's device current, and its current stream
   c10::cuda::CUDAGuard guard;
   void *stream;
@@ -168,6 +173,7 @@ PyObject *layer_norm(PyObject *const *a) {
   const On on(*x.t);
   check(ig_layer_norm(x.p, x.type, x.ld, x.rows, narrow(x.cols), w, b, wt < 0 ? IG_DT_F32 : wt, eps, y.data_ptr(), type, ldy,
                       static_cast<float *>(mean.data_ptr()), static_cast<float *>(rstd.data_ptr()), on.stream));
+  if (a[5] != Py_None) written(y);
   return tuple(y, mean, rstd);
 }
 
@@ -197,6 +203,7 @@ PyObject *layer_norm_backward(PyObject *const *a) {
   ws = scratch(x, bytes);
   check(ig_layer_norm_backward(dy.p, dy.type, dy.ld, x.p, x.type, x.ld, x.rows, narrow(x.cols), w, wt, mean, rstd, dx.data_ptr(), ldo,
                                address(dw), address(db), address(ws), bytes, on.stream));
+  if (a[7] != Py_None) written(dx);
   return tuple(dx, dw, db);
 }
 

@@ -1,0 +1,45 @@
+"""Calls of the training operators beside torch's own autograd, with lists that have gaps, and with values at the ends of
+their ranges."""
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+F32, BF16, F16 = torch.float32, torch.bfloat16, torch.float16
+
+
+def randn(*shape, seed=0, dtype=F32):
+    return torch.randn(shape, generator=torch.Generator(device="cuda").manual_seed(seed), device="cuda").to(dtype)
+
+
+@pytest.mark.parametrize("of", ["y", "dx"])
+def test_written_in_place_is_seen_by_autograd(igdev, of):
+    """A graph that keeps a tensor refuses to go on once a call wrote over it, as with torch's own in-place operations."""
+    from indecis_b200 import layers
+    leaf = randn(5, 64, seed=1).requires_grad_()
+    kept = leaf * 1.0
+    z = (kept * kept).sum()
+    r = layers.layer_norm(kept.detach().clone())
+    if of == "y":
+        layers.layer_norm(kept, out=kept)
+    else:
+        layers.layer_norm_backward(kept, randn(5, 64, seed=2), r.mean, r.rstd, out=kept)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        z.backward()
+
+
+def test_results_of_their_own_raise_no_version(igdev):
+    from indecis_b200 import layers
+    x, dy = randn(5, 64, seed=1), randn(5, 64, seed=2)
+    r = layers.layer_norm(x)
+    layers.layer_norm_backward(dy, x, r.mean, r.rstd)
+    assert x._version == 0 and dy._version == 1 - 1
+    with torch.inference_mode():  # tensors without a version
+        y = torch.empty(5, 64, device="cuda")
+        layers.layer_norm(x, out=y)
+        layers.layer_norm_backward(dy, x, r.mean, r.rstd, out=y)
+    with pytest.raises((RuntimeError, ValueError)):
+        layers.layer_norm(x, eps=-1.0, out=dy)
+    assert dy._version == 0  # refused: as it was
