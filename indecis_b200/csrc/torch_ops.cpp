@@ -353,9 +353,6 @@ PyObject *adamw_step(PyObject *const *a) {
       if (t != IG_DT_BF16 && t != IG_DT_F16) throw BadValue{"copies: expected bfloat16 or float16"};
       ct.push_back((uint8_t)t);
     }
-    // Autograd notices that what it may have kept is another value now.
-    if (!param.is_inference()) param.unsafeGetTensorImpl()->bump_version();
-    if (copying && !THPVariable_Unpack(copies[i]).is_inference()) THPVariable_Unpack(copies[i]).unsafeGetTensorImpl()->bump_version();
     wd.push_back((float)number(one_decay ? a[9] : decays[i], "weight_decay"));
   }
   ig_adamw_tensors t{};
@@ -377,6 +374,11 @@ PyObject *adamw_step(PyObject *const *a) {
   const On on(step);
   check(ig_adamw_step(&t, bits8 ? 8 : 32, number(a[5], "lr"), number(a[6], "beta1"), number(a[7], "beta2"), number(a[8], "eps"),
                       static_cast<int32_t *>(step.data_ptr()), gs, skip, on.stream));
+  for (Py_ssize_t i = 0; i < n; i++) {
+    if (grads[i] == Py_None) continue;
+    written(THPVariable_Unpack(params[i]));
+    if (copying) written(THPVariable_Unpack(copies[i]));
+  }
   Py_RETURN_NONE;
 }
 

@@ -43,3 +43,24 @@ def test_results_of_their_own_raise_no_version(igdev):
     with pytest.raises((RuntimeError, ValueError)):
         layers.layer_norm(x, eps=-1.0, out=dy)
     assert dy._version == 0  # refused: as it was
+
+
+def test_refused_step_raises_no_version(igdev):
+    """Only a step that was made changes parameters and copies for autograd."""
+    from indecis_b200 import _capi, optim
+    p = [randn(40, seed=i) for i in range(3)]
+    copies = [t.bfloat16() for t in p]
+    g = [randn(40, seed=10 + i) for i in range(3)]
+    m, v = ([torch.zeros(40, device="cuda") for _ in p] for _ in range(2))
+    step = torch.zeros(1, dtype=torch.int32, device="cuda")
+    before = [t._version for t in p + copies]
+    for grads, moments, kw in ((g, m, dict(lr=-1.0)), (g, m, dict(betas=(0.9, 1.0))), (g[:2] + [g[2][:39]], m, {}),
+                               (g, m[:2] + [m[2].double()], {}), (g, m[:2] + [m[0]], {}), (g, m, dict(weight_decay=[0.0, 0.0, -1.0])),
+                               (g, m, dict(skip=step))):
+        with pytest.raises((ValueError, _capi.IgError)):
+            optim.adamw_step(p, grads, moments, v, step, copies=copies, **kw)
+        assert [t._version for t in p + copies] == before
+    optim.adamw_step(p, g, m, v, step, copies=copies)
+    assert [t._version for t in p + copies] == [k + 1 for k in before]
+    optim.adamw_step(p, [g[0], None, g[2]], m, v, step, copies=copies)
+    assert [t._version for t in p + copies] == [k + 1 + (i % 3 != 1) for i, k in enumerate(before)]
