@@ -323,7 +323,9 @@ PyObject *adamw_step(PyObject *const *a) {
   std::vector<uint8_t> pt, gt, ct;
   std::vector<float> wd;
   size.reserve(n), p.reserve(n), m.reserve(n), v.reserve(n), g.reserve(n), pt.reserve(n), gt.reserve(n), wd.reserve(n);
-  const bool bits8 = n > 0 && !THPVariable_Check(ms[0]);
+  Py_ssize_t used = 0;  // the first tensor that takes part says how the moments are held
+  while (used < n && grads[used] == Py_None) used++;
+  const bool bits8 = used < n && !THPVariable_Check(ms[used]);
   for (Py_ssize_t i = 0; i < n; i++) {
     if (grads[i] == Py_None) continue;  // left out
     const at::Tensor &param = tensor(params[i], "params");

@@ -47,7 +47,7 @@ def adamw_step(params, grads, exp_avg, exp_avg_sq, step, lr=1e-3, betas=(0.9, 0.
     parameters, or None. grad_scale, skip: float32, one value each: the factor of
     every gradient, and where not 0 nothing changes (an overflow found elsewhere).
     No two tensors that are written may share memory. A gradient that is None
-    leaves its tensor out."""
+    leaves its tensor out (its moments may be None too)."""
     _torch_ops.adamw_step(params, grads, exp_avg, exp_avg_sq, step, lr, betas[0], betas[1], eps, weight_decay, copies, grad_scale,
                           skip)
 

@@ -64,3 +64,31 @@ def test_refused_step_raises_no_version(igdev):
     assert [t._version for t in p + copies] == [k + 1 for k in before]
     optim.adamw_step(p, [g[0], None, g[2]], m, v, step, copies=copies)
     assert [t._version for t in p + copies] == [k + 1 + (i % 3 != 1) for i, k in enumerate(before)]
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("gap", [0, 1, 2])
+def test_moments_of_tensors_that_are_left_out(igdev, bits, gap):
+    """A tensor without a gradient needs no moments, wherever it stands in the lists."""
+    from indecis_b200 import optim
+    p, q = ([randn(300, seed=i) for i in range(3)] for _ in range(2))
+    g = [randn(300, seed=10 + i) for i in range(3)]
+    moments = lambda: [None if i == gap else optim.new_moment(p[i], bits) for i in range(3)]  # noqa: E731
+    step = torch.zeros(1, dtype=torch.int32, device="cuda")
+    optim.adamw_step(p, [None if i == gap else g[i] for i in range(3)], moments(), moments(), step)
+    rest = [i for i in range(3) if i != gap]
+    full = [optim.new_moment(q[i], bits) for i in rest], [optim.new_moment(q[i], bits) for i in rest]
+    optim.adamw_step([q[i] for i in rest], [g[i] for i in rest], *full, torch.zeros(1, dtype=torch.int32, device="cuda"))
+    assert int(step) == 1 and all(torch.equal(a, b) for a, b in zip(p, q))
+    assert all(not torch.equal(p[i], randn(300, seed=i)) for i in rest)
+
+
+def test_moments_of_one_width(igdev):
+    from indecis_b200 import optim
+    p = [randn(300, seed=i) for i in range(2)]
+    mixed = lambda first: [optim.new_moment(t, b) for t, b in zip(p, (first, 40 - first))]  # noqa: E731
+    step = torch.zeros(1, dtype=torch.int32, device="cuda")
+    for first in (8, 32):
+        with pytest.raises(ValueError):
+            optim.adamw_step(p, [torch.ones_like(t) for t in p], mixed(first), mixed(first), step)
+    assert int(step) == 0
