@@ -92,3 +92,36 @@ def test_moments_of_one_width(igdev):
         with pytest.raises(ValueError):
             optim.adamw_step(p, [torch.ones_like(t) for t in p], mixed(first), mixed(first), step)
     assert int(step) == 0
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("offset", [0, 1])  # whole blocks on boundaries of four, and single elements
+@pytest.mark.parametrize("lr,decay", [(1e-5, 0.01), (1e-6, 0.01), (3e-6, 0.1)])
+def test_small_decay(igdev, bits, offset, lr, decay):
+    """The decay takes lr * decay of a parameter in the mean over many, however far that is below a step of float32, beside
+    updates that differ from element to element: between runs with and without it the parameters differ by that. p in
+    [0.5, 1) is stored to 2^-25 at most off, so is each run's result, evenly spread by the updates: both together leave
+    a deviation of 2^-25 * sqrt(2 / 3) / sqrt(n) of the mean, of which six are allowed, and 2^-22 of it for the
+    roundings of lr * decay and of the terms."""
+    from indecis_b200 import optim
+    n = (1 << 20) + offset
+    g = torch.Generator(device="cuda").manual_seed(3)
+    p = (torch.rand(n, generator=g, device="cuda") * 0.5 + 0.5)[offset:]
+    grad, m = (torch.randn(n, generator=g, device="cuda")[offset:] for _ in range(2))
+    v = (torch.rand(n, generator=g, device="cuda") + 0.1)[offset:]
+
+    def moved(decay):
+        q = torch.empty(n, device="cuda")[offset:].copy_(p)
+        step = torch.full((1,), 10, dtype=torch.int32, device="cuda")
+        if bits == 32:
+            a, b = [torch.empty(n, device="cuda")[offset:].copy_(t) for t in (m, v)]
+        else:
+            a, b = optim.new_moment(q, 8), optim.new_moment(q, 8)
+            for k, t in ((a, m), (b, v.sqrt())):
+                k.scales.fill_(4.0 / 448)
+                k.codes.copy_((t.clamp(-4, 4) * (448 / 4)).to(torch.float8_e4m3fn))
+        optim.adamw_step([q], [grad], [a], [b], step, lr=lr, betas=(0.9, 0.99), weight_decay=decay)
+        return q.double()
+    want = lr * decay * float(p.double().mean())
+    got = float((moved(0.0) - moved(decay)).mean())
+    assert abs(got - want) <= 6 * 2.0 ** -25 * math.sqrt(2 / 3 / (1 << 20)) + 2.0 ** -22 * want, (got / want)
