@@ -78,7 +78,8 @@ __device__ __forceinline__ void ff_act(float2 a, float2 &f, [[maybe_unused]] flo
     const float2 s = ff_rcp(__fadd2_rn(ff_ex2(ff_mul(a, ff_fma(a2, ff_both(-2 * k * c * log2e), ff_both(-2 * k * log2e)))), ff_both(1.0f)));
     f = ff_mul(a, s);
     if constexpr (GRAD) {
-      const float2 u1 = ff_fma(a2, ff_both(6 * k * c), ff_both(2 * k));  // d(2 u)
+      // d(2 u), which what is past float32 would make infinite beside a factor of 0: far before that f or rest is 0.
+      const float2 u1 = ff_fma(make_float2(fminf(a2.x, 1e30f), fminf(a2.y, 1e30f)), ff_both(6 * k * c), ff_both(2 * k));
       const float2 rest = ff_fma(s, ff_both(-1.0f), ff_both(1.0f));
       df = ff_fma(ff_mul(f, rest), u1, s);
     }

@@ -125,3 +125,17 @@ def test_small_decay(igdev, bits, offset, lr, decay):
     want = lr * decay * float(p.double().mean())
     got = float((moved(0.0) - moved(decay)).mean())
     assert abs(got - want) <= 6 * 2.0 ** -25 * math.sqrt(2 / 3 / (1 << 20)) + 2.0 ** -22 * want, (got / want)
+
+
+@pytest.mark.parametrize("kind", ["gelu", "gelu_tanh", "silu"])
+def test_activation_of_the_largest_values(igdev, kind):
+    """act(a) is a or 0 and act'(a) 1 or 0 for any finite a far from 0, those whose square is past float32 among them."""
+    from indecis_b200 import layers
+    top = 2.0 ** torch.arange(40, 128, device="cuda", dtype=torch.float64)
+    a = torch.cat([top, -top, torch.tensor([torch.finfo(BF16).max, -torch.finfo(BF16).max], device="cuda", dtype=torch.float64)]).to(BF16)
+    x = torch.stack([a, torch.ones_like(a)], 1)
+    w_in, w_out = torch.eye(2, device="cuda", dtype=BF16), torch.ones(1, 1, device="cuda", dtype=BF16)
+    y, saved = layers.gated_ff(x, w_in, w_out, kind, save=True)
+    assert torch.equal(y[:, 0], a.clamp(min=0.0))
+    dx, _, _ = layers.gated_ff_backward(torch.ones_like(y), x, w_in, w_out, saved, kind, need_in=False, need_out=False)
+    assert torch.equal(dx[:, 0], (a > 0).to(BF16))
