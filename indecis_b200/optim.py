@@ -15,6 +15,7 @@ from ._capi import torch_ops as _torch_ops
 
 BLOCK = 256  # elements of a tensor that share a scale in 8 bits
 
+
 class Moment8(NamedTuple):
     """A tensor's moment in 8 bits: codes times the scale of their 256 elements."""
     codes: torch.Tensor   # float8_e4m3fn, the parameter's shape
@@ -24,6 +25,9 @@ class Moment8(NamedTuple):
         """The moment (exp_avg), or the root of it (exp_avg_sq), in float32."""
         n = self.codes.numel()
         return (self.codes.float().reshape(-1) * self.scales.repeat_interleave(BLOCK)[:n]).view(self.codes.shape)
+
+
+torch.serialization.add_safe_globals([Moment8])  # torch.load takes a saved state_dict as it comes
 
 
 def new_moment(param, bits=32):

@@ -139,3 +139,18 @@ def test_activation_of_the_largest_values(igdev, kind):
     assert torch.equal(y[:, 0], a.clamp(min=0.0))
     dx, _, _ = layers.gated_ff_backward(torch.ones_like(y), x, w_in, w_out, saved, kind, need_in=False, need_out=False)
     assert torch.equal(dx[:, 0], (a > 0).to(BF16))
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_state_goes_through_a_file(igdev, tmp_path, bits):
+    """torch.save and torch.load as they come (weights_only), into moments on the GPU again."""
+    from indecis_b200 import optim
+    a, b = [randn(700, seed=1)], [randn(700, seed=1)]
+    one, two = optim.AdamW(a, bits=bits), optim.AdamW(b, bits=bits)
+    one.step([randn(700, seed=2)])
+    torch.save(one.state_dict(), tmp_path / "state.pt")
+    b[0].copy_(a[0])
+    two.load_state_dict(torch.load(tmp_path / "state.pt", map_location="cpu"))
+    one.step([randn(700, seed=3)])
+    two.step([randn(700, seed=3)])
+    assert int(two.steps) == 2 and torch.equal(a[0], b[0])
