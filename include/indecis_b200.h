@@ -480,6 +480,11 @@ IG_API int64_t ig_gated_ff_saved(int64_t rows, int32_t inner);
  * it (256-byte aligned); calls that share one must not overlap on the GPU. */
 IG_API int64_t ig_gated_ff_workspace(int64_t rows, int32_t hidden, int32_t inner, int32_t out_size, int32_t unaligned,
                                      int32_t pass);
+/* How calls of these sizes are cut on the current device (for tests of each
+ * cut): cut[0] the tile of h (pass 2: of [da | db]) and cut[1] that of the
+ * products, 0 a warp per weight row, 1 128 x 64 on a CTA, 2 256 x 256 on a pair;
+ * cut[2..4] the parts of K of y, or of dw_in, dw_out and dx. */
+IG_API int ig_check_gated_ff(int64_t rows, int32_t hidden, int32_t inner, int32_t out_size, int32_t pass, int32_t *cut);
 IG_API int ig_gated_ff(const void *x, int64_t ldx, const void *w_in, int64_t ldi, const void *w_out, int64_t ldw,
                        int32_t dtype, int64_t rows, int32_t hidden, int32_t inner, int32_t out_size, int32_t activation,
                        void *y, int64_t ldy, void *saved, void *workspace, int64_t workspace_bytes, void *stream);

@@ -37,7 +37,7 @@ SYMBOLS = ["ig_model_create", "ig_model_destroy", "ig_model_set_heads", "ig_enco
            "ig_profile_only", "ig_check_wait_timeout", "ig_token_logprobs", "ig_token_logprobs_backward",
            "ig_distill_topk", "ig_vocab_workspace", "ig_vocab_logprobs", "ig_vocab_logprobs_backward",
            "ig_layer_norm", "ig_layer_norm_workspace", "ig_layer_norm_backward", "ig_adamw_step",
-           "ig_gated_ff_saved", "ig_gated_ff_workspace", "ig_gated_ff", "ig_gated_ff_backward"]
+           "ig_gated_ff_saved", "ig_gated_ff_workspace", "ig_gated_ff", "ig_gated_ff_backward", "ig_check_gated_ff"]
 
 IG_EMB_F32 = 0
 IG_EMB_BF16 = 1
@@ -240,6 +240,7 @@ def load() -> C.CDLL:
     L.ig_gated_ff_saved.restype = i64
     L.ig_gated_ff_workspace.argtypes = [i64, i32, i32, i32, i32, i32]
     L.ig_gated_ff_workspace.restype = i64
+    L.ig_check_gated_ff.argtypes = [i64, i32, i32, i32, i32, i32p]
     L.ig_gated_ff.argtypes = [vp, i64, vp, i64, vp, i64, i32, i64, i32, i32, i32, i32, vp, i64, vp, vp, i64, vp]
     L.ig_gated_ff_backward.argtypes = [vp, i64, vp, i64, vp, i64, vp, i64, i32, i64, i32, i32, i32, i32, vp, vp, i64, vp, i64,
                                        vp, i64, vp, i64, vp]

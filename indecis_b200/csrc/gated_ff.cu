@@ -1089,19 +1089,25 @@ static int ff_add(FfMaps &maps, FfArgs &f, const FfTile &t, const FfMatrix &A, b
   return 0;
 }
 
-// h (and a, b), or [da | db], of the rows.
-template <int EPI>
-static int ff_inner(const FfMatrix &a, const FfMatrix &w, const FfSizes &s, int dtype, int act, void *out, int64_t ldo, float4 *z,
-                    cudaStream_t st) {
+// Whether h's products (grad: dh's) take the small tile: less estimated time, whole rounds of tiles.
+static bool ff_inner_small(const FfSizes &s, bool grad) {
   // h's tiles take twice its columns.
-  const FfShapeOf n{s.rows, s.I, EPI == kFfForward ? s.H : s.O}, cost{s.rows, EPI == kFfForward ? 2 * (int64_t)s.I : s.I, n.K};
+  const FfShapeOf cost{s.rows, grad ? s.I : 2 * (int64_t)s.I, grad ? s.O : s.H};
   double time[2];
   for (int small = 0; small < 2; small++) {
     const FfTile &t = small ? kFfSmall : kFfLarge;
     time[small] = (double)ff_div(ff_div(cost.M, 128 * t.cg) * ff_div(cost.N, t.bn), num_sms() / t.cg) *
-                  (ff_div(n.K, kVBK) * t.block + t.tile);
+                  (ff_div(cost.K, kVBK) * t.block + t.tile);
   }
-  const bool small = time[1] < time[0];
+  return time[1] < time[0];
+}
+
+// h (and a, b), or [da | db], of the rows.
+template <int EPI>
+static int ff_inner(const FfMatrix &a, const FfMatrix &w, const FfSizes &s, int dtype, int act, void *out, int64_t ldo, float4 *z,
+                    cudaStream_t st) {
+  const FfShapeOf n{s.rows, s.I, EPI == kFfForward ? s.H : s.O};
+  const bool small = ff_inner_small(s, EPI == kFfGrad);
   const FfTile &t = small ? kFfSmall : kFfLarge;
   FfMaps maps;
   FfArgs f;

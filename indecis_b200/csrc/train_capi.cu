@@ -159,6 +159,20 @@ int64_t ig_gated_ff_workspace(int64_t rows, int32_t hidden, int32_t inner, int32
   return (int64_t)ff_bytes(s, ff_plan(s, pass == 2), pass);
 }
 
+int ig_check_gated_ff(int64_t rows, int32_t hidden, int32_t inner, int32_t out_size, int32_t pass, int32_t *cut) {
+  t_last_error.clear();
+  const char *m = bad_gated_args(IG_DT_BF16, rows, hidden, inner, out_size, IG_ACT_GELU);
+  if (!m && (rows == 0 || pass < 0 || pass > 2 || !cut)) m = "no rows, no such pass or null argument";
+  if (m) return fail(IG_ERR_BAD_ARG, std::string("ig_check_gated_ff: ") + m);
+  const FfSizes s{rows, hidden, inner, out_size, 0};
+  const FfPlan p = ff_plan(s, pass == 2);
+  const bool few = ff_few(s, pass > 0);
+  cut[0] = few ? 0 : ff_inner_small(s, pass == 2) ? 1 : 2;
+  cut[1] = few ? 0 : p.cut.small ? 1 : 2;
+  for (int i = 0; i < kFfProblems; i++) cut[2 + i] = few || (pass < 2 && i > 0) ? 0 : p.cut.parts[i];
+  return 0;
+}
+
 int ig_gated_ff(const void *x, int64_t ldx, const void *w_in, int64_t ldi, const void *w_out, int64_t ldw, int32_t dtype,
                 int64_t rows, int32_t hidden, int32_t inner, int32_t out_size, int32_t activation, void *y, int64_t ldy,
                 void *saved, void *workspace, int64_t workspace_bytes, void *stream) {
