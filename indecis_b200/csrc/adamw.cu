@@ -186,6 +186,31 @@ __device__ __forceinline__ void adamw_codes(float (&x)[4], float inv, uint32_t k
   }
 }
 
+// Square roots: s = v y of an approximate y = 1 / sqrt(v), and Newton's step on
+// v - s^2, which one multiply-add forms exactly, with y for the slope (Markstein,
+// 1990). From v = 2^-102 on they are those to the nearest (compared for every
+// float), so that codes of a root are those of its definition; below, where v -
+// s^2 is rounded, the last place may be another. 0, infinities and NaN make s a
+// NaN, and denormal v too: there the approximate root does. 312 million
+// parameters in 8 bits: 1,018 us; 995 with the approximate root, off by 2^-23,
+// everywhere, which moved one code in 3.2 million and with it the next step; 1,125 with
+// the function for the root to the nearest.
+__device__ __forceinline__ float2 adamw_root(float2 v) {
+  float2 y;
+  asm("rsqrt.approx.ftz.f32 %0, %1;" : "=f"(y.x) : "f"(v.x));
+  asm("rsqrt.approx.ftz.f32 %0, %1;" : "=f"(y.y) : "f"(v.y));
+  const float2 s = __fmul2_rn(v, y), d = __ffma2_rn(make_float2(-s.x, -s.y), s, v);
+  float2 r = __ffma2_rn(d, __fmul2_rn(y, make_float2(0.5f, 0.5f)), s);
+  const float any = r.x + r.y;
+  if (any != any) {
+    float2 q;
+    asm("sqrt.approx.f32 %0, %1;" : "=f"(q.x) : "f"(v.x));
+    asm("sqrt.approx.f32 %0, %1;" : "=f"(q.y) : "f"(v.y));
+    r = make_float2(r.x == r.x ? r.x : q.x, r.y == r.y ? r.y : q.y);
+  }
+  return r;
+}
+
 // What a step needs beside the tensors.
 struct AdamwNow {
   float c1, c2, gs;  // -lr / (1 - b1^t), 1 / sqrt(1 - b2^t), the gradients' factor
@@ -196,8 +221,6 @@ struct AdamwNow {
 // decay is -lr times the tensor's. It joins the update before that meets p: 1 -
 // lr decay is off by up to 2^-25 in float32, to the same side for every element
 // and step (1e-5 times 0.01: 19% more decay, 1e-6 times 0.01: none).
-// The root is off by 2^-23 of itself at most (312 million parameters: 995 us;
-// 1,126 with it rounded to the nearest, 10 instructions more an element).
 template <bool BITS8>
 __device__ __forceinline__ void adamw_two(float2 &p, float2 g, float2 &m, float2 &v, float ms, float vs, float decay, const AdamwArgs &a,
                                           const AdamwNow &n) {
@@ -210,9 +233,8 @@ __device__ __forceinline__ void adamw_two(float2 &p, float2 g, float2 &m, float2
   }
   m = __fadd2_rn(adamw_mul(m, both(a.b1), a.zero), adamw_mul(g, both(a.ob1), a.zero));
   v = __fadd2_rn(adamw_mul(v, both(a.b2), a.zero), adamw_mul(__fmul2_rn(g, g), both(a.ob2), a.zero));
-  float2 r, q;
-  asm("sqrt.approx.f32 %0, %1;" : "=f"(r.x) : "f"(v.x));
-  asm("sqrt.approx.f32 %0, %1;" : "=f"(r.y) : "f"(v.y));
+  const float2 r = adamw_root(v);
+  float2 q;
   const float2 d = __ffma2_rn(r, both(n.c2), both(a.eps));
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(q.x) : "f"(d.x));
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(q.y) : "f"(d.y));
