@@ -532,7 +532,9 @@ typedef struct ig_adamw_tensors {
  * reaches 1 - u: u = frac of a Weyl sequence of element and step, so that the
  * codes follow the moments in the mean. A root above 0 keeps the smallest code
  * at least; a moment that is not finite becomes NaN. 32-bit arithmetic on the
- * decoded values; p uses the moments before they are rounded.
+ * decoded values; p uses the moments before they are rounded. The decay joins
+ * the update first, so that lr weight_decay below a step of float32 still takes
+ * its part in the mean (and an infinite parameter becomes NaN).
  * A parameter in 16 bits is rounded to the nearest once a step. eps >= 2^-126. */
 IG_API int ig_adamw_step(const ig_adamw_tensors *tensors, int32_t state_bits, double lr, double beta1, double beta2, double eps,
                          int32_t *step, const float *grad_scale, const float *skip, void *stream);

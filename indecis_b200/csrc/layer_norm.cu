@@ -334,7 +334,7 @@ constexpr int kLnGroupsMost = 20; // rows side by side in a CTA
 // way (persistent CTAs). BULK: the next a.ring rows of every group are on their
 // way into shared memory, by one copy each of x and dy. Without, for rows off
 // 16-byte boundaries: one row ahead in registers.
-// 16384 x 768 bf16: 21 us with 96 threads a row and 8 elements each; 37 with
+// 16384 x 768 bf16: 21 us; 25 with 96 threads a row and 8 elements each, 37 with
 // the rows copied 16 bytes a thread (cp.async).
 template <int TX, int TY, int V, int KV, int MAXT, bool BULK>
 __global__ void __launch_bounds__(MAXT) ln_bwd_kernel(const LnGradArgs a) {

@@ -57,7 +57,12 @@ def gated_ff(x, w_in, w_out, activation="gelu", save=False):
     """The gated feed-forward block (act(a) * b) @ w_out.T with [a | b] = x @
     w_in.T: x [rows, hidden], w_in [2 * inner, hidden] (the activated rows
     first), w_out [out, inner], all bfloat16 or all float16. activation: "gelu",
-    "gelu_tanh" or "silu". save=True: (y, what gated_ff_backward needs)."""
+    "gelu_tanh" or "silu". save=True: (y, what gated_ff_backward needs).
+
+    act(a) * b is rounded to the operands' type before the second product. One
+    row, or up to four where the weights are few, keeps it in float32 unless save
+    is asked for, so that its y may differ in the last place from the same row's
+    in a larger call."""
     r = _torch_ops.gated_ff(x, w_in, w_out, _activation(activation), bool(save))
     return r if save else r[0]
 
