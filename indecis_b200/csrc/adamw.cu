@@ -193,8 +193,9 @@ __device__ __forceinline__ void adamw_codes(float (&x)[4], float inv, uint32_t k
 // s^2 is rounded, the last place may be another. 0, infinities and NaN make s a
 // NaN, and denormal v too: there the approximate root does. 312 million
 // parameters in 8 bits: 1,018 us; 995 with the approximate root, off by 2^-23,
-// everywhere, which moved one code in 3.2 million and with it the next step; 1,125 with
-// the function for the root to the nearest.
+// everywhere, which moved one code in 3.2 million and with it the next step;
+// 1,125 with the function for the root to the nearest. 200 million: 559 us, 643
+// where all roots are 0 (549 and 598 with the approximate root).
 __device__ __forceinline__ float2 adamw_root(float2 v) {
   float2 y;
   asm("rsqrt.approx.ftz.f32 %0, %1;" : "=f"(y.x) : "f"(v.x));
